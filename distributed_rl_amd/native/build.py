@@ -25,8 +25,10 @@ HOST_SO = os.path.join(HERE, "libdrl_host.so")
 HIP_SO = os.path.join(HERE, "libdrl_hip.so")
 ARCH = "gfx950"
 
+# -packed-fp32-ops: no v_pk_{add,mul,fma}_f32, which the compiler otherwise forms by itself from ordinary float code and some
+# of whose forms have given wrong results now and then (the host pass does not know the feature and warns: harmless).
 HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=%s" % ARCH, "-ffast-math",
-               "-Wno-unused-result", "-munsafe-fp-atomics"]
+               "-Wno-unused-result", "-munsafe-fp-atomics", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 # The loss / priority / optimizer arithmetic (TD targets with the value rescale and its inverse, Huber, IS weights, the
 # clip coefficient, RMSprop / Adam) is compiled WITHOUT -ffast-math: IEEE division and square root, no reassociation. These
 # kernels are latency- or HBM-bound, so it costs nothing; the MFMA kernels keep it (their scalar code is address arithmetic
