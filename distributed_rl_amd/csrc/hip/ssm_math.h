@@ -1,0 +1,42 @@
+// Scalar math of the state-space operators (ssm.hip, short_conv.hip): 32-bit throughout, rounded to the tensors' type by the
+// caller, once, at a store.
+#pragma once
+#include "common.h"
+
+#define LOG2E 1.4426950408889634f
+#define LOG2E_LO 1.9259629911266175e-8f   // log2(e) - LOG2E
+#define LN2 0.6931471805599453f
+
+__device__ __forceinline__ float ld(const float* p) { return *p; }
+__device__ __forceinline__ float ld(const bf16_t* p) { return bf2f(*p); }
+__device__ __forceinline__ void st(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
+
+// exp(-|x|) by the hardware's 2^y: the part of x * log2(e) that its 24 bits lose comes back as a factor 1 + lost * ln 2
+// (without it the relative error grows with |x|: 4e-7 at 7, where a step size of 0.001 sits)
+__device__ __forceinline__ float exp_neg_abs(float x) {
+    const float ax = -fabsf(x), hi = ax * LOG2E;
+    const float lo = fmaf(ax, LOG2E, -hi) + ax * LOG2E_LO;
+    const float p = __builtin_amdgcn_exp2f(hi);
+    return fmaf(p, lo * LN2, p);
+}
+// log(1 + e) for 0 <= e <= 1 as 2 atanh(s), s = e / (2 + e) <= 1/3: s + s^3/3 + s^5/5 + ... to s^15 (next term < 2e-9 of
+// the sum). log(1 + e) itself would keep none of a small e's bits.
+__device__ __forceinline__ float log1p_unit(float e) {
+    const float s = e * __builtin_amdgcn_rcpf(2.0f + e), q = s * s;
+    float p = 1.0f / 15.0f;
+    p = fmaf(p, q, 1.0f / 13.0f);
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    return 2.0f * fmaf(s * q, p, s);
+}
+__device__ __forceinline__ float softplus_from(float x, float e) { return fmaxf(x, 0.f) + log1p_unit(e); }
+// 1 / (1 + exp(-x)), e = exp(-|x|)
+__device__ __forceinline__ float sigmoid_from(float x, float e) {
+    const float r = __builtin_amdgcn_rcpf(1.0f + e);
+    return x >= 0.f ? r : e * r;
+}
+__device__ __forceinline__ float sigmoidf(float x) { return sigmoid_from(x, exp_neg_abs(x)); }

@@ -33,7 +33,8 @@ HIPCC_FLAGS = ["-O3", "-std=c++17", "-fPIC", "--offload-arch=%s" % ARCH, "-ffast
 # clip coefficient, RMSprop / Adam) is compiled WITHOUT -ffast-math: IEEE division and square root, no reassociation. These
 # kernels are latency- or HBM-bound, so it costs nothing; the MFMA kernels keep it (their scalar code is address arithmetic
 # and epilogue scaling). Where a kernel wants an approximate transcendental it says so (__powf, __expf).
-PRECISE = {"td.hip", "optim.hip", "head.hip"}
+# The state-space operators are compared with 64-bit results at a few 1e-7 and compute log1p by hand: no reassociation there either.
+PRECISE = {"td.hip", "optim.hip", "head.hip", "ssm.hip", "short_conv.hip", "layer_norm.hip"}
 
 
 def flags_for(src: str) -> List[str]:

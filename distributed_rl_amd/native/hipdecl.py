@@ -1,5 +1,5 @@
 """ctypes signatures of libdrl_hip.so (csrc/hip/*.hip). Every entry point returns a hipError_t-style int."""
-from ctypes import c_double, c_float, c_int, c_longlong, c_ulonglong, c_void_p, POINTER
+from ctypes import c_char_p, c_double, c_float, c_int, c_longlong, c_ulonglong, c_void_p, POINTER
 
 P, I, L, F, U = c_void_p, c_int, c_longlong, c_float, c_ulonglong
 LP = POINTER(c_longlong)
@@ -98,6 +98,18 @@ SIGS = {
     "drl_lstm_set_spin_limit": [I],
     # gemm_big.hip
     "drl_gemm_big": [I, I, P, L, P, L, I, I, I, P, L, P, P, L, I, P, P, P, P, P, P],
+    # ssm.hip, short_conv.hip, layer_norm.hip: the arguments travel as one packed record (ops/hip.py)
+    "drl_ssm_ws": [L, L, L, L, I, LP],
+    "drl_ssm_fwd": [c_char_p, I, P],
+    "drl_ssm_bwd": [c_char_p, I, P],
+    "drl_ssm_step": [c_char_p, I, P],
+    "drl_short_conv_ws": [L, L, L, L, LP],
+    "drl_short_conv_fwd": [c_char_p, I, P],
+    "drl_short_conv_bwd": [c_char_p, I, P],
+    "drl_short_conv_step": [c_char_p, I, P],
+    "drl_norm_ws": [L, L, LP],
+    "drl_norm_fwd": [c_char_p, I, F, P],
+    "drl_norm_bwd": [c_char_p, I, P],
     "drl_xar_set_timeout": [P, c_double],
     "drl_xar_destroy": [P],
 }

@@ -186,6 +186,59 @@ def lstm_unroll(xg: torch.Tensor, w_hh: torch.Tensor, h0: torch.Tensor, c0: torc
 
 
 # --------------------------------------------------------------------------------------------
+# state-space recurrent core (time-major; the semantics of ops.hip.layer_norm_* / short_conv_* / ssm_*; autograd gives the
+# gradients). Padding (steps from lengths[b] on) is never read: its outputs are zero and it leaves the states alone.
+# --------------------------------------------------------------------------------------------
+def layer_norm(x: torch.Tensor, w: torch.Tensor, b: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    c = x - x.mean(-1, keepdim=True)
+    y = c * torch.rsqrt(c.square().mean(-1, keepdim=True) + eps) * w
+    return y if b is None else y + b
+
+
+def short_conv(x: torch.Tensor, w: torch.Tensor, bias: Optional[torch.Tensor] = None, state: Optional[torch.Tensor] = None,
+               reset: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+               silu: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """x (T,B,D), w (D,W), state (B,W-1,D) = the inputs before step 0 -> y (T,B,D), state after every row's last step."""
+    T, B, D = x.shape
+    W = w.shape[1]
+    state = x.new_zeros(B, W - 1, D) if state is None else state
+    ys = []
+    for t in range(T):
+        live = torch.ones(B, 1, 1, dtype=torch.bool, device=x.device) if lengths is None else (t < lengths).view(B, 1, 1)
+        old = state if reset is None else torch.where((live[:, :, 0] & (reset[t] != 0)[:, None])[..., None], 0.0, state)
+        rows = torch.cat([old, torch.where(live, x[t][:, None], 0.0)], 1)
+        y = (rows * w.t()).sum(1)
+        y = y if bias is None else y + bias
+        y = F.silu(y) if silu else y
+        ys.append(torch.where(live[:, 0], y, 0.0))
+        state = torch.where(live, rows[:, 1:], state)
+    return torch.stack(ys), state
+
+
+def ssm_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tensor, Cm: torch.Tensor, D: Optional[torch.Tensor] = None,
+             z: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, h0: Optional[torch.Tensor] = None,
+             reset: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+             softplus: bool = True) -> Tuple[torch.Tensor, torch.Tensor]:
+    """u, dt, z (T,B,D), A (D,N), Bm, Cm (T,B,N), h0 (B,D,N) -> y (T,B,D), hT (B,D,N):
+    s = softplus(dt + dt_bias), h = exp(s A) h + s u Bm, y = (sum_n Cm h + D u) silu(z)."""
+    T, B, Dc = u.shape
+    h = u.new_zeros(B, Dc, A.shape[1]) if h0 is None else h0
+    ys = []
+    for t in range(T):
+        live = torch.ones(B, 1, dtype=torch.bool, device=u.device) if lengths is None else (t < lengths)[:, None]
+        ut, st, Bt, Ct = (torch.where(live, v[t], 0.0) for v in (u, dt, Bm, Cm))
+        st = st if dt_bias is None else st + dt_bias
+        st = F.softplus(st, threshold=1e9) if softplus else st
+        old = h if reset is None else torch.where((reset[t] != 0)[:, None, None], 0.0, h)
+        h = torch.where(live[..., None], torch.exp(st[..., None] * A) * old + (st * ut)[..., None] * Bt[:, None], h)
+        y = (h * Ct[:, None]).sum(-1)
+        y = y if D is None else y + D * ut
+        y = y if z is None else y * F.silu(torch.where(live, z[t], 0.0))
+        ys.append(torch.where(live, y, 0.0))
+    return torch.stack(ys), h
+
+
+# --------------------------------------------------------------------------------------------
 # optimizers with fused global-norm clip   (learner.py:77-78; learner_node.py:28,40)
 # --------------------------------------------------------------------------------------------
 def clip_coef(grad_flat: torch.Tensor, max_norm: float) -> torch.Tensor:

@@ -1,0 +1,156 @@
+"""State-space operators on the CPU: the oracle against the formulas written out, its gradients against differences, cut
+sequences against whole ones, and what the entry points of the kernels refuse before anything is launched."""
+import pytest
+import torch
+
+import ssm_ref
+from distributed_rl_amd.ops import hip, oracle
+
+
+def rnd(g, *shape, scale=1.0):
+    return torch.randn(*shape, generator=g, dtype=torch.float64) * scale
+
+
+def scan_inputs(T, B, D, N, seed=0, grads=True):
+    g = torch.Generator().manual_seed(seed)
+    v = dict(u=rnd(g, T, B, D), dt=rnd(g, T, B, D, scale=0.5) - 2, A=-torch.rand(D, N, generator=g, dtype=torch.float64) * 3 - 0.1,
+             Bm=rnd(g, T, B, N), Cm=rnd(g, T, B, N), D=rnd(g, D), z=rnd(g, T, B, D), dt_bias=rnd(g, D, scale=0.2), h0=rnd(g, B, D, N),
+             reset=(torch.rand(T, B, generator=g) < 0.2).to(torch.uint8),
+             lengths=torch.randint(0, T + 1, (B,), generator=g).to(torch.int32))
+    if grads:
+        v.update(dy=rnd(g, T, B, D), dhT=rnd(g, B, D, N))
+    return v
+
+
+SCAN_KEYS = ("u", "dt", "A", "Bm", "Cm", "D", "z", "dt_bias", "h0")
+
+
+@pytest.mark.parametrize("softplus", [True, False])
+@pytest.mark.parametrize("T,B,D,N", [(1, 1, 1, 1), (7, 4, 3, 5), (19, 3, 2, 4)])
+def test_scan_oracle_and_its_gradients_are_the_formulas(T, B, D, N, softplus):
+    v = scan_inputs(T, B, D, N)
+    p = {k: v[k].clone().requires_grad_() for k in SCAN_KEYS}
+    y, hT = oracle.ssm_scan(**p, reset=v["reset"], lengths=v["lengths"], softplus=softplus)
+    ((y * v["dy"]).sum() + (hT * v["dhT"]).sum()).backward()
+    ref = ssm_ref.scan(v, softplus=softplus)
+    torch.testing.assert_close(y, ref["y"], rtol=1e-12, atol=1e-12)
+    torch.testing.assert_close(hT, ref["hT"], rtol=1e-12, atol=1e-12)
+    for k, r in dict(u="du", dt="ddt", A="dA", Bm="dB", Cm="dC", D="dD", z="dz", dt_bias="ddt_bias", h0="dh0").items():
+        torch.testing.assert_close(p[k].grad, ref[r], rtol=1e-11, atol=1e-11, msg=lambda s, k=k: "%s: %s" % (k, s))
+
+
+def test_scan_gradients_against_differences():
+    v = scan_inputs(6, 3, 2, 3, seed=5)
+    p = [v[k].clone().requires_grad_() for k in SCAN_KEYS]
+    assert torch.autograd.gradcheck(lambda *a: oracle.ssm_scan(**dict(zip(SCAN_KEYS, a)), reset=v["reset"], lengths=v["lengths"]), p)
+
+
+def test_scan_in_pieces_is_the_whole_scan():
+    v = scan_inputs(17, 3, 4, 5, seed=2, grads=False)
+    v["lengths"] = None
+    y, hT = oracle.ssm_scan(**v)
+    cut = lambda a, b: {k: (x[a:b] if k in ("u", "dt", "Bm", "Cm", "z", "reset") else x) for k, x in v.items()}     # noqa: E731
+    y1, h = oracle.ssm_scan(**cut(0, 5))
+    y2, h = oracle.ssm_scan(**{**cut(5, 17), "h0": h})
+    torch.testing.assert_close(torch.cat([y1, y2]), y, rtol=1e-13, atol=1e-13)
+    torch.testing.assert_close(h, hT, rtol=1e-13, atol=1e-13)
+
+
+def conv_inputs(T, B, D, W, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    return dict(x=rnd(g, T, B, D), w=rnd(g, D, W), bias=rnd(g, D), state_in=rnd(g, B, W - 1, D), dy=rnd(g, T, B, D),
+                dstate_out=rnd(g, B, W - 1, D), reset=(torch.rand(T, B, generator=g) < 0.25).to(torch.uint8),
+                lengths=torch.randint(0, T + 1, (B,), generator=g).to(torch.int32))
+
+
+@pytest.mark.parametrize("silu", [True, False])
+@pytest.mark.parametrize("T,B,D,W", [(1, 2, 3, 4), (2, 5, 1, 3), (23, 4, 3, 2), (40, 6, 2, 4)])
+def test_conv_oracle_and_its_gradients_are_the_formulas(T, B, D, W, silu):
+    v = conv_inputs(T, B, D, W)
+    p = {k: v[k].clone().requires_grad_() for k in ("x", "w", "bias", "state_in")}
+    y, st = oracle.short_conv(p["x"], p["w"], p["bias"], p["state_in"], v["reset"], v["lengths"], silu)
+    ((y * v["dy"]).sum() + (st * v["dstate_out"]).sum()).backward()
+    ref = ssm_ref.conv(v, silu)
+    for got, k in ((y, "y"), (st, "state_out"), (p["x"].grad, "dx"), (p["w"].grad, "dw"), (p["bias"].grad, "db"), (p["state_in"].grad, "dstate_in")):
+        torch.testing.assert_close(got, ref[k], rtol=1e-12, atol=1e-12, msg=lambda s, k=k: "%s: %s" % (k, s))
+
+
+def test_conv_gradients_against_differences():
+    v = conv_inputs(6, 3, 2, 3, seed=3)
+    p = [v[k].clone().requires_grad_() for k in ("x", "w", "bias", "state_in")]
+    assert torch.autograd.gradcheck(lambda x, w, b, s: oracle.short_conv(x, w, b, s, v["reset"], v["lengths"]), p)
+
+
+def test_norm_oracle_and_its_gradients_are_the_formulas():
+    g = torch.Generator().manual_seed(0)
+    v = dict(x=rnd(g, 5, 7) * 2 + 3, w=rnd(g, 7), b=rnd(g, 7), dy=rnd(g, 5, 7))
+    p = [v[k].clone().requires_grad_() for k in ("x", "w", "b")]
+    y = oracle.layer_norm(*p)
+    (y * v["dy"]).sum().backward()
+    ref = ssm_ref.norm(v)
+    for got, k in ((y, "y"), (p[0].grad, "dx"), (p[1].grad, "dw"), (p[2].grad, "db")):
+        torch.testing.assert_close(got, ref[k], rtol=1e-12, atol=1e-12)
+    assert torch.autograd.gradcheck(lambda x, w, b: oracle.layer_norm(x, w, b), p)
+
+
+# ---- refusals: raised on the host, before the library is touched ---------------------------------------------------------
+def test_cpu_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    with pytest.raises(TypeError):
+        hip.layer_norm_fwd(x, w, w, torch.empty_like(x))
+    with pytest.raises(TypeError):
+        hip.short_conv_fwd(x[None], torch.zeros(8, 4), w, torch.empty(1, 4, 8))
+    with pytest.raises(TypeError):
+        hip.short_conv_step(x, torch.zeros(8, 4), w, torch.zeros(4, 3, 8), torch.empty_like(x))
+    h = torch.zeros(4, 8, 2)
+    with pytest.raises(TypeError):
+        hip.ssm_step(x, x.clone(), torch.zeros(8, 2), torch.zeros(4, 2), torch.zeros(4, 2), h, torch.empty_like(x))
+    with pytest.raises(TypeError):
+        hip.ssm_scan_fwd(x[None], x[None], torch.zeros(8, 2), torch.zeros(1, 4, 2), torch.zeros(1, 4, 2), torch.empty(1, 4, 8), torch.empty(0))
+
+
+@pytest.mark.parametrize("T,B,D,N", [(0, 1, 8, 4), (3, 0, 8, 4), (3, 70000, 1, 1), (3, 1, 8, 65), (3, 1, 8, 0)])
+def test_sizes_are_refused(T, B, D, N):
+    u, bc = torch.empty(T, B, D), torch.empty(T, B, N)
+    with pytest.raises(ValueError):
+        hip.ssm_scan_fwd(u, u, torch.empty(D, N), bc, bc, u.clone(), torch.empty(0))
+    with pytest.raises(ValueError):
+        hip.short_conv_fwd(u, torch.empty(D, 5 if N else 1), None, u.clone())
+    with pytest.raises(ValueError):
+        hip.layer_norm_fwd(torch.empty(T * 0, 16385), torch.empty(16385), None, torch.empty(0, 16385))
+
+
+def test_missing_tensors_are_refused():
+    x, w = torch.zeros(4, 8), torch.ones(8)
+    with pytest.raises(ValueError, match="w is needed"):
+        hip.layer_norm_fwd(x, None, w, x.clone())
+    with pytest.raises(ValueError, match="A is needed"):
+        hip.ssm_step(x, x, None, x[:, :2], x[:, :2], torch.zeros(4, 8, 2), x.clone())
+    with pytest.raises(ValueError, match="both or neither"):
+        hip.layer_norm_fwd(x, w, w, x.clone(), mean=torch.zeros(4))
+    with pytest.raises(ValueError, match="eps"):
+        hip.layer_norm_fwd(x, w, w, x.clone(), eps=float("nan"))
+    u = torch.zeros(2, 4, 8)
+    bc = torch.zeros(2, 4, 2)
+    with pytest.raises(ValueError, match="z and dz"):
+        hip.ssm_scan_bwd(u, u, u, torch.zeros(8, 2), bc, bc, torch.zeros(1, 4, 8, 2), u, u, torch.zeros(8, 2), bc, bc, torch.zeros(1), z=u)
+    with pytest.raises(ValueError, match="without"):
+        hip.ssm_scan_bwd(u, u, u, torch.zeros(8, 2), bc, bc, torch.zeros(1, 4, 8, 2), u, u, torch.zeros(8, 2), bc, bc, torch.zeros(1), dD=w)
+
+
+def test_rows_of_outputs_may_not_overlap():
+    t = torch.zeros(64)
+    cpu = torch.device("cpu")
+    assert hip._rows(t.as_strided((2, 3, 4), (32, 8, 1)), (2, 3, 4), torch.float32, cpu, "y", True)[1:] == (32, 8)
+    assert hip._rows(t.as_strided((2, 3, 4), (4, 16, 1)), (2, 3, 4), torch.float32, cpu, "y", True)[1:] == (4, 16)
+    assert hip._rows(t.as_strided((2, 3, 4), (0, 0, 1)), (2, 3, 4), torch.float32, cpu, "x")[1:] == (0, 0)
+    for st in ((0, 4, 1), (4, 4, 1), (8, 4, 1), (12, 3, 1), (2, 8, 1)):
+        with pytest.raises(ValueError, match="overlap"):
+            hip._rows(t.as_strided((2, 3, 4), st), (2, 3, 4), torch.float32, cpu, "y", True)
+    with pytest.raises(ValueError, match="contiguous"):
+        hip._rows(t.as_strided((2, 3, 4), (24, 8, 2)), (2, 3, 4), torch.float32, cpu, "x")
+    with pytest.raises(ValueError, match="shares"):
+        hip._apart((8, 0, 16), (16, 24))
+    with pytest.raises(ValueError, match="shares"):
+        hip._apart((8, 8), ())
+    hip._apart((8, 16, 0, 0), (0, 24))

@@ -1,0 +1,513 @@
+"""The state-space kernels against the formulas in 64 bits (ssm_ref): sizes that divide nothing, episode resets, padding full
+of NaN, strided views, both types, missing options, cut sequences, single steps, streams and graphs."""
+import pytest
+import torch
+
+import ssm_ref
+from distributed_rl_amd.ops import hip as H
+from distributed_rl_amd.ops import oracle
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    H.native.hip()
+
+
+class Gen:
+    def __init__(self, seed):
+        self.g = torch.Generator().manual_seed(seed)
+
+    def n(self, *shape, dtype=F32, scale=1.0, shift=0.0):
+        return (torch.randn(*shape, generator=self.g) * scale + shift).to(dtype).to(DEV)
+
+    def u(self, *shape):
+        return torch.rand(*shape, generator=self.g).to(DEV)
+
+
+def like(*ts):
+    """Outputs full of NaN: what is not written shows."""
+    return [torch.full(t.shape, float("nan"), dtype=t.dtype, device=t.device) for t in ts]
+
+
+# ---- layer norm ---------------------------------------------------------------------------------------------------------
+def run_norm(v, eps=1e-5):
+    (y, dx), mean, rstd = like(v["x"], v["x"]), torch.empty(len(v["x"]), device=DEV), torch.empty(len(v["x"]), device=DEV)
+    dw, db = like(v["w"], v["w"])
+    H.layer_norm_fwd(v["x"], v["w"], v["b"], y, mean=mean, rstd=rstd, eps=eps)
+    H.layer_norm_bwd(v["dy"], v["x"], v["w"], mean, rstd, dx, dw, db if v["b"] is not None else None, H.layer_norm_ws(*v["x"].shape, DEV))
+    out = dict(y=y, dx=dx, mean=mean, rstd=rstd, dw=dw)
+    return dict(out, db=db) if v["b"] is not None else out
+
+
+def check_norm(v, eps=1e-5):
+    got = run_norm(v, eps)
+    w = ssm_ref.f64(v)
+    ref, mag = ssm_ref.norm(w, eps), ssm_ref.norm(w, eps, mag=True)
+    # a sum over a row: at most 64 terms in one register, then a tree of at most 2^10 of them: 74 roundings; three such
+    # sums stand behind dx, and 16 single operations. The sums over rows add at most one rounding for each row.
+    for k in got:
+        ssm_ref.close(got[k], ref[k], mag[k], 3 * 74 + 16 + (len(v["x"]) if k in ("dw", "db") else 0), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("M,D", [(1, 1), (3, 2), (1, 512), (5, 63), (4, 64), (7, 100), (257, 8), (33, 513), (9, 1024), (6, 1032), (5, 3136),
+                                 (2, 4099), (3, 8192), (2, 16384), (1030, 40)])
+def test_norm(M, D, dtype):
+    g = Gen(M * 31 + D)
+    check_norm(dict(x=g.n(M, D, dtype=dtype, scale=2.0, shift=0.7), w=g.n(D, shift=1.0), b=g.n(D), dy=g.n(M, D, dtype=dtype)))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_norm_strided_rows_without_bias_far_from_zero(dtype):
+    g = Gen(3)
+    wide = g.n(21, 3 * 96 + 5, dtype=dtype, shift=30.0)
+    check_norm(dict(x=wide[:, 3:99], w=g.n(96), b=None, dy=g.n(96, 21, dtype=dtype).t().contiguous()))
+    check_norm(dict(x=wide[:, 8:104], w=g.n(96), b=g.n(96), dy=wide[:, 104:200]))
+    row = g.n(1, 96, dtype=dtype)
+    check_norm(dict(x=row.expand(5, 96), w=g.n(96), b=None, dy=row.expand(5, 96)))
+
+
+def test_norm_constant_rows_and_one_column():
+    g = Gen(4)
+    check_norm(dict(x=torch.full((3, 40), 2.5, device=DEV), w=g.n(40), b=g.n(40), dy=g.n(3, 40)))
+    check_norm(dict(x=g.n(4, 1), w=g.n(1), b=g.n(1), dy=g.n(4, 1)))
+
+
+# ---- short convolution --------------------------------------------------------------------------------------------------
+def conv_case(T, B, D, W, dtype, seed=0, reset=0.2, ragged=True, state=True, bias=True, dstate=True, nan=True):
+    g = Gen(seed + T * 7 + B * 3 + D + W)
+    v = dict(x=g.n(T, B, D, dtype=dtype), w=g.n(D, W, scale=0.6), bias=g.n(D, scale=0.3) if bias else None,
+             state_in=g.n(B, W - 1, D, dtype=dtype) if state else None, dy=g.n(T, B, D, dtype=dtype),
+             dstate_out=g.n(B, W - 1, D, dtype=dtype) if dstate else None,
+             reset=(g.u(T, B) < reset).to(torch.uint8) if reset else None, lengths=None)
+    if ragged:
+        n = (g.u(B) * (T + 1)).int().clamp(max=T)
+        n[:1], n[1:2] = T, 0
+        v["lengths"] = n
+        if nan:
+            dead = torch.arange(T, device=DEV)[:, None] >= n[None]
+            v["x"][dead] = float("nan")
+            v["dy"][dead] = float("inf")
+    return v
+
+
+def run_conv(v, silu=True):
+    T, B, D = v["x"].shape
+    W = v["w"].shape[1]
+    y, dx = (torch.full((T, B, D), float("nan"), dtype=v["x"].dtype, device=DEV) for _ in range(2))
+    so, dsi = (torch.full((B, W - 1, D), float("nan"), dtype=v["x"].dtype, device=DEV) for _ in range(2))
+    dw, db = like(v["w"], v["w"][:, 0])
+    H.short_conv_fwd(v["x"], v["w"], v["bias"], y, state_in=v["state_in"], state_out=so, reset=v["reset"], lengths=v["lengths"], silu=silu)
+    H.short_conv_bwd(v["dy"], v["x"], v["w"], v["bias"], dx, dw, db if v["bias"] is not None else None, H.short_conv_ws(T, B, D, W, DEV),
+                     state_in=v["state_in"], dstate_in=dsi, dstate_out=v["dstate_out"], reset=v["reset"], lengths=v["lengths"], silu=silu)
+    out = dict(y=y, state_out=so, dx=dx, dw=dw, dstate_in=dsi)
+    return dict(out, db=db) if v["bias"] is not None else out
+
+
+def check_conv(v, silu=True):
+    got = run_conv(v, silu)
+    w = ssm_ref.f64(v)
+    w["x"], w["dy"] = torch.nan_to_num(w["x"], 0, 0, 0), torch.nan_to_num(w["dy"], 0, 0, 0)
+    ref, mag = ssm_ref.conv(w, silu), ssm_ref.conv(w, silu, mag=True)
+    T, B, _ = v["x"].shape
+    for k in got:    # W + 1 terms, 16 roundings of the sigmoid and its products, W more sums; one for every summed step
+        ssm_ref.close(got[k], ref[k], mag[k], 32 + (T * B if k in ("dw", "db") else 0), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("T,B,D,W", [(1, 1, 1, 4), (1, 3, 5, 2), (2, 4, 64, 4), (3, 2, 16, 4), (15, 3, 7, 3), (16, 2, 256, 4), (17, 5, 8, 4),
+                                     (31, 3, 130, 2), (33, 2, 264, 3), (65, 4, 40, 4)])
+def test_conv(T, B, D, W, dtype):
+    check_conv(conv_case(T, B, D, W, dtype))
+
+
+@pytest.mark.parametrize("kw", [dict(reset=0), dict(reset=1.0), dict(ragged=False), dict(state=False, dstate=False), dict(bias=False),
+                                dict(reset=0, ragged=False, state=False, bias=False, dstate=False)])
+def test_conv_options(kw):
+    check_conv(conv_case(37, 4, 24, 4, F32, **kw))
+    check_conv(conv_case(37, 4, 24, 3, BF, **kw), silu=False)
+
+
+def test_conv_of_views():
+    v = conv_case(20, 3, 48, 4, BF, ragged=False)
+    g = Gen(9)
+    wide = g.n(3, 20, 2 * 48, dtype=BF)
+    v["x"], v["dy"] = wide.transpose(0, 1)[..., :48], wide.transpose(0, 1)[..., 48:]
+    check_conv(v)
+    odd = g.n(20, 3, 101, dtype=BF)
+    v["x"], v["dy"] = odd[..., 1:49], odd[..., 52:100]
+    check_conv(v)
+    a = run_conv(v)
+    buf = torch.full((20, 3, 96), 7.0, dtype=BF, device=DEV)          # an output that is a slice: the rest stays
+    H.short_conv_fwd(v["x"], v["w"], v["bias"], buf[..., 48:], state_in=v["state_in"], reset=v["reset"])
+    assert torch.equal(buf[..., 48:], a["y"]) and bool((buf[..., :48] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+def test_conv_in_pieces_and_in_steps_is_the_whole(dtype):
+    v = conv_case(24, 3, 40, 4, dtype, ragged=False)
+    whole = run_conv(v)
+    st = v["state_in"].clone()
+    for a, b in ((0, 1), (1, 3), (3, 20), (20, 24)):
+        y, so = like(v["x"][a:b], st)
+        H.short_conv_fwd(v["x"][a:b], v["w"], v["bias"], y, state_in=st, state_out=so, reset=v["reset"][a:b])
+        assert torch.equal(y, whole["y"][a:b])
+        st = so
+    assert torch.equal(st, whole["state_out"])
+    st = v["state_in"].clone()
+    for t in range(24):
+        y, = like(v["x"][0])
+        H.short_conv_step(v["x"][t], v["w"], v["bias"], st, y, reset=v["reset"][t])
+        assert torch.equal(y, whole["y"][t])
+    assert torch.equal(st, whole["state_out"])
+
+
+@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (5, 33, 3), (3, 1024, 4), (257, 40, 4)])
+def test_conv_step_strided(B, D, W):
+    g = Gen(B + D)
+    wide = g.n(B, 2 * D + 3, dtype=BF)
+    x, w, st = wide[:, 1:D + 1], g.n(D, W), g.n(B, W - 1, D, dtype=BF)
+    y, ref = torch.empty(B, D, dtype=BF, device=DEV), st.clone()
+    yr, = like(y[None])
+    H.short_conv_fwd(x[None], w, None, yr, state_in=ref, silu=False)
+    H.short_conv_step(x, w, None, st, y, silu=False)
+    assert torch.equal(y, yr[0]) and torch.equal(st, torch.cat([ref[:, 1:], x[:, None]], 1))
+
+
+# ---- selective scan -----------------------------------------------------------------------------------------------------
+def scan_case(T, B, D, N, dtype, seed=0, reset=0.1, ragged=True, opt=True, shift=-2.0, scale=0.7):
+    g = Gen(seed + T * 5 + B * 3 + D + N)
+    v = dict(u=g.n(T, B, D, dtype=dtype), dt=g.n(T, B, D, dtype=dtype, scale=scale, shift=shift), A=-g.u(D, N) * 2 - 0.05,
+             Bm=g.n(T, B, N, dtype=dtype), Cm=g.n(T, B, N, dtype=dtype), dy=g.n(T, B, D, dtype=dtype),
+             reset=(g.u(T, B) < reset).to(torch.uint8) if reset else None, lengths=None)
+    for k, t in (("D", g.n(D)), ("z", g.n(T, B, D, dtype=dtype)), ("dt_bias", g.n(D, scale=0.3)), ("h0", g.n(B, D, N)), ("dhT", g.n(B, D, N))):
+        v[k] = t if opt is True or opt and k in opt else None
+    if ragged:
+        n = (g.u(B) * (T + 1)).int().clamp(max=T)
+        n[:1], n[1:2], n[2:3] = T, 0, 1
+        v["lengths"] = n
+        dead = torch.arange(T, device=DEV)[:, None] >= n[None]
+        for k, bad in (("u", "nan"), ("dt", "nan"), ("Bm", "inf"), ("Cm", "nan"), ("dy", "inf"), ("z", "nan")):
+            if v[k] is not None:
+                v[k][dead] = float(bad)
+    return v
+
+
+def run_scan(v, softplus=True, ws=None):
+    T, B, D = v["u"].shape
+    N = v["A"].shape[1]
+    typ = v["u"].dtype
+    nan = lambda *s, t=F32: torch.full(s, float("nan"), dtype=t, device=DEV)        # noqa: E731
+    o = dict(y=nan(T, B, D, t=typ), hT=nan(B, D, N), du=nan(T, B, D, t=typ), ddt=nan(T, B, D, t=typ), dB=nan(T, B, N, t=typ),
+             dC=nan(T, B, N, t=typ), dA=nan(D, N), dh0=nan(B, D, N))
+    if v["z"] is not None:
+        o["dz"] = nan(T, B, D, t=typ)
+    if v["D"] is not None:
+        o["dD"] = nan(D)
+    if v["dt_bias"] is not None:
+        o["ddt_bias"] = nan(D)
+    ws = H.ssm_scan_ws(T, B, D, N, DEV).fill_(float("nan")) if ws is None else ws
+    ckpt = H.ssm_scan_ckpt(T, B, D, N, DEV).fill_(float("nan"))
+    kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], reset=v["reset"], lengths=v["lengths"], softplus=softplus)
+    H.ssm_scan_fwd(v["u"], v["dt"], v["A"], v["Bm"], v["Cm"], o["y"], ws, h0=v["h0"], hT=o["hT"], ckpt=ckpt, **kw)
+    H.ssm_scan_bwd(v["dy"], v["u"], v["dt"], v["A"], v["Bm"], v["Cm"], ckpt, o["du"], o["ddt"], o["dA"], o["dB"], o["dC"], ws,
+                   dD=o.get("dD"), dz=o.get("dz"), ddt_bias=o.get("ddt_bias"), dhT=v["dhT"], dh0=o["dh0"], **kw)
+    return o
+
+
+def clean(v):
+    return {k: (torch.nan_to_num(x, 0, 0, 0) if torch.is_tensor(x) and x.dtype == torch.float64 else x) for k, x in ssm_ref.f64(v).items()}
+
+
+def check_scan(v, softplus=True):
+    got = run_scan(v, softplus)
+    w = clean(v)
+    ref, mag = ssm_ref.scan(w, softplus), ssm_ref.scan(w, softplus, mag=True)
+    for k in got:
+        ssm_ref.close(got[k], ref[k], mag[k], ssm_ref.scan_roundings(w, k not in ("y", "hT"), softplus), k)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("T,B,D,N", [(1, 1, 1, 1), (1, 3, 17, 16), (2, 4, 16, 4), (15, 3, 33, 5), (16, 3, 64, 16), (17, 4, 20, 8), (33, 3, 65, 16),
+                                     (40, 2, 130, 9), (50, 3, 24, 17), (20, 3, 40, 32), (37, 2, 18, 33), (35, 3, 70, 64), (70, 5, 96, 16)])
+def test_scan(T, B, D, N, dtype):
+    check_scan(scan_case(T, B, D, N, dtype))
+
+
+@pytest.mark.parametrize("kw", [dict(reset=0), dict(reset=1.0), dict(ragged=False), dict(opt=False), dict(opt=("z",)), dict(opt=("D",)),
+                                dict(opt=("dt_bias", "h0")), dict(reset=0, ragged=False, opt=False)])
+@pytest.mark.parametrize("N", [6, 16, 40])
+def test_scan_options(kw, N):
+    check_scan(scan_case(37, 4, 24, N, F32, **kw))
+    check_scan(scan_case(21, 4, 24, N, BF, **kw))
+
+
+def test_scan_step_sizes_as_given_and_extreme_ones():
+    check_scan(scan_case(19, 3, 20, 16, F32, shift=0.3, scale=0.2), softplus=False)             # growing and shrinking states
+    check_scan(scan_case(9, 3, 20, 16, F32, shift=15.0, scale=8.0))                             # decays down to nothing
+    check_scan(scan_case(9, 3, 20, 16, F32, shift=-60.0, scale=20.0))                           # steps down to nothing
+    v = scan_case(20, 3, 20, 16, F32)
+    v["A"].zero_()                                                                              # a plain sum
+    check_scan(v)
+
+
+def test_scan_rows_without_a_step():
+    v = scan_case(20, 3, 20, 16, F32, ragged=False)
+    v["lengths"] = torch.zeros(3, dtype=torch.int32, device=DEV)
+    got = run_scan(v)
+    assert torch.equal(got["hT"], v["h0"]) and torch.equal(got["dh0"], v["dhT"])
+    for k in ("y", "du", "ddt", "dz", "dB", "dC", "dA", "dD", "ddt_bias"):
+        assert bool((got[k] == 0).all()), k
+    v["lengths"] = torch.tensor([100, -5, 20], dtype=torch.int32, device=DEV)                   # beyond the batch: cut to it
+    a = run_scan(v)
+    v["lengths"] = torch.tensor([20, 0, 20], dtype=torch.int32, device=DEV)
+    b = run_scan(v)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+@pytest.mark.parametrize("T,B,D,N,dtype", [(300, 1, 16, 16, F32), (523, 1, 40, 8, BF), (1100, 2, 17, 5, F32), (260, 1, 64, 40, F32)])
+def test_scan_long_and_few_rows(T, B, D, N, dtype):
+    check_scan(scan_case(T, B, D, N, dtype, reset=0.004, shift=-4.0, scale=0.3))
+    check_scan(scan_case(T, B, D, N, dtype, reset=0, ragged=False, shift=-4.0, scale=0.3))
+
+
+def test_scan_of_views():
+    g = Gen(11)
+    T, B, D, N = 25, 3, 40, 16
+    v = scan_case(T, B, D, N, BF, ragged=False)
+    xz, bc = g.n(B, T, 2 * D + 1, dtype=BF).transpose(0, 1), g.n(T, B, 7 + 2 * N, dtype=BF)
+    v.update(u=xz[..., 1:D + 1], z=xz[..., D + 1:], Bm=bc[..., 7:7 + N], Cm=bc[..., 7 + N:], dy=g.n(T, 1, D, dtype=BF).expand(T, B, D))
+    check_scan(v)
+    a = run_scan(v)
+    dxz, dbc = torch.full((T, B, 2 * D), 7.0, dtype=BF, device=DEV), torch.full((B, T, 3 * N), 7.0, dtype=BF, device=DEV).transpose(0, 1)
+    ws, ckpt = H.ssm_scan_ws(T, B, D, N, DEV), H.ssm_scan_ckpt(T, B, D, N, DEV)
+    kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], reset=v["reset"])
+    H.ssm_scan_fwd(v["u"], v["dt"], v["A"], v["Bm"], v["Cm"], dxz[..., :D], ws, h0=v["h0"], ckpt=ckpt, **kw)
+    assert torch.equal(dxz[..., :D], a["y"]) and bool((dxz[..., D:] == 7).all())
+    ddt, dA = torch.empty(T, B, D, dtype=BF, device=DEV), torch.empty(D, N, device=DEV)
+    H.ssm_scan_bwd(v["dy"], v["u"], v["dt"], v["A"], v["Bm"], v["Cm"], ckpt, dxz[..., :D], ddt, dA, dbc[..., :N], dbc[..., N:2 * N], ws,
+                   dz=dxz[..., D:], dhT=v["dhT"], **kw)
+    for k, t in (("du", dxz[..., :D]), ("dz", dxz[..., D:]), ("ddt", ddt), ("dA", dA), ("dB", dbc[..., :N]), ("dC", dbc[..., N:2 * N])):
+        assert torch.equal(t, a[k]), k
+    assert bool((dbc[..., 2 * N:] == 7).all())
+
+
+def test_scan_in_pieces_is_the_whole():
+    """Burn-in and training window as two calls, the state carried over; and every step by itself."""
+    v = scan_case(56, 3, 48, 16, F32, ragged=False)
+    w = clean(v)
+    ref, mag = ssm_ref.scan(w), ssm_ref.scan(w, mag=True)
+    n = ssm_ref.scan_roundings(w, False)
+    h, ys = v["h0"], []
+    for a, b in ((0, 1), (1, 24), (24, 56)):
+        y, hT = torch.empty_like(v["u"][a:b]), torch.empty_like(h)
+        H.ssm_scan_fwd(*(v[k][a:b] if k != "A" else v[k] for k in ("u", "dt", "A", "Bm", "Cm")), y, H.ssm_scan_ws(b - a, 3, 48, 16, DEV, train=False),
+                       D=v["D"], z=v["z"][a:b], dt_bias=v["dt_bias"], h0=h, hT=hT, reset=v["reset"][a:b])
+        h = hT
+        ys.append(y)
+    ssm_ref.close(torch.cat(ys), ref["y"], mag["y"], n, "y")
+    ssm_ref.close(h, ref["hT"], mag["hT"], n, "hT")
+    h, ys = v["h0"].clone(), []
+    for t in range(56):
+        ys.append(torch.empty_like(v["u"][0]))
+        H.ssm_step(v["u"][t], v["dt"][t], v["A"], v["Bm"][t], v["Cm"][t], h, ys[-1], D=v["D"], z=v["z"][t], dt_bias=v["dt_bias"], reset=v["reset"][t])
+    ssm_ref.close(torch.stack(ys), ref["y"], mag["y"], n, "y by steps")
+    ssm_ref.close(h, ref["hT"], mag["hT"], n, "h by steps")
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("B,D,N", [(1, 1, 1), (3, 17, 16), (5, 64, 4), (2, 100, 8), (7, 33, 5), (4, 70, 32), (3, 40, 64), (2, 9, 47), (130, 40, 16)])
+def test_step(B, D, N, dtype):
+    v = scan_case(1, B, D, N, dtype, ragged=False, reset=0.3)
+    for opt in (True, False):
+        if not opt:
+            v.update(D=None, z=None, dt_bias=None, reset=None)
+        w = clean({k: x for k, x in v.items() if k not in ("dy", "dhT")})
+        ref, mag = ssm_ref.scan(w), ssm_ref.scan(w, mag=True)
+        h, y = v["h0"].clone(), torch.full((B, D), float("nan"), dtype=dtype, device=DEV)
+        sl = lambda k: v[k][0] if v[k] is not None else None                        # noqa: E731
+        H.ssm_step(sl("u"), sl("dt"), v["A"], sl("Bm"), sl("Cm"), h, y, D=v["D"], z=sl("z"), dt_bias=v["dt_bias"], reset=sl("reset"))
+        n = ssm_ref.scan_roundings(w, False)
+        ssm_ref.close(y, ref["y"][0], mag["y"][0], n, "y")
+        ssm_ref.close(h, ref["hT"], mag["hT"], n, "h")
+
+
+def test_step_of_views():
+    g = Gen(2)
+    B, D, N = 5, 24, 16
+    wide, bc = g.n(B, 3 * D + 1, dtype=BF), g.n(B, 2 * N + 3, dtype=BF)
+    A, h = -g.u(D, N), g.n(B, D, N)
+    h2, y, y2 = h.clone(), torch.full((B, 2 * D), 7.0, dtype=BF, device=DEV), torch.empty(B, D, dtype=BF, device=DEV)
+    a = (wide[:, 1:D + 1], wide[:, D + 1:2 * D + 1], A, bc[:, 3:3 + N], bc[:, 3 + N:])
+    H.ssm_step(*a, h, y[:, :D], z=wide[:, 2 * D + 1:])
+    H.ssm_step(*(t.contiguous() for t in a), h2, y2, z=wide[:, 2 * D + 1:].contiguous())
+    assert torch.equal(y[:, :D], y2) and torch.equal(h, h2) and bool((y[:, D:] == 7).all())
+
+
+# ---- same inputs, same bits; streams; graphs ----------------------------------------------------------------------------
+def test_results_do_not_change_from_call_to_call():
+    for v in (scan_case(70, 5, 96, 16, BF), scan_case(523, 1, 40, 8, F32)):
+        a, b = run_scan(v), run_scan(v)
+        assert all(torch.equal(a[k], b[k]) for k in a)
+    v = conv_case(65, 4, 264, 4, F32)
+    a, b = run_conv(v), run_conv(v)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+    g = Gen(0)
+    v = dict(x=g.n(1030, 40), w=g.n(40), b=g.n(40), dy=g.n(1030, 40))
+    a, b = run_norm(v), run_norm(v)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+
+
+def test_two_streams_at_once():
+    va, vb = scan_case(300, 2, 64, 16, F32, seed=1), scan_case(300, 2, 64, 16, F32, seed=2)
+    ra, rb = run_scan(va), run_scan(vb)
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        with torch.cuda.stream(sa):
+            a = run_scan(va)
+        with torch.cuda.stream(sb):
+            b = run_scan(vb)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a[k], ra[k]) for k in a) and all(torch.equal(b[k], rb[k]) for k in b)
+
+
+def core(v, s):
+    """One residual block of the core, forward and backward, the way an engine strings the operators together: norm -> short
+    convolution -> scan -> y + x, into the buffers of ``s``."""
+    T, B, D = v["x"].shape
+    flat = lambda t: t.view(T * B, D)                                              # noqa: E731
+    H.layer_norm_fwd(flat(v["x"]), v["nw"], v["nb"], flat(s["n"]), mean=s["mean"], rstd=s["rstd"])
+    H.short_conv_fwd(s["n"], v["w"], v["bias"], s["c"], state_in=v["cs"], state_out=s["cs"], reset=v["reset"], lengths=v["lengths"])
+    kw = dict(D=v["D"], z=v["z"], dt_bias=v["dt_bias"], reset=v["reset"], lengths=v["lengths"])
+    H.ssm_scan_fwd(s["c"], v["dt"], v["A"], v["Bm"], v["Cm"], s["y"], s["ws"], h0=v["h0"], hT=s["hT"], ckpt=s["ckpt"], **kw)
+    H.ssm_scan_bwd(v["dy"], s["c"], v["dt"], v["A"], v["Bm"], v["Cm"], s["ckpt"], s["dc"], s["ddt"], s["dA"], s["dB"], s["dC"], s["ws"], dD=s["dD"],
+                   dz=s["dz"], ddt_bias=s["ddt_bias"], dh0=s["dh0"], **kw)
+    H.short_conv_bwd(s["dc"], s["n"], v["w"], v["bias"], s["dn"], s["dw"], s["db"], s["cws"], state_in=v["cs"], dstate_in=s["dcs"],
+                     reset=v["reset"], lengths=v["lengths"])
+    H.layer_norm_bwd(flat(s["dn"]), flat(v["x"]), v["nw"], s["mean"], s["rstd"], flat(s["dx"]), s["dnw"], s["dnb"], s["nws"])
+
+
+def core_case(T=40, B=4, D=72, N=16, W=4, seed=0):
+    g = Gen(seed)
+    v = scan_case(T, B, D, N, F32, seed=seed, ragged=False)
+    v.update(x=g.n(T, B, D), nw=g.n(D, shift=1.0, scale=0.2), nb=g.n(D, scale=0.2), w=g.n(D, W, scale=0.5), bias=g.n(D, scale=0.1), cs=g.n(B, W - 1, D))
+    v["lengths"] = torch.tensor([T, 0, 1, T - 7][:B], dtype=torch.int32, device=DEV)
+    e = lambda *s: torch.full(s, float("nan"), device=DEV)                          # noqa: E731
+    s = {k: e(T, B, D) for k in ("n", "c", "y", "dc", "ddt", "dz", "dn", "dx")}
+    s.update(mean=e(T * B), rstd=e(T * B), cs=e(B, W - 1, D), hT=e(B, D, N), dA=e(D, N), dB=e(T, B, N), dC=e(T, B, N), dD=e(D), ddt_bias=e(D),
+             dh0=e(B, D, N), dw=e(D, W), db=e(D), dcs=e(B, W - 1, D), dnw=e(D), dnb=e(D), ws=H.ssm_scan_ws(T, B, D, N, DEV),
+             ckpt=H.ssm_scan_ckpt(T, B, D, N, DEV), cws=H.short_conv_ws(T, B, D, W, DEV), nws=H.layer_norm_ws(T * B, D, DEV))
+    return v, s
+
+
+def test_the_operators_together_against_autograd_in_64_bits():
+    v, s = core_case()
+    core(v, s)
+    p = {k: t.detach().cpu().double().requires_grad_() for k, t in v.items() if t is not None and t.is_floating_point() and k not in ("dy", "dhT", "u")}
+    reset, lengths = v["reset"].cpu(), v["lengths"].cpu()
+    n = oracle.layer_norm(p["x"], p["nw"], p["nb"])
+    c, cs = oracle.short_conv(n, p["w"], p["bias"], p["cs"], reset, lengths)
+    y, hT = oracle.ssm_scan(c, p["dt"], p["A"], p["Bm"], p["Cm"], p["D"], p["z"], p["dt_bias"], p["h0"], reset, lengths)
+    (y * v["dy"].cpu().double()).sum().backward()
+    pairs = dict(y=y, hT=hT, cs=cs, dx=p["x"].grad, dnw=p["nw"].grad, dnb=p["nb"].grad, dw=p["w"].grad, db=p["bias"].grad, dcs=p["cs"].grad,
+                 ddt=p["dt"].grad, dz=p["z"].grad, dA=p["A"].grad, dB=p["Bm"].grad, dC=p["Cm"].grad, dD=p["D"].grad, ddt_bias=p["dt_bias"].grad,
+                 dh0=p["h0"].grad)
+    for k, ref in pairs.items():
+        # the longest chain: 2 x 40 steps of (14 + exponents) roundings and sums over 160 rows; 2e-4 = 3 400 half steps
+        got = s[k].cpu().double()
+        assert float((got - ref).norm() / ref.norm()) < 2e-4, k
+
+
+def test_the_operators_together_acting_step_by_step():
+    """Acting one step at a time gives what the learner's sequence form gives."""
+    v, s = core_case()
+    v["lengths"] = None
+    core(v, s)
+    T, B, D = v["x"].shape
+    h, cs = v["h0"].clone(), v["cs"].clone()
+    for t in range(T):
+        n, c, y = like(v["x"][0], v["x"][0], v["x"][0])
+        H.layer_norm_fwd(v["x"][t], v["nw"], v["nb"], n)
+        H.short_conv_step(n, v["w"], v["bias"], cs, c, reset=v["reset"][t])
+        H.ssm_step(c, v["dt"][t], v["A"], v["Bm"][t], v["Cm"][t], h, y, D=v["D"], z=v["z"][t], dt_bias=v["dt_bias"], reset=v["reset"][t])
+        assert torch.equal(n, s["n"][t]) and torch.equal(c, s["c"][t])
+        torch.testing.assert_close(y, s["y"][t], rtol=1e-4, atol=1e-4)
+    assert torch.equal(cs, s["cs"])
+    torch.testing.assert_close(h, s["hT"], rtol=1e-4, atol=1e-4)
+
+
+def test_captured_and_replayed_on_new_inputs():
+    """Two graphs with a workspace each; every replay, with eager calls and synchronisations in between, is the eager result."""
+    sets = [core_case(T=300, B=2, D=40, seed=k) for k in (1, 2)]
+    graphs = []
+    for v, s in sets:
+        core(v, s)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            core(v, s)
+        graphs.append(g)
+    for k in range(3):
+        fresh = [core_case(T=300, B=2, D=40, seed=10 + 2 * k + i) for i in range(2)]
+        for (v, s), (w, _) in zip(sets, fresh):
+            for n, t in v.items():
+                if t is not None:
+                    t.copy_(w[n])
+        for g in graphs:
+            g.replay()
+        for (v, s), (w, e) in zip(sets, fresh):
+            core(w, e)
+            torch.cuda.synchronize()
+            for n in e:
+                if n not in ("ws", "ckpt", "cws", "nws"):
+                    assert torch.equal(e[n], s[n]), n
+
+
+# ---- refusals on the GPU ------------------------------------------------------------------------------------------------
+def test_refusals():
+    g = Gen(0)
+    T, B, D, N = 5, 2, 8, 4
+    v = scan_case(T, B, D, N, F32, ragged=False)
+    y, ws = torch.zeros_like(v["u"]), H.ssm_scan_ws(T, B, D, N, DEV)
+    ok = dict(u=v["u"], dt=v["dt"], A=v["A"], Bm=v["Bm"], Cm=v["Cm"], y=y, ws=ws)
+
+    def bad(exc, **kw):
+        with pytest.raises(exc):
+            H.ssm_scan_fwd(**{**ok, **kw})
+
+    H.ssm_scan_fwd(**ok)
+    bad(TypeError, dt=v["dt"].to(BF))
+    bad(TypeError, u=v["u"].half(), dt=v["dt"].half())
+    bad(TypeError, A=v["A"].double())
+    bad(TypeError, Bm=v["Bm"].cpu())
+    bad(TypeError, reset=torch.zeros(T, B, dtype=torch.bool, device=DEV))
+    bad(TypeError, lengths=torch.zeros(B, dtype=torch.int64, device=DEV))
+    bad(ValueError, A=v["A"][:, :3])
+    bad(ValueError, Cm=v["Cm"][:4])
+    bad(ValueError, lengths=torch.zeros(B + 1, dtype=torch.int32, device=DEV))
+    bad(ValueError, y=v["u"])
+    bad(ValueError, hT=v["h0"], h0=v["h0"])
+    bad(ValueError, dt=v["dt"].transpose(0, 2).contiguous().transpose(0, 2))
+    bad(ValueError, y=torch.zeros(1, B, D, device=DEV).expand(T, B, D))
+    bad(ValueError, ckpt=torch.zeros(2, B, D, N, device=DEV))
+    grads = dict(du=y.clone(), ddt=y.clone(), dA=torch.zeros(D, N, device=DEV), dB=torch.zeros(T, B, N, device=DEV), dC=torch.zeros(T, B, N, device=DEV))
+    with pytest.raises(RuntimeError, match="-2"):
+        H.ssm_scan_bwd(v["dy"], v["u"], v["dt"], v["A"], v["Bm"], v["Cm"], H.ssm_scan_ckpt(T, B, D, N, DEV), ws=torch.zeros(3, device=DEV), **grads)
+    with pytest.raises(ValueError):
+        H.ssm_scan_ws(5, 2, 8, 65, DEV)
+    x = g.n(6, 8)
+    with pytest.raises(RuntimeError, match="-2"):
+        H.layer_norm_bwd(x, x.clone(), g.n(8), g.n(6), g.n(6), torch.empty(6, 8, device=DEV), g.n(8), g.n(8), torch.zeros(2, device=DEV))
+    with pytest.raises(RuntimeError, match="-2"):
+        H.short_conv_bwd(v["dy"], v["u"], g.n(8, 4), None, y, g.n(8, 4), None, torch.zeros(2, device=DEV))
+    with pytest.raises(ValueError):
+        H.short_conv_ws(5, 2, 8, 5, DEV)
+    with pytest.raises(ValueError):
+        H.layer_norm_ws(5, 20000, DEV)
