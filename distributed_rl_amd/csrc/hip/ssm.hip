@@ -8,6 +8,7 @@
 // registers and walks the time in chunks of 16 steps. What depends on (step, channel) only is computed once - lane (g, j) has
 // the steps 4 i + g - and handed round through LDS; B and C of the chunk are staged in LDS as well.
 #include "ssm_math.h"
+#include <type_traits>
 
 #define KC 16            // steps per chunk = distance of the saved states
 
@@ -34,24 +35,120 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
+// a barrier that orders LDS only: loads and stores of global memory stay in flight
+__device__ __forceinline__ void block_sync_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
 
-// B and C rows of a chunk -> LDS (fp32, NP = 4 NS columns each, zeros beyond N and beyond the row's end)
-template <typename T, int NS>
-__device__ __forceinline__ void stage_bc(const SsmArgs& p, int b, int t0, int end, int lane, float* bc) {
-    constexpr int NP = 4 * NS;
+// Rows of a chunk of a [T, B, C] tensor through a buffer descriptor: uniform 64-bit base of the chunk's first step, 32-bit
+// offsets inside the chunk. A lane whose element does not exist takes the offset OOB: its load gives 0 and its store does
+// nothing, without a branch.
+#define OOB 0x80000000u
+template <typename T>
+struct Rows {
+    const char* base;            // the chunk's first step of row b
+    unsigned four;               // bytes over 4 steps (the host keeps 16 steps under 2^31 bytes)
+    __device__ __forceinline__ Rows(const void* q, long long st, long long sb, int b, int t0)
+        : base((const char*)q + (t0 * st + b * sb) * (long long)sizeof(T)), four((unsigned)st * (unsigned)(4 * sizeof(T))) {}
+    __device__ __forceinline__ void next() { base += 4ull * four; }
+    __device__ __forceinline__ void back() { base -= 4ull * four; }
+    __device__ __forceinline__ auto rsrc() const { return __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, 0x7fffffff, 0x00020000); }
+    static __device__ __forceinline__ unsigned offset(long long st, int s, long long c) { return ((unsigned)s * (unsigned)st + (unsigned)c) * (unsigned)sizeof(T); }
+    template <typename R> static __device__ __forceinline__ unsigned load(R r, unsigned voff, unsigned soff) {
+        if constexpr (sizeof(T) == 2) return (unsigned)__builtin_amdgcn_raw_buffer_load_b16(r, voff, soff, 0);
+        else return __builtin_amdgcn_raw_buffer_load_b32(r, voff, soff, 0);
+    }
+    static __device__ __forceinline__ float value(unsigned raw) { return __uint_as_float(sizeof(T) == 2 ? raw << 16 : raw); }
+    template <typename R> static __device__ __forceinline__ void store(R r, unsigned voff, unsigned soff, float v) {
+        if constexpr (sizeof(T) == 2) __builtin_amdgcn_raw_buffer_store_b16((short)f2bf(v), r, voff, soff, 0);
+        else __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v), r, voff, soff, 0);
+    }
+};
+
+// What a block of four waves needs of B and C in a chunk: NV values of each per thread, fetched ahead and written to LDS as
+// fp32, [step][B: NP | C: NP], zeros beyond N and beyond the row's end. WHICH: 1 = B, 2 = C, 3 = both.
+template <typename T, int NS, int WHICH>
+struct StageBC {
+    static constexpr int NP = 4 * NS, NV = KC * NP > 256 ? KC * NP / 256 : 1, ROW = WHICH == 3 ? 2 * NP : NP, STEP = 256 / NP;
+    Rows<T> B, C;
+    unsigned ob, oc, rb[WHICH & 1 ? NV : 1], rc[WHICH & 2 ? NV : 1];
+    __device__ __forceinline__ StageBC(const SsmArgs& p, int b, int t0)
+        : B(p.Bm, p.B_t, p.B_b, b, t0), C(p.Cm, p.C_t, p.C_b, b, t0) {
+        const int n = threadIdx.x % NP, s = threadIdx.x / NP;
+        const bool in = n < p.N && s < KC;
+        ob = in ? Rows<T>::offset(p.B_t, s, n) : OOB;
+        oc = in ? Rows<T>::offset(p.C_t, s, n) : OOB;
+    }
+    // live: steps of the chunk before the row's end
+    __device__ __forceinline__ void fetch(int live) {
+        const int s = threadIdx.x / NP;
 #pragma unroll
-    for (int k = 0; k < KC * NP / 64; ++k) {
-        const int e = k * 64 + lane, s = e / NP, n = e % NP, t = t0 + s;
-        const bool ok = t < end && n < p.N;
-        bc[s * 2 * NP + n] = ok ? ld((const T*)p.Bm + t * p.B_t + b * p.B_b + n) : 0.f;
-        bc[s * 2 * NP + NP + n] = ok ? ld((const T*)p.Cm + t * p.C_t + b * p.C_b + n) : 0.f;
+        for (int k = 0; k < NV; ++k) {
+            const unsigned bad = s + k * STEP < live ? 0u : OOB;
+            if (WHICH & 1) rb[k] = Rows<T>::load(B.rsrc(), ob | bad, k * STEP * (B.four / 4));
+            if (WHICH & 2) rc[k] = Rows<T>::load(C.rsrc(), oc | bad, k * STEP * (C.four / 4));
+        }
+    }
+    __device__ __forceinline__ void put(float* bc) const {
+        const int n = threadIdx.x % NP, s = threadIdx.x / NP;
+        if (KC * NP < 256 && s >= KC) return;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float* q = bc + (s + k * STEP) * ROW + n;
+            if (WHICH & 1) *q = Rows<T>::value(rb[k]);
+            if (WHICH & 2) q[WHICH == 3 ? NP : 0] = Rows<T>::value(rc[k]);
+        }
+    }
+};
+// NS consecutive values of an LDS image
+template <int NS>
+__device__ __forceinline__ void lds_row(const float* q, float (&v)[NS]) {
+    if constexpr (NS % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < NS; i += 4) { const float4 x = *reinterpret_cast<const float4*>(q + i); v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w; }
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(q);
+        v[0] = x.x; v[1] = x.y;
     }
 }
 
-__device__ __forceinline__ unsigned reset_mask(const SsmArgs& p, int b, int t0, int end, int lane) {
+// reset flags of a chunk, one byte in each of the first 16 lanes, and as a bit mask
+__device__ __forceinline__ unsigned fetch_resets(const SsmArgs& p, int b, int t0, int end, int lane) {
     if (!p.reset) return 0;
-    const int t = t0 + lane;
-    return (unsigned)__ballot(lane < KC && t < end && p.reset[(long long)t * p.B + b] != 0) & 0xffffu;
+    const int t = t0 + (lane & 15);
+    return t < end ? p.reset[(long long)t * p.B + b] : 0;
+}
+__device__ __forceinline__ unsigned reset_mask(unsigned flag) { return (unsigned)__ballot(flag != 0) & 0xffffu; }
+
+__device__ __forceinline__ int row_end(const SsmArgs& p, int b) { return p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T; }
+
+// the states of a lane in a [.., B, D, N] tensor, four at a time (v4: N and the tensor's address allow it, see vec4)
+__device__ __forceinline__ bool vec4(const float* q, long long N) { return (N & 3) == 0 && ((uintptr_t)q & 15) == 0; }
+template <int NS>
+__device__ __forceinline__ void put_states(float* q, const float (&h)[NS], int n0, int N, bool v4) {
+    if (NS % 4 == 0 && v4) {
+#pragma unroll
+        for (int i = 0; i + 3 < NS; i += 4) if (n0 + i < N) *reinterpret_cast<float4*>(q + i) = make_float4(h[i], h[i + 1], h[i + 2], h[i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) if (n0 + i < N) q[i] = h[i];
+    }
+}
+template <int NS>
+__device__ __forceinline__ void get_states(const float* q, float (&h)[NS], int n0, int N, bool ok, bool v4) {
+#pragma unroll
+    for (int i = 0; i < NS; ++i) h[i] = 0.f;
+    if (!ok) return;
+    if (NS % 4 == 0 && v4) {
+#pragma unroll
+        for (int i = 0; i + 3 < NS; i += 4)
+            if (n0 + i < N) { const float4 v = *reinterpret_cast<const float4*>(q + i); h[i] = v.x; h[i + 1] = v.y; h[i + 2] = v.z; h[i + 3] = v.w; }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) if (n0 + i < N) h[i] = q[i];
+    }
 }
 
 // Sums over the four lane groups (rows of 16 lanes): group g ends with the sum of v[g]. Swapping rows adds two values at a
@@ -72,37 +169,51 @@ __device__ __forceinline__ float sum_groups(float v0, float v1, float v2, float 
 // and holds all of their terms in registers until then.
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
-// Sums over the 16 lanes of a row, four at a time: quad 0 of r ends with the sum of be, quad 1 bo, quad 2 ce, quad 3 co. The
-// first two levels fold two values into one register (a bank mask writes half of the quads each), so a value costs 2 adds
-// instead of 4. The waits between a write and a cross-lane read of it (2 states) are the other registers' adds or s_nop.
-__device__ __forceinline__ void sum_rows2(const float (&be)[2], const float (&ce)[2], const float (&bo)[2], const float (&co)[2], float (&r)[2]) {
-    float t0, t1;
-    asm volatile("s_nop 1\n"
-        "v_add_f32_dpp %0, %4, %4 row_mirror row_mask:0xf bank_mask:0x3\n"
-        "v_add_f32_dpp %1, %5, %5 row_mirror row_mask:0xf bank_mask:0x3\n"
-        "v_add_f32_dpp %2, %6, %6 row_mirror row_mask:0xf bank_mask:0x3\n"
-        "v_add_f32_dpp %3, %7, %7 row_mirror row_mask:0xf bank_mask:0x3\n"
-        "v_add_f32_dpp %0, %8, %8 row_mirror row_mask:0xf bank_mask:0xc\n"
-        "v_add_f32_dpp %1, %9, %9 row_mirror row_mask:0xf bank_mask:0xc\n"
-        "v_add_f32_dpp %2, %10, %10 row_mirror row_mask:0xf bank_mask:0xc\n"
-        "v_add_f32_dpp %3, %11, %11 row_mirror row_mask:0xf bank_mask:0xc\n"
-        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(t0), "=&v"(t1)
-        : "v"(be[0]), "v"(be[1]), "v"(bo[0]), "v"(bo[1]), "v"(ce[0]), "v"(ce[1]), "v"(co[0]), "v"(co[1]));
-    float q0, q1;
-    asm volatile("s_nop 1\n"
-        "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0x5\n"
-        "v_add_f32_dpp %1, %3, %3 row_half_mirror row_mask:0xf bank_mask:0x5\n"
-        "v_add_f32_dpp %0, %4, %4 row_half_mirror row_mask:0xf bank_mask:0xa\n"
-        "v_add_f32_dpp %1, %5, %5 row_half_mirror row_mask:0xf bank_mask:0xa\n"
-        "s_nop 0\n"
-        "v_add_f32_dpp %0, %0, %0 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
-        "v_add_f32_dpp %1, %1, %1 quad_perm:[1,0,3,2] row_mask:0xf bank_mask:0xf\n"
-        "s_nop 0\n"
-        "v_add_f32_dpp %0, %0, %0 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
-        "v_add_f32_dpp %1, %1, %1 quad_perm:[2,3,0,1] row_mask:0xf bank_mask:0xf\n"
-        : "=&v"(q0), "=&v"(q1) : "v"(r[0]), "v"(r[1]), "v"(t0), "v"(t1));
-    r[0] = q0; r[1] = q1;
+// Sums over the 16 lanes of a row, NS x 4 of them at a time: quad 0 holds the sums of be, quad 1 bo, quad 2 ce, quad 3 co, and
+// lane q of a quad the one of index q (index q & 1 where there are two). Every level folds two values into one register - by
+// bank masks, which write half of the quads each, or within quads by exchanging what the other lane keeps - so a value costs
+// 2 to 2.3 instructions instead of 4 adds. Between a write and a cross-lane read of it there are 2 wait states: the other
+// registers' adds, or s_nop.
+#define DPP(D, S, CTRL, BANK) "v_add_f32_dpp %" #D ", %" #S ", %" #S " " CTRL " row_mask:0xf bank_mask:" BANK "\n"
+template <int CTRL>
+__device__ __forceinline__ float quad_fold(bool odd, float v0, float v1) {
+    const float keep = odd ? v1 : v0, give = odd ? v0 : v1;
+    return keep + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(give), CTRL, 0xf, 0xf, true));
 }
+#define QUAD_XOR1 0xB1
+#define QUAD_XOR2 0x4E
+__device__ __forceinline__ float sum_rows2(const float* be, const float* ce, const float* bo, const float* co, int j) {
+    float t0, t1, t2, t3, r0, r1;
+    asm volatile("s_nop 1\n"
+        DPP(0, 4, "row_mirror", "0x3") DPP(1, 5, "row_mirror", "0x3") DPP(2, 6, "row_mirror", "0x3") DPP(3, 7, "row_mirror", "0x3")
+        DPP(0, 8, "row_mirror", "0xc") DPP(1, 9, "row_mirror", "0xc") DPP(2, 10, "row_mirror", "0xc") DPP(3, 11, "row_mirror", "0xc")
+        : "=&v"(t0), "=&v"(t1), "=&v"(t2), "=&v"(t3)
+        : "v"(be[0]), "v"(be[1]), "v"(bo[0]), "v"(bo[1]), "v"(ce[0]), "v"(ce[1]), "v"(co[0]), "v"(co[1]));
+    asm volatile("s_nop 1\n"
+        DPP(0, 2, "row_half_mirror", "0x5") DPP(1, 3, "row_half_mirror", "0x5")
+        DPP(0, 4, "row_half_mirror", "0xa") DPP(1, 5, "row_half_mirror", "0xa")
+        : "=&v"(r0), "=&v"(r1) : "v"(t0), "v"(t1), "v"(t2), "v"(t3));
+    float v = quad_fold<QUAD_XOR1>(j & 1, r0, r1);
+    return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), QUAD_XOR2, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum_rows4(const float* be, const float* ce, const float* bo, const float* co, int j) {
+    float t[8], r[4];
+    asm volatile("s_nop 1\n"
+        DPP(0, 8, "row_mirror", "0x3") DPP(1, 9, "row_mirror", "0x3") DPP(2, 10, "row_mirror", "0x3") DPP(3, 11, "row_mirror", "0x3")
+        DPP(4, 12, "row_mirror", "0x3") DPP(5, 13, "row_mirror", "0x3") DPP(6, 14, "row_mirror", "0x3") DPP(7, 15, "row_mirror", "0x3")
+        DPP(0, 16, "row_mirror", "0xc") DPP(1, 17, "row_mirror", "0xc") DPP(2, 18, "row_mirror", "0xc") DPP(3, 19, "row_mirror", "0xc")
+        DPP(4, 20, "row_mirror", "0xc") DPP(5, 21, "row_mirror", "0xc") DPP(6, 22, "row_mirror", "0xc") DPP(7, 23, "row_mirror", "0xc")
+        : "=&v"(t[0]), "=&v"(t[1]), "=&v"(t[2]), "=&v"(t[3]), "=&v"(t[4]), "=&v"(t[5]), "=&v"(t[6]), "=&v"(t[7])
+        : "v"(be[0]), "v"(be[1]), "v"(be[2]), "v"(be[3]), "v"(bo[0]), "v"(bo[1]), "v"(bo[2]), "v"(bo[3]),
+          "v"(ce[0]), "v"(ce[1]), "v"(ce[2]), "v"(ce[3]), "v"(co[0]), "v"(co[1]), "v"(co[2]), "v"(co[3]));
+    asm volatile("s_nop 1\n"
+        DPP(0, 4, "row_half_mirror", "0x5") DPP(1, 5, "row_half_mirror", "0x5") DPP(2, 6, "row_half_mirror", "0x5") DPP(3, 7, "row_half_mirror", "0x5")
+        DPP(0, 8, "row_half_mirror", "0xa") DPP(1, 9, "row_half_mirror", "0xa") DPP(2, 10, "row_half_mirror", "0xa") DPP(3, 11, "row_half_mirror", "0xa")
+        : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
+        : "v"(t[0]), "v"(t[1]), "v"(t[2]), "v"(t[3]), "v"(t[4]), "v"(t[5]), "v"(t[6]), "v"(t[7]));
+    return quad_fold<QUAD_XOR2>(j & 2, quad_fold<QUAD_XOR1>(j & 1, r[0], r[1]), quad_fold<QUAD_XOR1>(j & 1, r[2], r[3]));
+}
+#undef DPP
 
 // A long time axis with few rows is cut into segments that run side by side: what a segment does to the state is
 // h -> P h + e with P = exp(A sum of s) and e its end state from h = 0 (k_ssm_carry), the segments are joined in order
@@ -111,14 +222,14 @@ __device__ __forceinline__ void sum_rows2(const float (&be)[2], const float (&ce
 template <typename T, int NS, bool BWD>
 __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float* __restrict__ carry, float* __restrict__ sums) {
     constexpr int NP = 4 * NS;
+    using R = Rows<T>;
     __shared__ __align__(16) float2 pw_s[4][KC][16];
-    __shared__ __align__(16) float bc_s[4][KC * NP];
+    __shared__ __align__(16) float bc_s[2][KC * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     const int b = blockIdx.y, seg = BWD ? blockIdx.z + 1 : blockIdx.z;          // the last one (the first one) passes nothing on
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
-    const int end = p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T;
-    const int ta = seg * seg_len, tb = min(ta + seg_len, (int)p.T);
+    const int end = row_end(p, b), ta = seg * seg_len, tb = min(ta + seg_len, (int)p.T);
     float A2[NS], h[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
@@ -126,56 +237,70 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
         h[i] = 0.f;
     }
     const float bias = dv && p.bias ? p.bias[d] : 0.f;
+    const void* v_p = BWD ? p.dy : p.u;
+    const long long v_t = BWD ? p.dy_t : p.u_t, v_b = BWD ? p.dy_b : p.u_b;
+    const unsigned ov = R::offset(v_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d);
+    const int n_chunks = max(0, (min(tb, end) - ta + KC - 1) / KC);
     float sum = 0.f;
     bool cut = false;
-    const int n_chunks = (min(tb, end) - ta + KC - 1) / KC;
+    unsigned rv[4], rd[4], rz[4], rr;
+    const int t_first = BWD ? ta + max(0, n_chunks - 1) * KC : ta;
+    R xv(v_p, v_t, v_b, b, t_first), xd(p.dt, p.dt_t, p.dt_b, b, t_first), xz(p.z, p.z_t, p.z_b, b, t_first);
+    StageBC<T, NS, BWD ? 2 : 1> st(p, b, t_first);
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned bad = dv && t0 + 4 * i + g < end ? 0u : OOB;
+            rv[i] = R::load(xv.rsrc(), ov | bad, i * xv.four);
+            rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
+            if (BWD && p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
+        }
+        st.fetch(end - t0);
+        rr = fetch_resets(p, b, t0, end, lane);
+        if (BWD) { xv.back(); xd.back(); xz.back(); st.C.back(); } else { xv.next(); xd.next(); st.B.next(); }
+    };
+    if (n_chunks) fetch(t_first);
     for (int c = 0; c < n_chunks; ++c) {
         const int t0 = ta + (BWD ? n_chunks - 1 - c : c) * KC;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = 4 * i + g, t = t0 + s;
-            const bool ok = dv && t < end;
-            float v;
-            if (BWD) {
-                v = ok ? ld((const T*)p.dy + t * p.dy_t + b * p.dy_b + d) : 0.f;
-                if (p.z && ok) { const float z = ld((const T*)p.z + t * p.z_t + b * p.z_b + d); v *= z * sigmoidf(z); }
-            } else {
-                v = ok ? ld((const T*)p.u + t * p.u_t + b * p.u_b + d) : 0.f;
-            }
-            float sp = ok ? ld((const T*)p.dt + t * p.dt_t + b * p.dt_b + d) + bias : 0.f;
-            if (ok && p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
+            float v = R::value(rv[i]);
+            if (BWD && p.z) { const float z = R::value(rz[i]); v *= z * sigmoidf(z); }
+            float sp = R::value(rd[i]) + bias;
+            if (p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
+            sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
             sum += sp;
-            pw_s[w][s][j] = make_float2(sp, BWD ? v : sp * v);
+            pw_s[w][4 * i + g][j] = make_float2(sp, BWD ? v : sp * v);
         }
-#pragma unroll
-        for (int k = 0; k < KC * NP / 64; ++k) {
-            const int e = k * 64 + lane, n = e % NP, t = t0 + e / NP;
-            const bool ok = t < end && n < p.N;
-            bc_s[w][e] = !ok ? 0.f : BWD ? ld((const T*)p.Cm + t * p.C_t + b * p.C_b + n) : ld((const T*)p.Bm + t * p.B_t + b * p.B_b + n);
-        }
-        const unsigned rm = reset_mask(p, b, t0, end, lane);
+        float* bcb = bc_s[c & 1];
+        st.put(bcb);
+        const unsigned rm = reset_mask(rr);
         cut |= rm != 0;
-        wave_sync();
+        if (c + 1 < n_chunks) fetch(BWD ? t0 - KC : t0 + KC);
+        block_sync_lds();
+        auto steps = [&](auto has) {
 #pragma unroll 4
-        for (int k = 0; k < KC; ++k) {
-            const int s = BWD ? KC - 1 - k : k;
-            const float2 pw = pw_s[w][s][j];
-            const float* bc = bc_s[w] + s * NP + g * NS;
-            const bool rs = rm >> s & 1;
+            for (int k = 0; k < KC; ++k) {
+                const int s = BWD ? KC - 1 - k : k;
+                const float2 pw = pw_s[w][s][j];
+                float bc[NS];
+                lds_row<NS>(bcb + s * NP + g * NS, bc);
+                const bool rs = has && (rm >> s & 1);
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const float a = __builtin_amdgcn_exp2f(pw.x * A2[i]);
-                h[i] = BWD ? (rs ? 0.f : a * fmaf(pw.y, bc[i], h[i])) : fmaf(a, rs ? 0.f : h[i], pw.y * bc[i]);
+                for (int i = 0; i < NS; ++i) {
+                    const float a = __builtin_amdgcn_exp2f(pw.x * A2[i]);
+                    h[i] = BWD ? (rs ? 0.f : a * fmaf(pw.y, bc[i], h[i])) : fmaf(a, rs ? 0.f : h[i], pw.y * bc[i]);
+                }
             }
-        }
+        };
+        if (rm) steps(std::true_type{}); else steps(std::false_type{});
         wave_sync();
     }
     sum += __shfl_xor(sum, 16, WAVE);
     sum += __shfl_xor(sum, 32, WAVE);
     if (!dv) return;
     const long long o = ((long long)seg * p.B + b) * p.D + d;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) if (g * NS + i < p.N) carry[o * p.N + g * NS + i] = h[i];
+    put_states<NS>(carry + o * p.N + g * NS, h, g * NS, p.N, vec4(carry, p.N));
     if (g == 0) sums[o] = cut ? __builtin_inff() : sum;
 }
 
@@ -201,215 +326,293 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const float* __restrict__ carry) {
     constexpr int NP = 4 * NS;
+    using R = Rows<T>;
     __shared__ __align__(16) float2 pw_s[4][KC][16];
-    __shared__ __align__(16) float bc_s[4][KC * 2 * NP];
+    __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     const int b = blockIdx.y;
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
-    const int end = p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T;
+    const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
     const long long so = ((long long)b * p.D + d) * p.N + g * NS;          // this lane's states in a [B, D, N] tensor
+    const long long BDN = p.B * p.D * p.N;
     float A2[NS], h[NS];
+    const float* hp = carry ? carry + blockIdx.z * BDN : p.h0;
+    get_states<NS>(hp + so, h, g * NS, p.N, dv && hp, vec4(hp, p.N));
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const bool ok = dv && g * NS + i < p.N;
-        A2[i] = ok ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
-        h[i] = !ok ? 0.f : carry ? carry[(long long)blockIdx.z * p.B * p.D * p.N + so + i] : p.h0 ? p.h0[so + i] : 0.f;
-    }
+    for (int i = 0; i < NS; ++i) A2[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
-    const int ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
-    for (int t0 = ta; t0 < tb; t0 += KC) {
+    const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.y_t, g, d);
+    unsigned ru[4], rd[4], rz[4], rr;
+    R xu(p.u, p.u_t, p.u_b, b, ta), xd(p.dt, p.dt_t, p.dt_b, b, ta), xz(p.z, p.z_t, p.z_b, b, ta), xy(p.y, p.y_t, p.y_b, b, ta);
+    StageBC<T, NS, 3> st(p, b, ta);
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned bad = dv && t0 + 4 * i + g < end ? 0u : OOB;
+            ru[i] = R::load(xu.rsrc(), ou | bad, i * xu.four);
+            rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
+            if (p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
+        }
+        st.fetch(end - t0);
+        rr = fetch_resets(p, b, t0, end, lane);
+        xu.next(); xd.next(); xz.next(); st.B.next(); st.C.next();
+    };
+    fetch(ta);
+    for (int t0 = ta, c = 0; t0 < tb; t0 += KC, ++c) {
         float u[4], zz[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = 4 * i + g, t = t0 + s;
-            const bool ok = dv && t < end;
-            u[i] = ok ? ld((const T*)p.u + t * p.u_t + b * p.u_b + d) : 0.f;
-            zz[i] = ok && p.z ? ld((const T*)p.z + t * p.z_t + b * p.z_b + d) : 0.f;
-            float sp = ok ? ld((const T*)p.dt + t * p.dt_t + b * p.dt_b + d) + bias : 0.f;
-            if (ok && p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
-            pw_s[w][s][j] = make_float2(sp, sp * u[i]);
+            u[i] = R::value(ru[i]);
+            zz[i] = 1.f;
+            if (p.z) { const float z = R::value(rz[i]); zz[i] = z * sigmoidf(z); }
+            float sp = R::value(rd[i]) + bias;
+            if (p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
+            sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
+            pw_s[w][4 * i + g][j] = make_float2(sp, sp * u[i]);
         }
-        stage_bc<T, NS>(p, b, t0, end, lane, bc_s[w]);
-        const unsigned rm = reset_mask(p, b, t0, end, lane);
-        wave_sync();
-        if (p.ckpt && dv) {
-            float* c = p.ckpt + (long long)(t0 / KC) * p.B * p.D * p.N + so;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) if (g * NS + i < p.N) c[i] = h[i];
-        }
+        float* bcb = bc_s[c & 1];
+        st.put(bcb);
+        const unsigned rm = reset_mask(rr);
+        if (t0 + KC < tb) fetch(t0 + KC);
+        block_sync_lds();                 // B and C of this chunk are there; the image of the chunk before last is free again
+        if (p.ckpt && dv) put_states<NS>(p.ckpt + (t0 / KC) * BDN + so, h, g * NS, p.N, vec4(p.ckpt, p.N));
         float y[4];
+        auto steps = [&](auto has) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            float part[4];
+            for (int q = 0; q < 4; ++q) {
+                float part[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int s = 4 * q + r;
-                const float2 pw = pw_s[w][s][j];
-                if (rm >> s & 1) {
+                for (int r = 0; r < 4; ++r) {
+                    const int s = 4 * q + r;
+                    const float2 pw = pw_s[w][s][j];
+                    const bool rs = has && (rm >> s & 1);
+                    float Bv[NS], Cv[NS];
+                    lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
+                    lds_row<NS>(bcb + s * 2 * NP + NP + g * NS, Cv);
+                    float acc = 0.f;
 #pragma unroll
-                    for (int i = 0; i < NS; ++i) h[i] = 0.f;
+                    for (int i = 0; i < NS; ++i) {
+                        h[i] = fmaf(__builtin_amdgcn_exp2f(pw.x * A2[i]), rs ? 0.f : h[i], pw.y * Bv[i]);
+                        acc = fmaf(Cv[i], h[i], acc);
+                    }
+                    part[r] = acc;
                 }
-                const float* bc = bc_s[w] + s * 2 * NP + g * NS;
-                float acc = 0.f;
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    h[i] = fmaf(__builtin_amdgcn_exp2f(pw.x * A2[i]), h[i], pw.y * bc[i]);
-                    acc = fmaf(bc[NP + i], h[i], acc);
-                }
-                part[r] = acc;
+                y[q] = sum_groups(part[0], part[1], part[2], part[3]);
             }
-            y[q] = sum_groups(part[0], part[1], part[2], part[3]);
-        }
+        };
+        if (rm) steps(std::true_type{}); else steps(std::false_type{});
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int t = t0 + 4 * i + g;
-            if (!dv || t >= p.T) continue;
-            float v = 0.f;
-            if (t < end) {
-                v = fmaf(Dd, u[i], y[i]);
-                if (p.z) v *= zz[i] * sigmoidf(zz[i]);
-            }
-            st((T*)p.y + t * p.y_t + b * p.y_b + d, v);
+            // dead steps: u = 0 and C = 0, so the sum is 0 but for what a diverged state makes of it
+            R::store(xy.rsrc(), dv && t < p.T ? oy : OOB, i * xy.four, t < end ? fmaf(Dd, u[i], y[i]) * zz[i] : 0.f);
         }
-        wave_sync();                                        // the next chunk overwrites the LDS images
+        xy.next();
+        wave_sync();                                        // the next chunk overwrites this wave's LDS image
     }
-    if (p.hT && dv && blockIdx.z == gridDim.z - 1) {
-#pragma unroll
-        for (int i = 0; i < NS; ++i) if (g * NS + i < p.N) p.hT[so + i] = h[i];
-    }
+    if (p.hT && dv && blockIdx.z == gridDim.z - 1) put_states<NS>(p.hT + so, h, g * NS, p.N, vec4(p.hT, p.N));
 }
 
 // Backward. g_t = C ds + a_{t+1} g_{t+1} runs against the time; the states it needs are recomputed chunk by chunk from the
 // saved ones and kept in registers (16 steps x NS, next to the decays). The sums over channels of dB and dC leave as partials
 // of 64 channels (a block), the sums over rows of dA, dD and the bias as partials of a row: second launches add them in a
 // fixed order.
-template <typename T, int NS>
-__global__ __launch_bounds__(256, 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
-                                                    float* __restrict__ part_bc, float* __restrict__ part_a, float* __restrict__ part_d) {
+// KH steps of a chunk, s0 .. s0 + KH - 1, from the state before them: forward with the states and decays kept, then back.
+// mid() is called half way back, when half of those registers are free again: the next chunk's loads start there.
+template <int NS, int KH, bool RS, typename F>
+__device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const float* bcb, float* red_w, unsigned rm, int s0, int g, int j,
+                                          const float (&An)[NS], float (&hs)[KH + 1][NS], float (&G)[NS], float (&dAc)[NS],
+                                          float4 (&ex_w)[KC][16], float (&gb)[4], float (&wa)[4], F mid) {
     constexpr int NP = 4 * NS;
-    constexpr int KH = NS > 4 ? 64 / NS : KC;               // steps whose states are held at a time
-    __shared__ __align__(16) float4 pw_s[4][KC][16];
-    __shared__ __align__(16) float bc_s[4][KC * 2 * NP];
-    __shared__ __align__(16) float red_s[4][KC * 2 * NP];
+    float a[KH][NS], part[4];
+#pragma unroll
+    for (int k = 0; k < KH; ++k) {
+        if ((k & 1) == 0) __builtin_amdgcn_sched_barrier(0);
+        const int s = s0 + k;
+        const float4 pw = pw_w[s][j];
+        float Bv[NS], Cv[NS];
+        lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
+        lds_row<NS>(bcb + s * 2 * NP + NP + g * NS, Cv);
+        const bool rs = RS && (rm >> s & 1);        // hs[k] stays: dC of the step before needs it
+        float acc = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            a[k][i] = __builtin_amdgcn_exp2f(pw.x * An[i]);
+            hs[k + 1][i] = fmaf(a[k][i], rs ? 0.f : hs[k][i], pw.y * Bv[i]);
+            acc = fmaf(Cv[i], hs[k + 1][i], acc);
+        }
+        part[k & 3] = acc;
+        if ((k & 3) == 3) {
+            ex_w[s - 3 + g][j].w = sum_groups(part[0], part[1], part[2], part[3]);
+        }
+    }
+    int again = 0;                                  // hides that B, C and the step's scalars are read a second time:
+    asm volatile("" : "+v"(again));                 // kept from the first, they would fill the registers
+    float pb[4], pa[4];
+#pragma unroll
+    for (int k = KH - 2; k >= 0; k -= 2) {          // two steps at a time: k + 1, then k
+        float vB[2][NS], vC[2][NS];
+        if (k == KH / 2 - 2 || (KH == 4 && k == 0)) mid();
+#pragma unroll
+        for (int o = 1; o >= 0; --o) {
+            const int s = s0 + k + o, c = (k + o) & 3;
+            const float4 pw = pw_w[s][j + again];
+            float Bv[NS], Cv[NS];
+            lds_row<NS>(bcb + s * 2 * NP + g * NS + again, Bv);
+            lds_row<NS>(bcb + s * 2 * NP + NP + g * NS + again, Cv);
+            const bool rs = RS && (rm >> s & 1);
+            pb[c] = 0.f; pa[c] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float gh = fmaf(pw.z, Cv[i], G[i]);
+                vB[o][i] = gh * pw.y;
+                vC[o][i] = pw.z * hs[k + o + 1][i];
+                pb[c] = fmaf(gh, Bv[i], pb[c]);
+                const float q = rs ? 0.f : gh * a[k + o][i], x = q * (rs ? 0.f : hs[k + o][i]);
+                G[i] = q;
+                pa[c] = fmaf(x, An[i], pa[c]);
+                dAc[i] = fmaf(x, pw.x, dAc[i]);
+                pin(dAc[i]);
+            }
+            pin(pb[c]); pin(pa[c]);
+        }
+        float* red = red_w + (s0 + k + (j >> 2 & 1)) * 2 * NP + (j >> 3) * NP + g * NS;
+        if constexpr (NS % 4 == 0) {
+#pragma unroll
+            for (int i = 0; i < NS; i += 4) red[i + (j & 3)] = sum_rows4(vB[0] + i, vC[0] + i, vB[1] + i, vC[1] + i, j);
+        } else {
+            red[j & 1] = sum_rows2(vB[0], vC[0], vB[1], vC[1], j);
+        }
+        if ((k & 3) == 0) {
+            float sb = sum_groups(pb[0], pb[1], pb[2], pb[3]), sa = sum_groups(pa[0], pa[1], pa[2], pa[3]);
+            pin(sb); pin(sa);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (i == (s0 + k) / 4) { gb[i] = sb; wa[i] = sa; }
+        }
+    }
+}
+
+template <typename T, int NS>
+__global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
+                                                    float* __restrict__ part_bc, float* __restrict__ part_a) {
+    constexpr int NP = 4 * NS;
+    constexpr int KH = NS > 4 ? 4 : KC;                     // steps whose states are held at a time
+    using R = Rows<T>;
+    __shared__ __align__(16) float4 pw_s[4][KC][16];        // s log2(e), s u, ds, u
+    __shared__ __align__(16) float4 ex_s[4][KC][16];        // z, dy, ds/d(pre), sum_n C h
+    __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
+    __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
+    __shared__ float mid_s[KH < KC ? 4 : 1][KH < KC ? KC / KH - 1 : 1][KH < KC ? NS : 1][64];      // states before each piece
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     const int b = blockIdx.y;
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
-    const int end = p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T;
-    const long long so = ((long long)b * p.D + d) * p.N + g * NS;
-    float An[NS], G[NS], dA[NS];
+    const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
+    const long long so = ((long long)b * p.D + d) * p.N + g * NS, BDN = p.B * p.D * p.N;
+    float An[NS], G[NS], dA[NS];                            // G = a_{t+1} g_{t+1}: dL/dh_t from the steps behind
+    const float* Gp = carry ? carry + blockIdx.z * BDN : p.dhT;
+    get_states<NS>(Gp + so, G, g * NS, p.N, dv && Gp, vec4(Gp, p.N));
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        const bool ok = dv && g * NS + i < p.N;
-        An[i] = ok ? p.A[(long long)d * p.N + g * NS + i] : 0.f;
-        // a_{t+1} g_{t+1}: dL/dh_t from the steps behind
-        G[i] = !ok ? 0.f : carry ? carry[(long long)blockIdx.z * p.B * p.D * p.N + so + i] : p.dhT ? p.dhT[so + i] : 0.f;
+        An[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] : 0.f;
         dA[i] = 0.f;
     }
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
     float dD = 0.f, dbias = 0.f;
-    const int ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
-    for (int t0 = ta + (tb - ta - 1) / KC * KC; t0 >= ta; t0 -= KC) {
-        float u[4], zz[4], dy[4], sp[4], sg[4], ds[4];
+    const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.dy_t, g, d);
+    const unsigned odu = R::offset(p.du_t, g, d), odd = R::offset(p.ddt_t, g, d), odz = R::offset(p.dz_t, g, d);
+    unsigned ru[4], rd[4], rz[4], ry[4], rr;
+    float hc[NS];
+    const int t_last = ta + (tb - ta - 1) / KC * KC;
+    R xu(p.u, p.u_t, p.u_b, b, t_last), xd(p.dt, p.dt_t, p.dt_b, b, t_last), xz(p.z, p.z_t, p.z_b, b, t_last), xy(p.dy, p.dy_t, p.dy_b, b, t_last);
+    R wu(p.du, p.du_t, p.du_b, b, t_last), wd(p.ddt, p.ddt_t, p.ddt_b, b, t_last), wz(p.dz, p.dz_t, p.dz_b, b, t_last);
+    StageBC<T, NS, 3> st(p, b, t_last);
+    const float* ck = p.ckpt + t_last / KC * BDN;
+    const bool ck4 = vec4(p.ckpt, p.N);
+    auto fetch = [&](int t0) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int s = 4 * i + g, t = t0 + s;
-            const bool ok = dv && t < end;
-            u[i] = ok ? ld((const T*)p.u + t * p.u_t + b * p.u_b + d) : 0.f;
-            zz[i] = ok && p.z ? ld((const T*)p.z + t * p.z_t + b * p.z_b + d) : 0.f;
-            dy[i] = ok ? ld((const T*)p.dy + t * p.dy_t + b * p.dy_b + d) : 0.f;
-            sp[i] = ok ? ld((const T*)p.dt + t * p.dt_t + b * p.dt_b + d) + bias : 0.f;
-            sg[i] = ok ? 1.f : 0.f;
-            if (ok && p.softplus) {
-                const float e = exp_neg_abs(sp[i]);
-                sg[i] = sigmoid_from(sp[i], e);
-                sp[i] = softplus_from(sp[i], e);
-            }
-            ds[i] = p.z ? dy[i] * zz[i] * sigmoidf(zz[i]) : dy[i];
-            pw_s[w][s][j] = make_float4(sp[i], sp[i] * u[i], ds[i], 0.f);
+            const unsigned bad = dv && t0 + 4 * i + g < end ? 0u : OOB;
+            ru[i] = R::load(xu.rsrc(), ou | bad, i * xu.four);
+            rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
+            ry[i] = R::load(xy.rsrc(), oy | bad, i * xy.four);
+            if (p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
         }
-        stage_bc<T, NS>(p, b, t0, end, lane, bc_s[w]);
-        const unsigned rm = reset_mask(p, b, t0, end, lane);
-        wave_sync();
-        float yq[4], gb[4], wa[4], dAc[NS];
+        st.fetch(end - t0);
+        rr = fetch_resets(p, b, t0, end, lane);
+        get_states<NS>(ck + so, hc, g * NS, p.N, dv, ck4);
+        xu.back(); xd.back(); xz.back(); xy.back(); st.B.back(); st.C.back(); ck -= BDN;
+    };
+    // sums of the block's four waves over a finished chunk's dB, dC
+    const long long prow = p.B * gridDim.x * 2 * NP;        // partials of a step
+    auto put_partials = [&](int t0, const float (*red)[KC * 2 * NP]) {
+        constexpr int RS = 256 / (2 * NP);                  // steps that the block covers at a time
+        const int x = threadIdx.x % (2 * NP), y = threadIdx.x / (2 * NP);
+        float* q = part_bc + (t0 + y) * prow + ((long long)b * gridDim.x + blockIdx.x) * (2 * NP) + x;
+#pragma unroll
+        for (int k = 0; k < KC / RS; ++k) {
+            const int e = k * 256 + threadIdx.x;
+            if (t0 + y + k * RS < tb) q[k * RS * prow] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+        }
+    };
+    fetch(t_last);
+    int c = 0;
+    for (int t0 = t_last; t0 >= ta; t0 -= KC, ++c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const bool ok = dv && t0 + 4 * i + g < end;
+            const float u = R::value(ru[i]), dy = R::value(ry[i]);
+            float sp = R::value(rd[i]) + bias, ds = dy, sg = 1.f, z = 0.f;
+            if (p.softplus) {
+                const float e = exp_neg_abs(sp);
+                sg = sigmoid_from(sp, e);
+                sp = softplus_from(sp, e);
+            }
+            sp = ok ? sp : 0.f;
+            if (p.z) { z = R::value(rz[i]); ds *= z * sigmoidf(z); }
+            pw_s[w][4 * i + g][j] = make_float4(sp * LOG2E, sp * u, ds, u);
+            ex_s[w][4 * i + g][j] = make_float4(z, dy, sg, 0.f);
+        }
+        float* bcb = bc_s[c & 1];
+        st.put(bcb);
+        const unsigned rm = reset_mask(rr);
+        float hs[KH + 1][NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) hs[0][i] = hc[i];
+        auto next = [&] {
+            asm volatile("" ::: "memory");                  // not earlier
+            if (t0 > ta) fetch(t0 - KC);
+        };
+        block_sync_lds();
+        if (c) put_partials(t0 + KC, red_s[(c - 1) & 1]);
+        float gb[4], wa[4], dAc[NS];
 #pragma unroll
         for (int i = 0; i < NS; ++i) dAc[i] = 0.f;
-        // pieces of KH steps, last one first: the states are run up to the piece, then kept through it
-        for (int s0 = KC - KH; s0 >= 0; s0 -= KH) {
-            float hs[KH + 1][NS], a[KH][NS];
-            const float* c = p.ckpt + (long long)(t0 / KC) * p.B * p.D * p.N + so;
+        float* red = red_s[c & 1][w];
+        if constexpr (KH == KC) {
+            if (rm) bwd_piece<NS, KH, true>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, next);
+            else bwd_piece<NS, KH, false>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, next);
+        } else {
+#pragma unroll 1
+            for (int s = 0; s < KC - KH; ++s) {             // the states before each piece
+                if (s % KH == 0) {
 #pragma unroll
-            for (int i = 0; i < NS; ++i) hs[0][i] = dv && g * NS + i < p.N ? c[i] : 0.f;
-            for (int s = 0; s < s0; ++s) {
+                    for (int i = 0; i < NS; ++i) mid_s[w][s / KH][i][lane] = hs[0][i];
+                }
                 const float4 pw = pw_s[w][s][j];
-                const float* bc = bc_s[w] + s * 2 * NP + g * NS;
+                float Bv[NS];
+                lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
                 const bool rs = rm >> s & 1;
 #pragma unroll
-                for (int i = 0; i < NS; ++i)
-                    hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * (An[i] * LOG2E)), rs ? 0.f : hs[0][i], pw.y * bc[i]);
+                for (int i = 0; i < NS; ++i) hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * An[i]), rs ? 0.f : hs[0][i], pw.y * Bv[i]);
             }
-            float part[4];
+#pragma unroll 1
+            for (int s0 = KC - KH; s0 >= 0; s0 -= KH) {
+                bwd_piece<NS, KH, true>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, [&] { if (!s0) next(); });
+                if (s0) {
 #pragma unroll
-            for (int k = 0; k < KH; ++k) {
-                const int s = s0 + k;
-                const float4 pw = pw_s[w][s][j];
-                const float* bc = bc_s[w] + s * 2 * NP + g * NS;
-                const bool rs = rm >> s & 1;                // hs[k] stays: dC of the step before needs it
-                float acc = 0.f;
-#pragma unroll
-                for (int i = 0; i < NS; ++i) {
-                    a[k][i] = __builtin_amdgcn_exp2f(pw.x * (An[i] * LOG2E));
-                    hs[k + 1][i] = fmaf(a[k][i], rs ? 0.f : hs[k][i], pw.y * bc[i]);
-                    acc = fmaf(bc[NP + i], hs[k + 1][i], acc);
-                }
-                part[k & 3] = acc;
-                if ((k & 3) == 3) {
-                    float sy = sum_groups(part[0], part[1], part[2], part[3]);
-                    pin(sy);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) if (i == s / 4) yq[i] = sy;
-                }
-            }
-            int again = 0;                                  // hides that B, C and the step's scalars are read a second time:
-            asm volatile("" : "+v"(again));                 // kept from the first, they would fill the registers
-            float pb[4], pa[4];
-#pragma unroll
-            for (int k = KH - 2; k >= 0; k -= 2) {          // two steps at a time: k + 1, then k
-                float vB[2][NS], vC[2][NS];
-#pragma unroll
-                for (int o = 1; o >= 0; --o) {
-                    const int s = s0 + k + o, c = (k + o) & 3;
-                    const float4 pw = pw_s[w][s][j + again];
-                    const float* bc = bc_s[w] + s * 2 * NP + g * NS + again;
-                    const bool rs = rm >> s & 1;
-                    pb[c] = 0.f; pa[c] = 0.f;
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) {
-                        const float gh = fmaf(pw.z, bc[NP + i], G[i]);
-                        vB[o][i] = gh * pw.y;
-                        vC[o][i] = pw.z * hs[k + o + 1][i];
-                        pb[c] = fmaf(gh, bc[i], pb[c]);
-                        const float q = rs ? 0.f : gh * a[k + o][i], x = q * hs[k + o][i];
-                        G[i] = q;
-                        pa[c] = fmaf(x, An[i], pa[c]);
-                        dAc[i] = fmaf(x, pw.x, dAc[i]);
-                        pin(dAc[i]);
-                    }
-                    pin(pb[c]); pin(pa[c]);
-                }
-                float* red = red_s[w] + (s0 + k + (j >> 2 & 1)) * 2 * NP + (j >> 3) * NP + g * NS;
-#pragma unroll
-                for (int i = 0; i < NS; i += 2) {
-                    float r[2];
-                    sum_rows2({vB[0][i], vB[0][i + 1]}, {vC[0][i], vC[0][i + 1]}, {vB[1][i], vB[1][i + 1]}, {vC[1][i], vC[1][i + 1]}, r);
-                    if ((j & 3) == 0) { red[i] = r[0]; red[i + 1] = r[1]; }
-                }
-                if ((k & 3) == 0) {
-                    float sb = sum_groups(pb[0], pb[1], pb[2], pb[3]), sa = sum_groups(pa[0], pa[1], pa[2], pa[3]);
-                    pin(sb); pin(sa);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) if (i == (s0 + k) / 4) { gb[i] = sb; wa[i] = sa; }
+                    for (int i = 0; i < NS; ++i) hs[0][i] = mid_s[w][s0 / KH - 1][i][lane];
                 }
             }
         }
@@ -418,64 +621,73 @@ __global__ __launch_bounds__(256, 2) void k_ssm_bwd(SsmArgs p, int seg_len, cons
         float dDc = 0.f, dbc = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            const float4 pw = pw_s[w][4 * i + g][j], ex = ex_s[w][4 * i + g][j];
             const int t = t0 + 4 * i + g;
-            const float dpre = fmaf(u[i], gb[i], wa[i]) * sg[i];
-            dDc = fmaf(ds[i], u[i], dDc);
+            const float dpre = t < end ? fmaf(pw.w, gb[i], wa[i]) * ex.z : 0.f;
+            dDc = fmaf(pw.z, pw.w, dDc);
             dbc += dpre;
-            if (!dv || t >= p.T) continue;
-            st((T*)p.du + t * p.du_t + b * p.du_b + d, fmaf(Dd, ds[i], sp[i] * gb[i]));
-            st((T*)p.ddt + t * p.ddt_t + b * p.ddt_b + d, dpre);
+            const unsigned bad = dv && t < p.T ? 0u : OOB;
+            R::store(wu.rsrc(), odu | bad, i * wu.four, t < end ? fmaf(Dd, pw.z, pw.x * LN2 * gb[i]) : 0.f);
+            R::store(wd.rsrc(), odd | bad, i * wd.four, dpre);
             if (p.z) {
-                const float sz = sigmoidf(zz[i]);
-                st((T*)p.dz + t * p.dz_t + b * p.dz_b + d, t < end ? dy[i] * fmaf(Dd, u[i], yq[i]) * sz * (1.f + zz[i] * (1.f - sz)) : 0.f);
+                const float sz = sigmoidf(ex.x);
+                R::store(wz.rsrc(), odz | bad, i * wz.four, t < end ? ex.y * fmaf(Dd, pw.w, ex.w) * sz * (1.f + ex.x * (1.f - sz)) : 0.f);
             }
         }
         dD += dDc; dbias += dbc;
-        __syncthreads();
-        for (int e = threadIdx.x; e < KC * 2 * NP; e += 256) {
-            const int t = t0 + e / (2 * NP);
-            if (t < p.T)
-                part_bc[(((long long)t * p.B + b) * gridDim.x + blockIdx.x) * (2 * NP) + e % (2 * NP)] =
-                    (red_s[0][e] + red_s[1][e]) + (red_s[2][e] + red_s[3][e]);
-        }
-        __syncthreads();
+        wu.back(); wd.back(); wz.back();
+        wave_sync();
     }
+    block_sync_lds();
+    put_partials(ta, red_s[(c - 1) & 1]);
     dD += __shfl_xor(dD, 16, WAVE); dD += __shfl_xor(dD, 32, WAVE);
     dbias += __shfl_xor(dbias, 16, WAVE); dbias += __shfl_xor(dbias, 32, WAVE);
     if (!dv) return;
 #pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        if (g * NS + i >= p.N) continue;
-        part_a[(long long)blockIdx.z * p.B * p.D * p.N + so + i] = dA[i];
-        if (p.dh0 && blockIdx.z == 0) p.dh0[so + i] = G[i];
-    }
-    if (g == 0) {
-        const long long r = (long long)blockIdx.z * p.B + b;
-        part_d[r * p.D + d] = dD;
-        part_d[((long long)gridDim.z * p.B + r) * p.D + d] = dbias;
-    }
+    for (int i = 0; i < NS; ++i) dA[i] *= LN2;              // the step sizes were carried times log2(e)
+    // a row of partials: dA [D, N], dD [D], dbias [D]
+    const long long cols = p.D * (p.N + 2);
+    float* q = part_a + ((long long)blockIdx.z * p.B + b) * cols;
+    put_states<NS>(q + (long long)d * p.N + g * NS, dA, g * NS, p.N, vec4(q, p.N));
+    if (p.dh0 && blockIdx.z == 0) put_states<NS>(p.dh0 + so, G, g * NS, p.N, vec4(p.dh0, p.N));
+    if (g == 0) { q[p.D * p.N + d] = dD; q[p.D * (p.N + 1) + d] = dbias; }
 }
 
-// out[i] = sum over r < R of part[r][i], in order
-__global__ void k_sum_rows(const float* __restrict__ part, int R, long long n, float* __restrict__ out) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n) return;
-    float v = 0.f;
-    for (int r = 0; r < R; ++r) v += part[r * n + i];
-    out[i] = v;
-}
+// Second launch of the backward: blocks [0, n_bc) add the channel blocks' partials of dB and dC, the others the rows' partials
+// of dA, dD and the bias, 32 columns by 8 groups of rows each, all in a fixed order.
 template <typename T>
-__global__ void k_ssm_sum_bc(SsmArgs p, const float* __restrict__ part, int nblk, int NP) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const long long row = i / (2 * p.N);
-    if (row >= p.T * p.B) return;
-    const int c = (int)(i % (2 * p.N)), isC = c >= p.N, n = isC ? c - (int)p.N : c;
-    const float* q = part + row * nblk * 2 * NP + isC * NP + n;
+__global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __restrict__ part_bc, int nblk, int NP, unsigned n_bc,
+                                                    const float* __restrict__ part_a, int rows) {
+    if (blockIdx.x < n_bc) {
+        const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / (2 * p.N);
+        if (row >= p.T * p.B) return;
+        const int c = (int)(i - row * 2 * p.N), isC = c >= p.N, n = isC ? c - (int)p.N : c;
+        const float* q = part_bc + row * nblk * 2 * NP + isC * NP + n;
+        float v = 0.f;
+#pragma unroll 4
+        for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
+        const long long t = row / p.B, b = row - t * p.B;
+        if (isC) st((T*)p.dCm + t * p.dC_t + b * p.dC_b + n, v);
+        else st((T*)p.dBm + t * p.dB_t + b * p.dB_b + n, v);
+        return;
+    }
+    __shared__ float acc[8][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long long DN = p.D * p.N, cols = DN + 2 * p.D, i = (long long)(blockIdx.x - n_bc) * 32 + x;
     float v = 0.f;
-    for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
-    const long long t = row / p.B, b = row % p.B;
-    if (isC) st((T*)p.dCm + t * p.dC_t + b * p.dC_b + n, v);
-    else st((T*)p.dBm + t * p.dB_t + b * p.dB_b + n, v);
+    if (i < cols) {
+#pragma unroll 4
+        for (int r = y; r < rows; r += 8) v += part_a[r * cols + i];
+    }
+    acc[y][x] = v;
+    __syncthreads();
+    if (y || i >= cols) return;
+    v = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v += acc[k][x];
+    if (i < DN) p.dA[i] = v;
+    else if (i < DN + p.D) { if (p.dD) p.dD[i - DN] = v; }
+    else if (p.dbias) p.dbias[i - DN - p.D] = v;
 }
 
 // One step: h [B, D, N] is read and written once, the rest is small. A thread per (row, channel).
@@ -520,7 +732,7 @@ static Segs segments(long long T, long long B, long long D) {
 
 // floats of scratch that a forward (train = 0) or a forward and its backward (1) need
 DRL_API int drl_ssm_ws(long long T, long long B, long long D, long long N, int train, long long* n) {
-    if (T <= 0 || T >= (1ll << 31) || B <= 0 || D <= 0 || N <= 0 || N > 64 || B > 65535) return -1;
+    if (T <= 0 || T >= (1ll << 31) || B <= 0 || D <= 0 || D >= (1ll << 25) || N <= 0 || N > 64 || B > 65535 || T * B > (1ll << 31)) return -1;
     const long long nblk = (D + 63) / 64, S = segments(T, B, D).n;
     *n = S > 1 ? S * B * D * (N + 1) : 0;
     if (train) *n += T * B * nblk * 8 * ns_of(N) + S * B * D * (N + 2);
@@ -551,13 +763,9 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
     const long long rows = sg.n * p.B;
     float* part_bc = p.ws + (sg.n > 1 ? rows * p.D * (p.N + 1) : 0);
     float* part_a = part_bc + p.T * p.B * nblk * 2 * NP;
-    float* part_d = part_a + rows * p.D * p.N;
-    k_ssm_bwd<T, NS><<<dim3((unsigned)nblk, (unsigned)p.B, (unsigned)sg.n), 256, 0, s>>>(p, sg.len, carry, part_bc, part_a, part_d);
-    const long long nbc = p.T * p.B * 2 * p.N, na = p.D * p.N;
-    k_ssm_sum_bc<T><<<(unsigned)((nbc + 255) / 256), 256, 0, s>>>(p, part_bc, nblk, NP);
-    k_sum_rows<<<(unsigned)((na + 255) / 256), 256, 0, s>>>(part_a, (int)rows, na, p.dA);
-    if (p.dD) k_sum_rows<<<(unsigned)((p.D + 255) / 256), 256, 0, s>>>(part_d, (int)rows, p.D, p.dD);
-    if (p.dbias) k_sum_rows<<<(unsigned)((p.D + 255) / 256), 256, 0, s>>>(part_d + rows * p.D, (int)rows, p.D, p.dbias);
+    k_ssm_bwd<T, NS><<<dim3((unsigned)nblk, (unsigned)p.B, (unsigned)sg.n), 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
+    const unsigned n_bc = (unsigned)((p.T * p.B * 2 * p.N + 255) / 256), n_a = (unsigned)((p.D * (p.N + 2) + 31) / 32);
+    k_ssm_finish<T><<<n_bc + n_a, 256, 0, s>>>(p, part_bc, nblk, NP, n_bc, part_a, (int)rows);
 }
 
 #define SSM_NS(NAME, T)                       \

@@ -1249,6 +1249,8 @@ def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None,
     rp, lp = _vec(reset, (T, B), torch.uint8, dev, "reset"), _vec(lengths, (B,), torch.int32, dev, "lengths")
     ck = _vec(ckpt, ((T + SSM_CHUNK - 1) // SSM_CHUNK, B, Dc, N), f32, dev, "ckpt")
     wsp = _vec(ws, (ws.numel(),), f32, dev, "ws")
+    if T > 1 and max(r[1] for r in (ur, dtr, zr, Br, Cr, yr, dyr, dur, ddtr, dzr)) >= 1 << 25:
+        raise ValueError("ssm_scan: steps of one tensor are 2^25 elements or more apart")
     ins = (ur[0], dtr[0], zr[0], Br[0], Cr[0], Ap, Dp, bp, h0p, rp, lp, dyr[0], dhTp)
     _apart((yr[0], hTp, ck, wsp if ws.numel() else 0, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0], dAp, dDp, dbp, dh0p), ins)
     return _SSM.pack(ur[0], dtr[0], zr[0], Br[0], Cr[0], *ur[1:], *dtr[1:], *zr[1:], *Br[1:], *Cr[1:], Ap, Dp, bp, h0p, rp, lp, *yr,
