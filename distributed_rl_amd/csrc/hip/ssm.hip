@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
         const bool last = k == S - 1;
         const float e = last ? 0.f : carry[s * n + i], sum = last ? 0.f : sums[s * p.B * p.D + r];
         carry[s * n + i] = h;
-        h = fmaf(sum == __builtin_inff() ? 0.f : __builtin_amdgcn_exp2f(sum * A2), h, e);
+        h = sum == __builtin_inff() ? e : fmaf(__builtin_amdgcn_exp2f(sum * A2), h, e);
     }
 }
 
@@ -358,8 +358,9 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
         rr = fetch_resets(p, b, t0, end, lane);
         xu.next(); xd.next(); xz.next(); st.B.next(); st.C.next();
     };
-    fetch(ta);
-    for (int t0 = ta, c = 0; t0 < tb; t0 += KC, ++c) {
+    const int live = min(tb, end);                          // padding is not walked: its rows are zeroed below
+    if (live > ta) fetch(ta);
+    for (int t0 = ta, c = 0; t0 < live; t0 += KC, ++c) {
         float u[4], zz[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
         float* bcb = bc_s[c & 1];
         st.put(bcb);
         const unsigned rm = reset_mask(rr);
-        if (t0 + KC < tb) fetch(t0 + KC);
+        if (t0 + KC < live) fetch(t0 + KC);
         block_sync_lds();                 // B and C of this chunk are there; the image of the chunk before last is free again
         if (p.ckpt && dv) put_states<NS>(p.ckpt + (t0 / KC) * BDN + so, h, g * NS, p.N, vec4(p.ckpt, p.N));
         float y[4];
@@ -411,6 +412,11 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
         xy.next();
         wave_sync();                                        // the next chunk overwrites this wave's LDS image
     }
+    for (int t0 = ta + (max(live - ta, 0) + KC - 1) / KC * KC; t0 < tb; t0 += KC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) R::store(xy.rsrc(), dv && t0 + 4 * i + g < tb ? oy : OOB, i * xy.four, 0.f);
+        xy.next();
+    }
     if (p.hT && dv && blockIdx.z == gridDim.z - 1) put_states<NS>(p.hT + so, h, g * NS, p.N, vec4(p.hT, p.N));
 }
 
@@ -419,60 +425,68 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
 // of 64 channels (a block), the sums over rows of dA, dD and the bias as partials of a row: second launches add them in a
 // fixed order.
 // KH steps of a chunk, s0 .. s0 + KH - 1, from the state before them: forward with the states and decays kept, then back.
-// mid() is called half way back, when half of those registers are free again: the next chunk's loads start there.
-template <int NS, int KH, bool RS, typename F>
+// mid() is called half way back, when half of those registers are free again: the next chunk's loads start there. emit(s, gB, wA)
+// gets the sums over the states for the lane's own step of each four that are done (s = their first).
+template <int NS, int KH, bool RS, typename F, typename E>
 __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const float* bcb, float* red_w, unsigned rm, int s0, int g, int j,
                                           const float (&An)[NS], float (&hs)[KH + 1][NS], float (&G)[NS], float (&dAc)[NS],
-                                          float4 (&ex_w)[KC][16], float (&gb)[4], float (&wa)[4], F mid) {
+                                          float4 (&ex_w)[KC][16], F mid, E emit) {
     constexpr int NP = 4 * NS;
+    struct In { float4 pw; float B[NS], C[NS]; };           // what a step reads from LDS, fetched a step (two steps) ahead
+    auto load = [&](int s, int again) {
+        In x;
+        x.pw = pw_w[s][j + again];
+        lds_row<NS>(bcb + s * 2 * NP + g * NS + again, x.B);
+        lds_row<NS>(bcb + s * 2 * NP + NP + g * NS + again, x.C);
+        return x;
+    };
     float a[KH][NS], part[4];
+    In x = load(s0, 0);
 #pragma unroll
     for (int k = 0; k < KH; ++k) {
-        if ((k & 1) == 0) __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_sched_barrier(0);
         const int s = s0 + k;
-        const float4 pw = pw_w[s][j];
-        float Bv[NS], Cv[NS];
-        lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
-        lds_row<NS>(bcb + s * 2 * NP + NP + g * NS, Cv);
-        const bool rs = RS && (rm >> s & 1);        // hs[k] stays: dC of the step before needs it
+        In nx;
+        if (k + 1 < KH) nx = load(s + 1, 0);
+        const bool rs = RS && (rm >> s & 1);        // hs[k] itself stays: dC of the step before needs it
         float acc = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            a[k][i] = __builtin_amdgcn_exp2f(pw.x * An[i]);
-            hs[k + 1][i] = fmaf(a[k][i], rs ? 0.f : hs[k][i], pw.y * Bv[i]);
-            acc = fmaf(Cv[i], hs[k + 1][i], acc);
+            const float e = __builtin_amdgcn_exp2f(x.pw.x * An[i]), in = x.pw.y * x.B[i], n = fmaf(e, hs[k][i], in);
+            a[k][i] = rs ? 0.f : e;
+            hs[k + 1][i] = rs ? in : n;
+            acc = fmaf(x.C[i], hs[k + 1][i], acc);
         }
         part[k & 3] = acc;
-        if ((k & 3) == 3) {
-            ex_w[s - 3 + g][j].w = sum_groups(part[0], part[1], part[2], part[3]);
-        }
+        if ((k & 3) == 3) ex_w[s - 3 + g][j].w = sum_groups(part[0], part[1], part[2], part[3]);
+        if (k + 1 < KH) x = nx;
     }
     int again = 0;                                  // hides that B, C and the step's scalars are read a second time:
     asm volatile("" : "+v"(again));                 // kept from the first, they would fill the registers
     float pb[4], pa[4];
+    In xs[2] = {load(s0 + KH - 2, again), load(s0 + KH - 1, again)};
 #pragma unroll
     for (int k = KH - 2; k >= 0; k -= 2) {          // two steps at a time: k + 1, then k
         float vB[2][NS], vC[2][NS];
+        __builtin_amdgcn_sched_barrier(0);
         if (k == KH / 2 - 2 || (KH == 4 && k == 0)) mid();
+        In nx[2];
+        if (k >= 2) { nx[1] = load(s0 + k - 1, again); nx[0] = load(s0 + k - 2, again); }
 #pragma unroll
         for (int o = 1; o >= 0; --o) {
-            const int s = s0 + k + o, c = (k + o) & 3;
-            const float4 pw = pw_w[s][j + again];
-            float Bv[NS], Cv[NS];
-            lds_row<NS>(bcb + s * 2 * NP + g * NS + again, Bv);
-            lds_row<NS>(bcb + s * 2 * NP + NP + g * NS + again, Cv);
-            const bool rs = RS && (rm >> s & 1);
+            const int c = (k + o) & 3;
+            const float4 pw = xs[o].pw;
             pb[c] = 0.f; pa[c] = 0.f;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                const float gh = fmaf(pw.z, Cv[i], G[i]);
+                const float gh = fmaf(pw.z, xs[o].C[i], G[i]);
                 vB[o][i] = gh * pw.y;
                 vC[o][i] = pw.z * hs[k + o + 1][i];
-                pb[c] = fmaf(gh, Bv[i], pb[c]);
-                const float q = rs ? 0.f : gh * a[k + o][i], x = q * (rs ? 0.f : hs[k + o][i]);
+                pb[c] = fmaf(gh, xs[o].B[i], pb[c]);
+                const float q = gh * a[k + o][i], y = q * hs[k + o][i];
                 G[i] = q;
-                pa[c] = fmaf(x, An[i], pa[c]);
-                dAc[i] = fmaf(x, pw.x, dAc[i]);
+                pa[c] = fmaf(y, An[i], pa[c]);
+                dAc[i] = fmaf(y, pw.x, dAc[i]);
                 pin(dAc[i]);
             }
             pin(pb[c]); pin(pa[c]);
@@ -485,22 +499,21 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
             red[j & 1] = sum_rows2(vB[0], vC[0], vB[1], vC[1], j);
         }
         if ((k & 3) == 0) {
-            float sb = sum_groups(pb[0], pb[1], pb[2], pb[3]), sa = sum_groups(pa[0], pa[1], pa[2], pa[3]);
-            pin(sb); pin(sa);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) if (i == (s0 + k) / 4) { gb[i] = sb; wa[i] = sa; }
+            emit(s0 + k, sum_groups(pb[0], pb[1], pb[2], pb[3]), sum_groups(pa[0], pa[1], pa[2], pa[3]));
         }
+        if (k >= 2) { xs[0] = nx[0]; xs[1] = nx[1]; }
     }
 }
 
-template <typename T, int NS>
+// HAS: the call has reset flags. (A branch on each chunk's flags instead holds the registers of both paths: spills.)
+template <typename T, int NS, bool HAS>
 __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
                                                     float* __restrict__ part_bc, float* __restrict__ part_a) {
     constexpr int NP = 4 * NS;
-    constexpr int KH = NS > 4 ? 4 : KC;                     // steps whose states are held at a time
+    constexpr int KH = NS > 4 ? 4 : NS == 4 ? 8 : KC;                   // steps whose states are held at a time
     using R = Rows<T>;
     __shared__ __align__(16) float4 pw_s[4][KC][16];        // s log2(e), s u, ds, u
-    __shared__ __align__(16) float4 ex_s[4][KC][16];        // z, dy, ds/d(pre), sum_n C h
+    __shared__ __align__(16) float4 ex_s[4][KC][16];        // dy silu'(z), -, ds/d(pre), sum_n C h
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
     __shared__ float mid_s[KH < KC ? 4 : 1][KH < KC ? KC / KH - 1 : 1][KH < KC ? NS : 1][64];      // states before each piece
@@ -520,11 +533,13 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     }
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
     float dD = 0.f, dbias = 0.f;
+    const bool has_z = p.z != nullptr, soft = p.softplus != 0;
+    const int n_t = (int)p.T;
     const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.dy_t, g, d);
     const unsigned odu = R::offset(p.du_t, g, d), odd = R::offset(p.ddt_t, g, d), odz = R::offset(p.dz_t, g, d);
     unsigned ru[4], rd[4], rz[4], ry[4], rr;
     float hc[NS];
-    const int t_last = ta + (tb - ta - 1) / KC * KC;
+    const int live = min(tb, end), t_last = ta + max(live - ta - 1, 0) / KC * KC;       // padding is not walked, see below
     R xu(p.u, p.u_t, p.u_b, b, t_last), xd(p.dt, p.dt_t, p.dt_b, b, t_last), xz(p.z, p.z_t, p.z_b, b, t_last), xy(p.dy, p.dy_t, p.dy_b, b, t_last);
     R wu(p.du, p.du_t, p.du_b, b, t_last), wd(p.ddt, p.ddt_t, p.ddt_b, b, t_last), wz(p.dz, p.dz_t, p.dz_b, b, t_last);
     StageBC<T, NS, 3> st(p, b, t_last);
@@ -537,10 +552,10 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
             ru[i] = R::load(xu.rsrc(), ou | bad, i * xu.four);
             rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
             ry[i] = R::load(xy.rsrc(), oy | bad, i * xy.four);
-            if (p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
+            if (has_z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
         }
         st.fetch(end - t0);
-        rr = fetch_resets(p, b, t0, end, lane);
+        if (HAS) rr = fetch_resets(p, b, t0, end, lane);
         get_states<NS>(ck + so, hc, g * NS, p.N, dv, ck4);
         xu.back(); xd.back(); xz.back(); xy.back(); st.B.back(); st.C.back(); ck -= BDN;
     };
@@ -553,46 +568,70 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
 #pragma unroll
         for (int k = 0; k < KC / RS; ++k) {
             const int e = k * 256 + threadIdx.x;
-            if (t0 + y + k * RS < tb) q[k * RS * prow] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+            if (t0 + y + k * RS < live) q[k * RS * prow] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
         }
     };
-    fetch(t_last);
+    for (int t0 = live > ta ? t_last + KC : ta; t0 < tb; t0 += KC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const unsigned bad = dv && t0 + 4 * i + g < tb ? 0u : OOB;
+            const R qu(p.du, p.du_t, p.du_b, b, t0), qd(p.ddt, p.ddt_t, p.ddt_b, b, t0), qz(p.dz, p.dz_t, p.dz_b, b, t0);
+            R::store(qu.rsrc(), odu | bad, i * qu.four, 0.f);
+            R::store(qd.rsrc(), odd | bad, i * qd.four, 0.f);
+            if (has_z) R::store(qz.rsrc(), odz | bad, i * qz.four, 0.f);
+        }
+    }
+    if (live > ta) fetch(t_last);
     int c = 0;
-    for (int t0 = t_last; t0 >= ta; t0 -= KC, ++c) {
+    for (int t0 = live > ta ? t_last : ta - 1; t0 >= ta; t0 -= KC, ++c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const bool ok = dv && t0 + 4 * i + g < end;
             const float u = R::value(ru[i]), dy = R::value(ry[i]);
-            float sp = R::value(rd[i]) + bias, ds = dy, sg = 1.f, z = 0.f;
-            if (p.softplus) {
+            float sp = R::value(rd[i]) + bias, ds = dy, sg = 1.f, dz = 0.f;
+            if (soft) {
                 const float e = exp_neg_abs(sp);
                 sg = sigmoid_from(sp, e);
                 sp = softplus_from(sp, e);
             }
             sp = ok ? sp : 0.f;
-            if (p.z) { z = R::value(rz[i]); ds *= z * sigmoidf(z); }
+            if (has_z) {
+                const float z = R::value(rz[i]), sz = sigmoidf(z);
+                ds = dy * (z * sz);
+                dz = dy * sz * fmaf(z, 1.f - sz, 1.f);
+            }
             pw_s[w][4 * i + g][j] = make_float4(sp * LOG2E, sp * u, ds, u);
-            ex_s[w][4 * i + g][j] = make_float4(z, dy, sg, 0.f);
+            ex_s[w][4 * i + g][j] = make_float4(dz, 0.f, sg, 0.f);
         }
         float* bcb = bc_s[c & 1];
         st.put(bcb);
-        const unsigned rm = reset_mask(rr);
+        const unsigned rm = HAS ? reset_mask(rr) : 0;
         float hs[KH + 1][NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) hs[0][i] = hc[i];
+        for (int i = 0; i < NS; ++i) hs[0][i] = HAS && (rm & 1) ? 0.f : hc[i];
         auto next = [&] {
             asm volatile("" ::: "memory");                  // not earlier
             if (t0 > ta) fetch(t0 - KC);
         };
         block_sync_lds();
         if (c) put_partials(t0 + KC, red_s[(c - 1) & 1]);
-        float gb[4], wa[4], dAc[NS];
+        float dAc[NS], dDc = 0.f, dbc = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) dAc[i] = 0.f;
         float* red = red_s[c & 1][w];
+        auto emit = [&](int s, float gB, float wA) {
+            const float4 pw = pw_s[w][s + g][j], ex = ex_s[w][s + g][j];
+            const int t = t0 + s + g;
+            const float dpre = t < end ? fmaf(pw.w, gB, wA) * ex.z : 0.f;
+            dDc = fmaf(pw.z, pw.w, dDc);
+            dbc += dpre;
+            const unsigned bad = dv && t < n_t ? 0u : OOB;
+            R::store(wu.rsrc(), odu | bad, (unsigned)(s / 4) * wu.four, t < end ? fmaf(Dd, pw.z, pw.x * LN2 * gB) : 0.f);
+            R::store(wd.rsrc(), odd | bad, (unsigned)(s / 4) * wd.four, dpre);
+            if (has_z) R::store(wz.rsrc(), odz | bad, (unsigned)(s / 4) * wz.four, t < end ? ex.x * fmaf(Dd, pw.w, ex.w) : 0.f);
+        };
         if constexpr (KH == KC) {
-            if (rm) bwd_piece<NS, KH, true>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, next);
-            else bwd_piece<NS, KH, false>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, next);
+            bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], next, emit);
         } else {
 #pragma unroll 1
             for (int s = 0; s < KC - KH; ++s) {             // the states before each piece
@@ -603,13 +642,13 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
                 const float4 pw = pw_s[w][s][j];
                 float Bv[NS];
                 lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
-                const bool rs = rm >> s & 1;
+                const bool rs = HAS && (rm >> s & 1);
 #pragma unroll
                 for (int i = 0; i < NS; ++i) hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * An[i]), rs ? 0.f : hs[0][i], pw.y * Bv[i]);
             }
 #pragma unroll 1
             for (int s0 = KC - KH; s0 >= 0; s0 -= KH) {
-                bwd_piece<NS, KH, true>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], gb, wa, [&] { if (!s0) next(); });
+                bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], [&] { if (!s0) next(); }, emit);
                 if (s0) {
 #pragma unroll
                     for (int i = 0; i < NS; ++i) hs[0][i] = mid_s[w][s0 / KH - 1][i][lane];
@@ -618,28 +657,14 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) dA[i] += dAc[i];
-        float dDc = 0.f, dbc = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float4 pw = pw_s[w][4 * i + g][j], ex = ex_s[w][4 * i + g][j];
-            const int t = t0 + 4 * i + g;
-            const float dpre = t < end ? fmaf(pw.w, gb[i], wa[i]) * ex.z : 0.f;
-            dDc = fmaf(pw.z, pw.w, dDc);
-            dbc += dpre;
-            const unsigned bad = dv && t < p.T ? 0u : OOB;
-            R::store(wu.rsrc(), odu | bad, i * wu.four, t < end ? fmaf(Dd, pw.z, pw.x * LN2 * gb[i]) : 0.f);
-            R::store(wd.rsrc(), odd | bad, i * wd.four, dpre);
-            if (p.z) {
-                const float sz = sigmoidf(ex.x);
-                R::store(wz.rsrc(), odz | bad, i * wz.four, t < end ? ex.y * fmaf(Dd, pw.w, ex.w) * sz * (1.f + ex.x * (1.f - sz)) : 0.f);
-            }
-        }
         dD += dDc; dbias += dbc;
         wu.back(); wd.back(); wz.back();
         wave_sync();
     }
-    block_sync_lds();
-    put_partials(ta, red_s[(c - 1) & 1]);
+    if (c) {
+        block_sync_lds();
+        put_partials(ta, red_s[(c - 1) & 1]);
+    }
     dD += __shfl_xor(dD, 16, WAVE); dD += __shfl_xor(dD, 32, WAVE);
     dbias += __shfl_xor(dbias, 16, WAVE); dbias += __shfl_xor(dbias, 32, WAVE);
     if (!dv) return;
@@ -663,10 +688,12 @@ __global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __re
         if (row >= p.T * p.B) return;
         const int c = (int)(i - row * 2 * p.N), isC = c >= p.N, n = isC ? c - (int)p.N : c;
         const float* q = part_bc + row * nblk * 2 * NP + isC * NP + n;
-        float v = 0.f;
-#pragma unroll 4
-        for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
         const long long t = row / p.B, b = row - t * p.B;
+        float v = 0.f;
+        if (t < row_end(p, (int)b)) {                       // padding has no partials
+#pragma unroll 4
+            for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
+        }
         if (isC) st((T*)p.dCm + t * p.dC_t + b * p.dC_b + n, v);
         else st((T*)p.dBm + t * p.dB_t + b * p.dB_b + n, v);
         return;
@@ -763,7 +790,9 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
     const long long rows = sg.n * p.B;
     float* part_bc = p.ws + (sg.n > 1 ? rows * p.D * (p.N + 1) : 0);
     float* part_a = part_bc + p.T * p.B * nblk * 2 * NP;
-    k_ssm_bwd<T, NS><<<dim3((unsigned)nblk, (unsigned)p.B, (unsigned)sg.n), 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
+    const dim3 grid((unsigned)nblk, (unsigned)p.B, (unsigned)sg.n);
+    if (p.reset) k_ssm_bwd<T, NS, true><<<grid, 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
+    else k_ssm_bwd<T, NS, false><<<grid, 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
     const unsigned n_bc = (unsigned)((p.T * p.B * 2 * p.N + 255) / 256), n_a = (unsigned)((p.D * (p.N + 2) + 31) / 32);
     k_ssm_finish<T><<<n_bc + n_a, 256, 0, s>>>(p, part_bc, nblk, NP, n_bc, part_a, (int)rows);
 }

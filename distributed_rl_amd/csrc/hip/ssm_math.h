@@ -39,4 +39,5 @@ __device__ __forceinline__ float sigmoid_from(float x, float e) {
     const float r = __builtin_amdgcn_rcpf(1.0f + e);
     return x >= 0.f ? r : e * r;
 }
-__device__ __forceinline__ float sigmoidf(float x) { return sigmoid_from(x, exp_neg_abs(x)); }
+// for gates: exp's error of |x| half steps stands next to 1, or where the gate is nearly shut
+__device__ __forceinline__ float sigmoidf(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -LOG2E)); }
