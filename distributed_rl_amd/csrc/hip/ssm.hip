@@ -71,13 +71,13 @@ struct Rows {
 // fp32, [step][B: NP | C: NP], zeros beyond N and beyond the row's end. WHICH: 1 = B, 2 = C, 3 = both.
 template <typename T, int NS, int WHICH>
 struct StageBC {
-    static constexpr int NP = 4 * NS, NV = KC * NP > 256 ? KC * NP / 256 : 1, ROW = WHICH == 3 ? 2 * NP : NP, STEP = 256 / NP;
+    static constexpr int NP = 4 * NS, STEP = 256 / NP < KC ? 256 / NP : KC, NV = (KC + STEP - 1) / STEP, ROW = WHICH == 3 ? 2 * NP : NP;
     Rows<T> B, C;
     unsigned ob, oc, rb[WHICH & 1 ? NV : 1], rc[WHICH & 2 ? NV : 1];
     __device__ __forceinline__ StageBC(const SsmArgs& p, int b, int t0)
         : B(p.Bm, p.B_t, p.B_b, b, t0), C(p.Cm, p.C_t, p.C_b, b, t0) {
         const int n = threadIdx.x % NP, s = threadIdx.x / NP;
-        const bool in = n < p.N && s < KC;
+        const bool in = n < p.N && s < STEP;
         ob = in ? Rows<T>::offset(p.B_t, s, n) : OOB;
         oc = in ? Rows<T>::offset(p.C_t, s, n) : OOB;
     }
@@ -86,16 +86,17 @@ struct StageBC {
         const int s = threadIdx.x / NP;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
-            const unsigned bad = s + k * STEP < live ? 0u : OOB;
+            const unsigned bad = s + k * STEP < min(live, KC) ? 0u : OOB;
             if (WHICH & 1) rb[k] = Rows<T>::load(B.rsrc(), ob | bad, k * STEP * (B.four / 4));
             if (WHICH & 2) rc[k] = Rows<T>::load(C.rsrc(), oc | bad, k * STEP * (C.four / 4));
         }
     }
     __device__ __forceinline__ void put(float* bc) const {
         const int n = threadIdx.x % NP, s = threadIdx.x / NP;
-        if (KC * NP < 256 && s >= KC) return;
+        if (s >= STEP) return;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
+            if (KC % STEP && s + k * STEP >= KC) break;
             float* q = bc + (s + k * STEP) * ROW + n;
             if (WHICH & 1) *q = Rows<T>::value(rb[k]);
             if (WHICH & 2) q[WHICH == 3 ? NP : 0] = Rows<T>::value(rc[k]);
@@ -313,13 +314,22 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
     const float A2 = p.A[r % p.D * p.N + i % p.N] * LOG2E;
     const float* h0 = BWD ? p.dhT : p.h0;
     float h = h0 ? h0[i] : 0.f;
-#pragma unroll 4
-    for (int k = 0; k < S; ++k) {
-        const int s = BWD ? S - 1 - k : k;
-        const bool last = k == S - 1;
-        const float e = last ? 0.f : carry[s * n + i], sum = last ? 0.f : sums[s * p.B * p.D + r];
-        carry[s * n + i] = h;
-        h = sum == __builtin_inff() ? e : fmaf(__builtin_amdgcn_exp2f(sum * A2), h, e);
+    constexpr int AHEAD = 16;                               // loads in flight: a carry is overwritten only after its batch is read
+    for (int k0 = 0; k0 < S; k0 += AHEAD) {
+        float e[AHEAD], sum[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            const int s = BWD ? S - 1 - k0 - k : k0 + k;
+            const bool in = k0 + k < S - 1;
+            e[k] = in ? carry[s * n + i] : 0.f;
+            sum[k] = in ? sums[s * p.B * p.D + r] : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            if (k0 + k >= S) break;
+            carry[(BWD ? S - 1 - k0 - k : k0 + k) * n + i] = h;
+            h = sum[k] == __builtin_inff() ? e[k] : fmaf(__builtin_amdgcn_exp2f(sum[k] * A2), h, e[k]);
+        }
     }
 }
 
@@ -562,13 +572,13 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     // sums of the block's four waves over a finished chunk's dB, dC
     const long long prow = p.B * gridDim.x * 2 * NP;        // partials of a step
     auto put_partials = [&](int t0, const float (*red)[KC * 2 * NP]) {
-        constexpr int RS = 256 / (2 * NP);                  // steps that the block covers at a time
+        constexpr int RS = 256 / (2 * NP) < KC ? 256 / (2 * NP) : KC;       // steps that the block covers at a time
         const int x = threadIdx.x % (2 * NP), y = threadIdx.x / (2 * NP);
         float* q = part_bc + (t0 + y) * prow + ((long long)b * gridDim.x + blockIdx.x) * (2 * NP) + x;
 #pragma unroll
-        for (int k = 0; k < KC / RS; ++k) {
-            const int e = k * 256 + threadIdx.x;
-            if (t0 + y + k * RS < live) q[k * RS * prow] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
+        for (int k = 0; k < (KC + RS - 1) / RS; ++k) {
+            const int s = y + k * RS, e = s * 2 * NP + x;
+            if (y < RS && s < KC && t0 + s < live) q[k * RS * prow] = (red[0][e] + red[1][e]) + (red[2][e] + red[3][e]);
         }
     };
     for (int t0 = live > ta ? t_last + KC : ta; t0 < tb; t0 += KC) {
@@ -740,16 +750,16 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
     st((T*)p.y + b * p.y_b + d, y);
 }
 
-static int ns_of(long long N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+static int ns_of(long long N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 48 ? 12 : 16; }
 
-// Segments: one where the rows alone give the chip 768 waves, else as many as bring it to 2 048, of at least 64 steps. A cut
+// Segments: one where the rows alone give the chip 768 waves, else as many as bring it to 4 096, of at least 64 steps. A cut
 // costs the carry pass (the recurrence without its read-out), so rows that fill the chip are never cut.
 struct Segs { int n, len; };
 static Segs segments(long long T, long long B, long long D) {
     const long long waves = (D + 15) / 16 * B, chunks = (T + KC - 1) / KC;
     long long n = 1;
     if (waves < 768) {
-        n = (2048 + waves - 1) / waves;
+        n = (4096 + waves - 1) / waves;
         if (n > chunks / 4) n = chunks / 4;
         if (n < 1) n = 1;
     }
@@ -802,6 +812,7 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
         case 2: NAME<T, 2>(p, s); break;      \
         case 4: NAME<T, 4>(p, s); break;      \
         case 8: NAME<T, 8>(p, s); break;      \
+        case 12: NAME<T, 12>(p, s); break;    \
         default: NAME<T, 16>(p, s); break;    \
     }
 
