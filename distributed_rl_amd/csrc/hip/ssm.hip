@@ -154,14 +154,6 @@ __device__ __forceinline__ void get_states(const float* q, float (&h)[NS], int n
 
 // Sums over the four lane groups (rows of 16 lanes): group g ends with the sum of v[g]. Swapping rows adds two values at a
 // time: 3 swaps + 3 adds for four sums, where a butterfly of each value would take 8 of each.
-__device__ __forceinline__ float add_swap16(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);     // rows a0+a1, b0+b1, a2+a3, b2+b3
-}
-__device__ __forceinline__ float add_swap32(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);     // rows a0+a2, a1+a3, b0+b2, b1+b3
-}
 __device__ __forceinline__ float sum_groups(float v0, float v1, float v2, float v3) {
     return add_swap32(add_swap16(v0, v1), add_swap16(v2, v3));
 }

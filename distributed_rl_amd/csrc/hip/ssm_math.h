@@ -41,3 +41,26 @@ __device__ __forceinline__ float sigmoid_from(float x, float e) {
 }
 // for gates: exp's error of |x| half steps stands next to 1, or where the gate is nearly shut
 __device__ __forceinline__ float sigmoidf(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -LOG2E)); }
+
+// Swapping rows of 16 lanes adds two values at a time.
+__device__ __forceinline__ float add_swap16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);     // rows a0+a1, b0+b1, a2+a3, b2+b3
+}
+__device__ __forceinline__ float add_swap32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);     // rows a0+a2, a1+a3, b0+b2, b1+b3
+}
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+    return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
+}
+// sum over the 64 lanes, in every lane: four adds across neighbours, two row swaps, no trip through LDS
+__device__ __forceinline__ float lane_sum(float v) {
+    v = add_dpp<0xB1>(v);          // quad: lane ^ 1
+    v = add_dpp<0x4E>(v);          // quad: lane ^ 2
+    v = add_dpp<0x141>(v);         // row_half_mirror: the other quad of 8 lanes
+    v = add_dpp<0x140>(v);         // row_mirror: the other 8 lanes
+    v = add_swap16(v, v);
+    return add_swap32(v, v);
+}
