@@ -3,10 +3,12 @@
 // Steps before the first come from state_in [B, W - 1, D]; a set reset flag at t cuts every tap from t on off from the steps
 // before t; steps from lengths[b] on are not read and write zeros.
 //
-// A thread owns one channel of one row and walks SEG steps with the last W - 1 inputs in registers.
+// Bound by memory: a thread owns V neighbouring channels (16 bytes of fp32, 8 of bf16; 1 where addresses or strides do not
+// allow it) of one row and a run of steps, reads BATCH steps ahead and keeps the last W - 1 inputs in registers. Runs of one
+// row are walked side by side; each starts by reading the W - 1 steps before it again.
 #include "ssm_math.h"
 
-#define SEG 16
+#define BATCH 8
 
 struct ConvArgs {        // mirrored by ops/hip.py (_conv_args): 64-bit words in this order
     const void *x, *state_in;
@@ -25,183 +27,337 @@ struct ConvArgs {        // mirrored by ops/hip.py (_conv_args): 64-bit words in
     long long ws_n;
 };
 
+struct ConvGrid { int L, seg, n_seg, rows; };       // L threads across channels, steps a run, runs a row, rows of partials
+
+template <typename T, int V>
+__device__ __forceinline__ void cload(const T* q, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = ld(q);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint2 r = *reinterpret_cast<const uint2*>(q);
+        v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
+        v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
+    } else {
+        const float4 r = *reinterpret_cast<const float4*>(q);
+        v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void cstore(T* q, const float (&v)[V]) {
+    if constexpr (V == 1) st(q, v[0]);
+    else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+    else *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+}
+template <int V>
+__device__ __forceinline__ void czero(float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.f;
+}
+
 __device__ __forceinline__ int row_end(const ConvArgs& p, int b) {
     return p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T;
 }
-// input row of time t (t < 0: the carried state)
-template <typename T, int W>
-__device__ __forceinline__ float input(const ConvArgs& p, int b, int t, int d) {
-    if (t >= 0) return ld((const T*)p.x + t * p.x_t + b * p.x_b + d);
-    return p.state_in ? ld((const T*)p.state_in + ((long long)b * (W - 1) + (t + W - 1)) * p.D + d) : 0.f;
-}
 __device__ __forceinline__ bool resets(const ConvArgs& p, int b, int t) { return t >= 0 && p.reset && p.reset[(long long)t * p.B + b] != 0; }
 
-// xw = the inputs of times ta - W + 1 .. ta - 1, as a step at ta - 1 leaves them (resets applied); end > ta - 1
-template <typename T, int W>
-__device__ __forceinline__ void window(const ConvArgs& p, int b, int ta, int d, float (&xw)[W]) {
+// xw[0 .. W - 2] = the inputs of times ta - W + 1 .. ta - 1 as the step at ta - 1 leaves them (what a reset cut off is 0 and
+// not live); needs ta <= the row's end
+template <typename T, int V, int W>
+__device__ __forceinline__ void window(const ConvArgs& p, int b, int ta, int d, float (&xw)[W][V], bool (&live)[W]) {
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
         const int t = ta - W + 1 + k;
+        live[k] = true;
         if (resets(p, b, t)) {
 #pragma unroll
-            for (int q = 0; q < k; ++q) xw[q] = 0.f;
+            for (int q = 0; q < k; ++q) { czero(xw[q]); live[q] = false; }
         }
-        xw[k] = input<T, W>(p, b, t, d);
+        if (t >= 0) cload<T, V>((const T*)p.x + t * p.x_t + b * p.x_b + d, xw[k]);
+        else if (p.state_in) cload<T, V>((const T*)p.state_in + ((long long)b * (W - 1) + (t + W - 1)) * p.D + d, xw[k]);
+        else czero(xw[k]);
+    }
+}
+template <int V, int W>
+__device__ __forceinline__ void load_w(const ConvArgs& p, int d, float (&w)[W][V], float (&bias)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k][i] = p.w[(long long)(d + i) * W + k];
+        bias[i] = p.bias ? p.bias[d + i] : 0.f;
     }
 }
 
-template <typename T, int W>
-__global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p) {
-    const int d = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y, ta = blockIdx.z * SEG;
-    if (d >= p.D) return;
-    const int end = row_end(p, b), tb = min(ta + SEG, (int)p.T);
-    float w[W], xw[W];
+template <typename T, int V, int W>
+__global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
+    const int d = (blockIdx.x * cg.L + threadIdx.x % cg.L) * V, b = blockIdx.y;
+    const int run = blockIdx.z * (256 / cg.L) + threadIdx.x / cg.L, ta = run * cg.seg;
+    if (d >= p.D || run >= cg.n_seg) return;
+    const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), stop = min(tb, end);
+    float w[W][V], bias[V], xw[W][V];
+    bool live[W];
+    T* y = (T*)p.y + b * p.y_b + d;
+    const auto put_state = [&] {
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[k] = p.w[(long long)d * W + k];
-    const float bias = p.bias ? p.bias[d] : 0.f;
-    if (ta <= end) window<T, W>(p, b, ta, d, xw);
-    for (int t = ta; t <= tb; ++t) {
-        // the state a row leaves: the segment that holds its last step (the first one, for an empty row) writes it
-        if (t == end && (t > ta || t == 0) && p.state_out) {
+        for (int k = 0; k < W - 1; ++k) cstore<T, V>((T*)p.state_out + ((long long)b * (W - 1) + k) * p.D + d, xw[k]);
+    };
+    if (ta <= end) {
+        load_w<V, W>(p, d, w, bias);
+        window<T, V, W>(p, b, ta, d, xw, live);
+        if (ta == 0 && end == 0 && p.state_out) put_state();                   // an empty row passes its state on
+    }
+    const T* x = (const T*)p.x + b * p.x_b + d;
+    for (int t0 = ta; t0 < stop; t0 += BATCH) {
+        float in[BATCH][V];
+        unsigned rm = 0;
 #pragma unroll
-            for (int k = 0; k < W - 1; ++k) st((T*)p.state_out + ((long long)b * (W - 1) + k) * p.D + d, xw[k]);
+        for (int q = 0; q < BATCH; ++q) {
+            const int t = min(t0 + q, stop - 1);                               // beyond the run: read again, not used
+            cload<T, V>(x + t * p.x_t, in[q]);
+            if (p.reset) rm |= (p.reset[(long long)t * p.B + b] != 0 ? 1u : 0u) << q;
         }
-        if (t == tb) break;
-        float v = 0.f;
-        if (t < end) {
-            if (resets(p, b, t)) {
 #pragma unroll
-                for (int k = 0; k < W - 1; ++k) xw[k] = 0.f;
+        for (int q = 0; q < BATCH; ++q) {
+            if (t0 + q >= stop) break;
+            if (rm >> q & 1) {
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) czero(xw[k]);
             }
-            xw[W - 1] = input<T, W>(p, b, t, d);
-            v = bias;
+            float v[V];
 #pragma unroll
-            for (int k = 0; k < W; ++k) v = fmaf(w[k], xw[k], v);
-            if (p.silu) v *= sigmoidf(v);
+            for (int i = 0; i < V; ++i) {
+                xw[W - 1][i] = in[q][i];
+                v[i] = bias[i];
 #pragma unroll
-            for (int k = 0; k < W - 1; ++k) xw[k] = xw[k + 1];
+                for (int k = 0; k < W; ++k) v[i] = fmaf(w[k][i], xw[k][i], v[i]);
+                if (p.silu) v[i] *= sigmoidf(v[i]);
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) xw[k][i] = xw[k + 1][i];
+            }
+            cstore<T, V>(y + (t0 + q) * p.y_t, v);
         }
-        st((T*)p.y + t * p.y_t + b * p.y_b + d, v);
+    }
+    if (stop == end && stop > ta && p.state_out) put_state();                  // the row's last step was this run's
+    float zero[V];
+    czero(zero);
+    for (int t = max(ta, stop); t < tb; ++t) cstore<T, V>(y + t * p.y_t, zero);
+}
+
+// dx[tau] collects w[k] dpre[tau + W - 1 - k]: one walk forward in time with W open sums. A run emits its steps ta .. tb - 1
+// and goes W - 1 steps further for them; dw and db count its own steps only and stay in registers over all the runs that a
+// thread takes (every cg.rows-th).
+template <typename T, int V, int W>
+__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
+    __shared__ float acc[W + 1][256 * V];
+    const int lx = threadIdx.x % cg.L, ly = threadIdx.x / cg.L, per = 256 / cg.L;
+    const int d = (blockIdx.x * cg.L + lx) * V;
+    float w[W][V], bias[V], dw[W][V], db[V];
+    const bool dv = d < p.D;
+    if (dv) load_w<V, W>(p, d, w, bias);
+#pragma unroll
+    for (int k = 0; k < W; ++k) czero(dw[k]);
+    czero(db);
+    const long long n_runs = (long long)cg.n_seg * p.B;
+    for (long long r = (long long)blockIdx.y * per + ly; dv && r < n_runs; r += (long long)cg.rows * per) {
+        const int run = (int)(r / p.B), b = (int)(r - run * p.B), ta = run * cg.seg;
+        const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), last = tb + W - 1, stop = min(last, end);
+        float xw[W][V], open[W][V];
+        bool live[W];
+#pragma unroll
+        for (int k = 0; k < W; ++k) { czero(open[k]); czero(xw[k]); live[k] = true; }
+        if (ta < end) window<T, V, W>(p, b, ta, d, xw, live);
+        const T *x = (const T*)p.x + b * p.x_b + d, *dy = (const T*)p.dy + b * p.dy_b + d;
+        T* dx = (T*)p.dx + b * p.dx_b + d;
+        // tau = t - W + 1 is complete once step t is through: no later step reaches back to it
+        const auto emit = [&](int t) {
+            const int tau = t - W + 1;
+            if (tau < 0) {
+                if (p.dstate_in && ta == 0) cstore<T, V>((T*)p.dstate_in + ((long long)b * (W - 1) + tau + W - 1) * p.D + d, open[0]);
+            } else if (tau >= ta) {
+                cstore<T, V>(dx + tau * p.dx_t, open[0]);
+            }
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) {
+                live[k] = live[k + 1];
+#pragma unroll
+                for (int i = 0; i < V; ++i) { xw[k][i] = xw[k + 1][i]; open[k][i] = open[k + 1][i]; }
+            }
+            czero(open[W - 1]);
+        };
+        for (int t0 = ta; t0 < stop; t0 += BATCH) {
+            float in[BATCH][V], gy[BATCH][V];
+            unsigned rm = 0;
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) {
+                const int t = min(t0 + q, stop - 1);
+                cload<T, V>(x + t * p.x_t, in[q]);
+                cload<T, V>(dy + t * p.dy_t, gy[q]);
+                if (p.reset) rm |= (p.reset[(long long)t * p.B + b] != 0 ? 1u : 0u) << q;
+            }
+#pragma unroll
+            for (int q = 0; q < BATCH; ++q) {
+                const int t = t0 + q;
+                if (t >= stop) break;
+                if (rm >> q & 1) {
+#pragma unroll
+                    for (int k = 0; k < W - 1; ++k) { czero(xw[k]); live[k] = false; }
+                }
+                live[W - 1] = true;
+                const bool mine = t < tb;
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    xw[W - 1][i] = in[q][i];
+                    float v = bias[i], g = gy[q][i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) v = fmaf(w[k][i], xw[k][i], v);
+                    if (p.silu) { const float s = sigmoidf(v); g *= s * fmaf(v, 1.f - s, 1.f); }
+#pragma unroll
+                    for (int k = 0; k < W; ++k) open[k][i] = live[k] ? fmaf(w[k][i], g, open[k][i]) : open[k][i];
+                    if (mine) {
+                        db[i] += g;
+#pragma unroll
+                        for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, xw[k][i], dw[k][i]);
+                    }
+                }
+                emit(t);
+            }
+        }
+        for (int t = max(ta, stop); t < last; ++t) {
+            if (t == end && p.dstate_out) {           // the state the row left = its last W - 1 inputs: their gradient comes in here
+#pragma unroll
+                for (int k = 0; k < W - 1; ++k) {
+                    if (!live[k]) continue;
+                    float g[V];
+                    cload<T, V>((const T*)p.dstate_out + ((long long)b * (W - 1) + k) * p.D + d, g);
+#pragma unroll
+                    for (int i = 0; i < V; ++i) open[k][i] += g[i];
+                }
+            }
+            emit(t);
+        }
+    }
+    // the block's sums: its `per` groups one after the other, then a row of partials [W + 1][D]
+    for (int t = 0; t < per; ++t) {
+        if (ly == t) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+#pragma unroll
+                for (int k = 0; k < W; ++k) acc[k][lx * V + i] = (t ? acc[k][lx * V + i] : 0.f) + dw[k][i];
+                acc[W][lx * V + i] = (t ? acc[W][lx * V + i] : 0.f) + db[i];
+            }
+        }
+        if (per > 1) __syncthreads();
+    }
+    if (ly == 0 && dv) {
+        float* q = p.ws + (long long)blockIdx.y * (W + 1) * p.D + d;
+#pragma unroll
+        for (int k = 0; k <= W; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) q[k * p.D + i] = acc[k][lx * V + i];
     }
 }
 
-// dx[tau] collects w[k] dpre[tau + W - 1 - k]: one walk forward in time with W open sums. A segment emits the steps
-// ta .. tb - 1 and runs W - 1 steps further for them; dw and db count its own steps only.
-template <typename T, int W>
-__global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, float* __restrict__ part) {
-    const int d = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y, ta = blockIdx.z * SEG;
-    if (d >= p.D) return;
-    const int end = row_end(p, b), tb = min(ta + SEG, (int)p.T);
-    float w[W], xw[W], open[W], dw[W], db = 0.f;
-    bool live[W];                                     // the window's step belongs to the current episode
-#pragma unroll
-    for (int k = 0; k < W; ++k) { w[k] = p.w[(long long)d * W + k]; open[k] = 0.f; dw[k] = 0.f; live[k] = true; xw[k] = 0.f; }
-    const float bias = p.bias ? p.bias[d] : 0.f;
-    if (ta < end) {
-        window<T, W>(p, b, ta, d, xw);
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) {             // a reset at a window step cuts the ones before it
-            if (resets(p, b, ta - W + 1 + k)) {
-#pragma unroll
-                for (int q = 0; q < k; ++q) live[q] = false;
-            }
-        }
-    }
-    for (int t = ta; t < tb + W - 1; ++t) {
-        if (t < end) {
-            if (resets(p, b, t)) {
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) { xw[k] = 0.f; live[k] = false; }
-            }
-            xw[W - 1] = input<T, W>(p, b, t, d);
-            live[W - 1] = true;
-            float v = bias;
-#pragma unroll
-            for (int k = 0; k < W; ++k) v = fmaf(w[k], xw[k], v);
-            float g = ld((const T*)p.dy + t * p.dy_t + b * p.dy_b + d);
-            if (p.silu) { const float s = sigmoidf(v); g *= s * fmaf(v, 1.f - s, 1.f); }
-            if (t < tb) {
-#pragma unroll
-                for (int k = 0; k < W; ++k) dw[k] = fmaf(g, xw[k], dw[k]);
-                db += g;
-            }
-#pragma unroll
-            for (int k = 0; k < W; ++k) if (live[k]) open[k] = fmaf(w[k], g, open[k]);
-        } else if (t == end && p.dstate_out) {        // the state the row left = its last W - 1 inputs: their gradient comes in here
-#pragma unroll
-            for (int k = 0; k < W - 1; ++k)
-                if (live[k]) open[k] += ld((const T*)p.dstate_out + ((long long)b * (W - 1) + k) * p.D + d);
-        }
-        const int tau = t - W + 1;                    // complete: no later step reaches back to it
-        if (tau < 0) {
-            if (p.dstate_in && ta == 0) st((T*)p.dstate_in + ((long long)b * (W - 1) + tau + W - 1) * p.D + d, open[0]);
-        } else if (tau >= ta) {
-            st((T*)p.dx + tau * p.dx_t + b * p.dx_b + d, open[0]);
-        }
-#pragma unroll
-        for (int k = 0; k < W - 1; ++k) { xw[k] = xw[k + 1]; open[k] = open[k + 1]; live[k] = live[k + 1]; }
-        open[W - 1] = 0.f;
-    }
-    float* q = part + ((long long)blockIdx.z * p.B + b) * (W + 1) * p.D + d;
-#pragma unroll
-    for (int k = 0; k < W; ++k) q[k * p.D] = dw[k];
-    q[W * p.D] = db;
-}
-
-__global__ void k_conv_sum(const float* __restrict__ part, int R, int W, long long D, float* __restrict__ dw, float* __restrict__ db) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= (W + 1) * D) return;
-    const long long k = i / D, d = i - k * D;
+// R rows of partials [W + 1][D] -> dw [D, W], db: 32 columns by 32 groups of rows a block, in a fixed order
+__global__ __launch_bounds__(1024) void k_conv_sum(const float* __restrict__ part, int R, int W, long long D, float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ float acc[32][33];
+    const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
+    const long long n = (W + 1) * D, c = (long long)blockIdx.x * 32 + x;
     float v = 0.f;
-    for (int r = 0; r < R; ++r) v += part[r * (W + 1) * D + i];
-    if (k < W) dw[d * W + k] = v;
-    else if (db) db[d] = v;
+    if (c < n) {
+#pragma unroll 8
+        for (int r = y; r < R; r += 32) v += part[r * n + c];
+    }
+    acc[y][x] = v;
+    __syncthreads();
+    if (y == 0 && c < n) {
+        v = 0.f;
+#pragma unroll
+        for (int k = 0; k < 32; ++k) v += acc[k][x];
+        const long long k = c / D, d = c - k * D;
+        if (k < W) dw[d * W + k] = v;
+        else if (db) db[d] = v;
+    }
 }
 
-template <typename T, int W>
+// One step. A thread per V channels of a row.
+template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V;
     if (i >= p.B * p.D) return;
     const long long b = i / p.D, d = i - b * p.D;
     T* s = (T*)p.state_out + b * (W - 1) * p.D + d;
     const bool rs = p.reset && p.reset[b] != 0;
-    const T* xp = (const T*)p.x + b * p.x_b + d;
-    T row[W];
+    float row[W][V], w[W][V], v[V];
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) row[k] = rs ? (T)0 : s[k * p.D];
-    row[W - 1] = *xp;
-    float v = p.bias ? p.bias[d] : 0.f;
+    for (int k = 0; k < W - 1; ++k) cload<T, V>(s + k * p.D, row[k]);
+    cload<T, V>((const T*)p.x + b * p.x_b + d, row[W - 1]);
+    load_w<V, W>(p, (int)d, w, v);
+    if (rs) {
 #pragma unroll
-    for (int k = 0; k < W; ++k) v = fmaf(p.w[d * W + k], ld(&row[k]), v);
-#pragma unroll
-    for (int k = 0; k < W - 1; ++k) s[k * p.D] = row[k + 1];
-    if (p.silu) v *= sigmoidf(v);
-    st((T*)p.y + b * p.y_b + d, v);
-}
-
-#define CONV_W(NAME, T, GRID, ...)                                             \
-    switch (p.W) {                                                              \
-        case 2: NAME<T, 2><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;            \
-        case 3: NAME<T, 3><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;            \
-        default: NAME<T, 4><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;           \
+        for (int k = 0; k < W - 1; ++k) czero(row[k]);
     }
+#pragma unroll
+    for (int q = 0; q < V; ++q) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) v[q] = fmaf(w[k][q], row[k][q], v[q]);
+        if (p.silu) v[q] *= sigmoidf(v[q]);
+    }
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) cstore<T, V>(s + k * p.D, row[k + 1]);
+    cstore<T, V>((T*)p.y + b * p.y_b + d, v);
+}
 
 static bool conv_ok(long long T, long long B, long long D, long long W) {
-    return T > 0 && T <= 65535ll * SEG && B > 0 && B <= 65535 && D > 0 && D < (1ll << 31) && W >= 2 && W <= 4;
+    return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && D > 0 && D < (1ll << 29) && W >= 2 && W <= 4;
 }
 
-// floats of scratch of a backward pass
+// Runs of 16 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves. vec: V > 1.
+static ConvGrid conv_grid(long long T, long long B, long long D, bool vec) {
+    const long long cv = vec ? D / 4 : D;
+    int L = 1;
+    while (L < cv && L < 256) L *= 2;
+    const long long waves = (cv + L - 1) / L * L * B / 64;                    // of one run a row
+    int seg = 16;
+    while (seg < 64 && waves * ((T + 2 * seg - 1) / (2 * seg)) >= 4096) seg *= 2;
+    const long long n_seg = (T + seg - 1) / seg, blocks = (n_seg * B + 256 / L - 1) / (256 / L), cols = (cv + L - 1) / L;
+    long long rows = (1024 + cols - 1) / cols;
+    if (rows > blocks) rows = blocks;
+    return {L, seg, (int)n_seg, (int)rows};
+}
+
+// floats of scratch of a backward pass, whatever the alignment of its tensors
 DRL_API int drl_short_conv_ws(long long T, long long B, long long D, long long W, long long* n) {
     if (!conv_ok(T, B, D, W)) return -1;
-    *n = (T + SEG - 1) / SEG * B * (W + 1) * D;
+    const int a = conv_grid(T, B, D, false).rows, b = D % 4 ? 0 : conv_grid(T, B, D, true).rows;
+    *n = (a > b ? a : b) * (W + 1) * D;
     return 0;
 }
+
+// whether 4 channels travel at once: every address and stride a multiple of their size
+static bool conv_vec(const ConvArgs& p, long long e, bool bwd) {
+    long long m = (long long)((uintptr_t)p.x | (uintptr_t)p.state_in | (uintptr_t)p.state_out) | ((p.x_t | p.x_b) * e);
+    m |= bwd ? (long long)((uintptr_t)p.dy | (uintptr_t)p.dx | (uintptr_t)p.dstate_in | (uintptr_t)p.dstate_out) | ((p.dy_t | p.dy_b | p.dx_t | p.dx_b) * e)
+             : (long long)(uintptr_t)p.y | ((p.y_t | p.y_b) * e);
+    return p.D % 4 == 0 && (m & (4 * e - 1)) == 0;
+}
+
+#define CONV_W(NAME, T, V, GRID, ...)                                          \
+    switch (p.W) {                                                              \
+        case 2: NAME<T, V, 2><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;         \
+        case 3: NAME<T, V, 3><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;         \
+        default: NAME<T, V, 4><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;        \
+    }
+#define CONV_ALL(NAME, GRID, ...)                                                                                       \
+    if (bf16) { if (vec) { CONV_W(NAME, bf16_t, 4, GRID, __VA_ARGS__) } else { CONV_W(NAME, bf16_t, 1, GRID, __VA_ARGS__) } }    \
+    else { if (vec) { CONV_W(NAME, float, 4, GRID, __VA_ARGS__) } else { CONV_W(NAME, float, 1, GRID, __VA_ARGS__) } }
 
 DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(p.T, p.B, p.D, p.W)) return -1;
-    const dim3 grid((unsigned)((p.D + 255) / 256), (unsigned)p.B, (unsigned)((p.T + SEG - 1) / SEG));
-    if (bf16) { CONV_W(k_conv_fwd, bf16_t, grid, p) } else { CONV_W(k_conv_fwd, float, grid, p) }
+    const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec);
+    const long long cv = vec ? p.D / 4 : p.D, per = 256 / cg.L;
+    if ((cg.n_seg + per - 1) / per > 65535) return -1;
+    const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)p.B, (unsigned)((cg.n_seg + per - 1) / per));
+    CONV_ALL(k_conv_fwd, grid, p, cg)
     return (int)hipGetLastError();
 }
 
@@ -210,19 +366,22 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
     long long need;
     if (drl_short_conv_ws(p.T, p.B, p.D, p.W, &need)) return -1;
     if (p.ws_n < need) return -2;
-    const dim3 grid((unsigned)((p.D + 255) / 256), (unsigned)p.B, (unsigned)((p.T + SEG - 1) / SEG));
-    if (bf16) { CONV_W(k_conv_bwd, bf16_t, grid, p, p.ws) } else { CONV_W(k_conv_bwd, float, grid, p, p.ws) }
-    const long long n = (p.W + 1) * p.D;
-    k_conv_sum<<<(unsigned)((n + 255) / 256), 256, 0, s>>>(p.ws, (int)(grid.z * p.B), (int)p.W, p.D, p.dw, p.db);
+    const bool vec = conv_vec(p, bf16 ? 2 : 4, true);
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec);
+    const long long cv = vec ? p.D / 4 : p.D, n = (p.W + 1) * p.D;
+    const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)cg.rows);
+    CONV_ALL(k_conv_bwd, grid, p, cg)
+    k_conv_sum<<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(p.ws, cg.rows, (int)p.W, p.D, p.dw, p.db);
     return (int)hipGetLastError();
 }
 
 DRL_API int drl_short_conv_step(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(1, 1, p.D, p.W) || p.B <= 0) return -1;
-    const long long nb = (p.B * p.D + 255) / 256;
+    const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
+    const long long nb = (p.B * p.D / (vec ? 4 : 1) + 255) / 256;
     if (nb > 0x7fffffffll) return -1;
     const dim3 grid((unsigned)nb);
-    if (bf16) { CONV_W(k_conv_step, bf16_t, grid, p) } else { CONV_W(k_conv_step, float, grid, p) }
+    CONV_ALL(k_conv_step, grid, p)
     return (int)hipGetLastError();
 }

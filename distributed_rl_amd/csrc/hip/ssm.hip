@@ -126,7 +126,7 @@ __device__ __forceinline__ unsigned reset_mask(unsigned flag) { return (unsigned
 __device__ __forceinline__ int row_end(const SsmArgs& p, int b) { return p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T; }
 
 // the states of a lane in a [.., B, D, N] tensor, four at a time (v4: N and the tensor's address allow it, see vec4)
-__device__ __forceinline__ bool vec4(const float* q, long long N) { return (N & 3) == 0 && ((uintptr_t)q & 15) == 0; }
+__host__ __device__ __forceinline__ bool vec4(const float* q, long long N) { return (N & 3) == 0 && ((uintptr_t)q & 15) == 0; }
 template <int NS>
 __device__ __forceinline__ void put_states(float* q, const float (&h)[NS], int n0, int N, bool v4) {
     if (NS % 4 == 0 && v4) {
@@ -719,27 +719,66 @@ __global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __re
     else if (p.dbias) p.dbias[i - DN - p.D] = v;
 }
 
-// One step: h [B, D, N] is read and written once, the rest is small. A thread per (row, channel).
-template <typename T>
+// One step: h [B, D, N] is read and written once and is nearly all of the bytes. Consecutive lanes own consecutive V states
+// (16 bytes; one state where N or an address does not allow it), L = 2^k >= N / V lanes a channel, and add up the read-out
+// with cross-lane adds; what depends on the channel only is computed by each of its lanes. A thread takes R channels with
+// the loads of all of them under way.
+template <typename T, int V, int L, int R>
 __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= p.B * p.D) return;
-    const long long b = i / p.D, d = i - b * p.D;
-    const float u = ld((const T*)p.u + b * p.u_b + d);
-    float sp = ld((const T*)p.dt + b * p.dt_b + d) + (p.bias ? p.bias[d] : 0.f);
-    if (p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
-    const bool rs = p.reset && p.reset[b] != 0;
-    float y = 0.f;
-    for (int n = 0; n < p.N; ++n) {
-        float* hp = p.hT + i * p.N + n;
-        const float h = fmaf(__builtin_amdgcn_exp2f(sp * (p.A[d * p.N + n] * LOG2E)), rs ? 0.f : *hp,
-                             sp * u * ld((const T*)p.Bm + b * p.B_b + n));
-        *hp = h;
-        y = fmaf(ld((const T*)p.Cm + b * p.C_b + n), h, y);
+    const int lane = threadIdx.x % L, n0 = lane * V, N = (int)p.N, D = (int)p.D;
+    const long long total = p.B * p.D, step = (long long)gridDim.x * (256 / L);
+    const long long i0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    float h[R][V], A[R][V], Bv[R][V], Cv[R][V], u[R], dt[R], z[R], Dd[R];
+    bool rs[R];
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const long long i = min(i0 + k * step, total - 1), b = (unsigned long long)i / (unsigned)D;
+        const int d = (int)(i - b * D);
+        u[k] = ld((const T*)p.u + b * p.u_b + d);
+        dt[k] = ld((const T*)p.dt + b * p.dt_b + d) + (p.bias ? p.bias[d] : 0.f);
+        z[k] = p.z ? ld((const T*)p.z + b * p.z_b + d) : 0.f;
+        Dd[k] = p.Dp ? p.Dp[d] : 0.f;
+        rs[k] = p.reset && p.reset[b] != 0;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const bool in = V > 1 || n0 < N;
+            h[k][v] = A[k][v] = Bv[k][v] = Cv[k][v] = 0.f;
+            if (V == 1 && in) { h[k][v] = p.hT[i * N + n0]; A[k][v] = p.A[(long long)d * N + n0]; }
+            if (in) { Bv[k][v] = ld((const T*)p.Bm + b * p.B_b + n0 + v); Cv[k][v] = ld((const T*)p.Cm + b * p.C_b + n0 + v); }
+        }
+        if constexpr (V == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(p.hT + i * N + n0), a = *reinterpret_cast<const float4*>(p.A + (long long)d * N + n0);
+            h[k][0] = x.x; h[k][1] = x.y; h[k][2] = x.z; h[k][3] = x.w;
+            A[k][0] = a.x; A[k][1] = a.y; A[k][2] = a.z; A[k][3] = a.w;
+        }
     }
-    if (p.Dp) y = fmaf(p.Dp[d], u, y);
-    if (p.z) { const float z = ld((const T*)p.z + b * p.z_b + d); y *= z * sigmoidf(z); }
-    st((T*)p.y + b * p.y_b + d, y);
+#pragma unroll
+    for (int k = 0; k < R; ++k) {
+        const long long i = i0 + k * step;
+        float s = dt[k], y = 0.f;
+        if (p.softplus) s = softplus_from(s, exp_neg_abs(s));
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const float e = __builtin_amdgcn_exp2f(s * (A[k][v] * LOG2E));
+            h[k][v] = fmaf(e, rs[k] ? 0.f : h[k][v], s * u[k] * Bv[k][v]);
+            y = fmaf(Cv[k][v], h[k][v], y);
+        }
+        if constexpr (L > 1) y = add_dpp<0xB1>(y);
+        if constexpr (L > 2) y = add_dpp<0x4E>(y);
+        if constexpr (L > 4) y = add_dpp<0x141>(y);
+        if constexpr (L > 8) y = add_dpp<0x140>(y);
+        if constexpr (L > 16) y = add_swap16(y, y);
+        if constexpr (L > 32) y = add_swap32(y, y);
+        if (i >= total) continue;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(p.hT + i * N + n0) = make_float4(h[k][0], h[k][1], h[k][2], h[k][3]);
+        else if (n0 < N) p.hT[i * N + n0] = h[k][0];
+        if (lane == 0) {
+            const long long b = (unsigned long long)i / (unsigned)D;
+            y = fmaf(Dd[k], u[k], y);
+            if (p.z) y *= z[k] * sigmoidf(z[k]);
+            st((T*)p.y + b * p.y_b + (i - b * D), y);
+        }
+    }
 }
 
 static int ns_of(long long N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 48 ? 12 : 16; }
@@ -826,12 +865,36 @@ DRL_API int drl_ssm_bwd(const SsmArgs* a, int bf16, hipStream_t s) {
     return (int)hipGetLastError();
 }
 
+template <typename T, int V, int L>
+static void launch_step(const SsmArgs& p, hipStream_t s) {
+    const long long ch = p.B * p.D, nb = (ch + 256 / L - 1) / (256 / L);
+    if (nb >= 8192) k_ssm_step<T, V, L, 4><<<(unsigned)((nb + 3) / 4), 256, 0, s>>>(p);
+    else k_ssm_step<T, V, L, 1><<<(unsigned)nb, 256, 0, s>>>(p);
+}
+template <typename T>
+static void dispatch_step(const SsmArgs& p, hipStream_t s) {
+    if (vec4(p.hT, p.N) && vec4(p.A, p.N) && (p.N & (p.N - 1)) == 0) {
+        switch (p.N) {
+            case 4: launch_step<T, 4, 1>(p, s); return;
+            case 8: launch_step<T, 4, 2>(p, s); return;
+            case 16: launch_step<T, 4, 4>(p, s); return;
+            case 32: launch_step<T, 4, 8>(p, s); return;
+            default: launch_step<T, 4, 16>(p, s); return;
+        }
+    }
+    if (p.N <= 1) launch_step<T, 1, 1>(p, s);
+    else if (p.N <= 2) launch_step<T, 1, 2>(p, s);
+    else if (p.N <= 4) launch_step<T, 1, 4>(p, s);
+    else if (p.N <= 8) launch_step<T, 1, 8>(p, s);
+    else if (p.N <= 16) launch_step<T, 1, 16>(p, s);
+    else if (p.N <= 32) launch_step<T, 1, 32>(p, s);
+    else launch_step<T, 1, 64>(p, s);
+}
+
 DRL_API int drl_ssm_step(const SsmArgs* a, int bf16, hipStream_t s) {
     const SsmArgs p = *a;
-    if (p.B <= 0 || p.D <= 0 || p.N <= 0 || p.N > 64) return -1;
-    const long long nb = (p.B * p.D + 255) / 256;
-    if (nb > 0x7fffffffll) return -1;
-    if (bf16) k_ssm_step<bf16_t><<<(unsigned)nb, 256, 0, s>>>(p);
-    else k_ssm_step<float><<<(unsigned)nb, 256, 0, s>>>(p);
+    if (p.B <= 0 || p.D <= 0 || p.D >= (1ll << 31) || p.N <= 0 || p.N > 64 || p.B * p.D >= (1ll << 33)) return -1;
+    if (bf16) dispatch_step<bf16_t>(p, s);
+    else dispatch_step<float>(p, s);
     return (int)hipGetLastError();
 }

@@ -1022,12 +1022,14 @@ def add2(a, b, out) -> None:
 _NORM, _CONV, _SSM = (struct.Struct("<%dq" % n) for n in (18, 29, 56))
 
 
-def _dev(t: torch.Tensor) -> torch.device:
-    if not t.is_cuda:
+def _dev(t: torch.Tensor) -> int:
+    """Ordinal of the tensor's GPU, which has to be the current one: launches go to its current stream."""
+    i = t.get_device()
+    if i < 0:
         raise TypeError("state-space operators run on CUDA tensors (got %s): the CPU forms are in ops/oracle.py" % t.device)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError("tensors are on %s but the current device is cuda:%d" % (t.device, torch.cuda.current_device()))
-    return t.device
+    if i != torch.cuda.current_device():
+        raise ValueError("tensors are on cuda:%d but the current device is cuda:%d" % (i, torch.cuda.current_device()))
+    return i
 
 
 def _typ(t: torch.Tensor) -> int:
@@ -1038,32 +1040,41 @@ def _typ(t: torch.Tensor) -> int:
     raise TypeError("fp32 or bf16 tensors are needed (got %s)" % t.dtype)
 
 
-def _vec(t: Optional[torch.Tensor], shape: tuple, dtype, dev, name: str) -> int:
-    """Address of a contiguous tensor of a given shape (0 for None)."""
+def _refuse(t, shape, dtype, dev: int, name: str):
     if t is None:
-        return 0
-    if t.dtype is not dtype or t.device != dev:
-        raise TypeError("%s must be a %s tensor on %s (got %s on %s)" % (name, dtype, dev, t.dtype, t.device))
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError("%s must be contiguous of shape %s (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), t.stride()))
+        raise ValueError("%s is needed" % name)
+    if t.dtype is not dtype or t.get_device() != dev:
+        raise TypeError("%s must be a %s tensor on cuda:%d (got %s on %s)" % (name, dtype, dev, t.dtype, t.device))
+    raise ValueError("%s must be contiguous of shape %s (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), t.stride()))
+
+
+def _vec(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str) -> int:
+    """Address of a contiguous tensor of a given shape."""
+    if t is None or t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.get_device() != dev:
+        _refuse(t, shape, dtype, dev, name)
     return t.data_ptr()
 
 
-def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev, name: str, out: bool = False) -> tuple:
+def _opt(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str) -> int:
+    """The same for a tensor that may be None (0)."""
+    return 0 if t is None else _vec(t, shape, dtype, dev, name)
+
+
+def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, out: bool = False) -> tuple:
     """(address, strides of the leading dims) of a tensor whose last dim is contiguous; zeros for None. ``out``: no two
     elements may share an address."""
     if t is None:
         return (0,) * len(shape)
-    if t.dtype is not dtype or t.device != dev:
-        raise TypeError("%s must be a %s tensor on %s (got %s on %s)" % (name, dtype, dev, t.dtype, t.device))
-    if t.shape != shape:
-        raise ValueError("%s must have shape %s (got %s)" % (name, tuple(shape), tuple(t.shape)))
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(t, shape, dtype, dev, name)
     st = t.stride()
+    if t.is_contiguous():
+        return (t.data_ptr(),) + st[:-1]
     if st[-1] != 1 and shape[-1] > 1:
         raise ValueError("%s: the last dimension must be contiguous (strides %s)" % (name, st))
     if out:
         need = shape[-1]
-        for n, s in sorted(zip(shape[:-1], st[:-1]), key=lambda v: v[1]):
+        for s, n in sorted(zip(st[:-1], shape[:-1])):
             if n > 1:
                 if s < need:
                     raise ValueError("%s: rows of an output may not overlap (shape %s, strides %s)" % (name, tuple(shape), st))
@@ -1071,11 +1082,11 @@ def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev, name: str, out: b
     return (t.data_ptr(),) + st[:-1]
 
 
-def _apart(outs, ins) -> None:
-    """No output starts where an input or another output does."""
-    outs = [a for a in outs if a]
-    if len(set(outs)) != len(outs) or not set(outs).isdisjoint(ins):
-        raise ValueError("an output shares its memory with an input or another output")
+def _apart(outs: tuple, ins: tuple) -> None:
+    """No output starts where an input or another output does (0: not given)."""
+    for i, a in enumerate(outs):
+        if a and (a in ins or a in outs[i + 1:]):
+            raise ValueError("an output shares its memory with an input or another output")
 
 
 def _need(**tensors) -> None:
@@ -1095,32 +1106,17 @@ def _ws_numel(rc: int, n: ctypes.c_longlong, what: str, sizes) -> int:
     return n.value
 
 
+def _run(fn, *args) -> None:
+    """Launch on the current stream of the tensors' device (the last argument is its ordinal)."""
+    rc = fn(*args[:-1], torch._C._cuda_getCurrentRawStream(args[-1]))
+    if rc != 0:
+        raise RuntimeError("%s failed with code %d%s" % (fn.__name__, rc, " (workspace too small)" if rc == -2 else ""))
+
+
 def layer_norm_ws(M: int, D: int, device) -> torch.Tensor:
     """Scratch of :func:`layer_norm_bwd` for M rows of D."""
     n = ctypes.c_longlong()
     return torch.empty(_ws_numel(native.hip().drl_norm_ws(M, D, ctypes.byref(n)), n, "layer_norm", (M, D)), device=device)
-
-
-def _norm_args(x, w, b, y, mean, rstd, dy=None, dx=None, dw=None, db=None, ws=None):
-    if x.dim() != 2:
-        raise ValueError("x must be [rows, D] (got %s)" % (tuple(x.shape),))
-    M, D = shape = x.shape
-    if M < 1 or not 1 <= D <= 16384:
-        raise ValueError("layer_norm: unsupported sizes %s" % ((M, D),))
-    dev, typ, f32 = _dev(x), x.dtype, torch.float32
-    bf16 = _typ(x)
-    xr = _rows(x, shape, typ, dev, "x")
-    yr = _rows(y, shape, typ, dev, "y", True)
-    dyr, dxr = _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
-    wp, bp = _vec(w, (D,), f32, dev, "w"), _vec(b, (D,), f32, dev, "b")
-    mp, rp = _vec(mean, (M,), f32, dev, "mean"), _vec(rstd, (M,), f32, dev, "rstd")
-    dwp, dbp = _vec(dw, (D,), f32, dev, "dw"), _vec(db, (D,), f32, dev, "db")
-    wsp = _vec(ws, (ws.numel(),), f32, dev, "ws") if ws is not None else 0
-    if y is not None:
-        _apart((yr[0], mp, rp), (xr[0], wp, bp))
-    else:
-        _apart((dxr[0], dwp, dbp, wsp), (xr[0], dyr[0], wp, mp, rp))
-    return _NORM.pack(*xr, wp, bp, *yr, mp, rp, M, D, *dyr, *dxr, dwp, dbp, wsp, ws.numel() if ws is not None else 0), bf16
 
 
 def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
@@ -1129,17 +1125,38 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
     _none_or_both(mean, rstd, "mean and rstd")
     if not eps >= 0:
         raise ValueError("eps must not be negative (got %r)" % (eps,))
-    _need(x=x, w=w, y=y)
-    rec, bf16 = _norm_args(x, w, b, y, mean, rstd)
-    _ck(native.hip().drl_norm_fwd(rec, bf16, float(eps), _s()), "layer_norm_fwd")
+    shape, typ, f32 = _norm_shape(x), x.dtype, torch.float32
+    _need(w=w, y=y)
+    dev, bf16 = _dev(x), _typ(x)
+    M, D = shape
+    xp, xs = _rows(x, shape, typ, dev, "x")
+    yp, ys = _rows(y, shape, typ, dev, "y", True)
+    wp, bp = _vec(w, (D,), f32, dev, "w"), _opt(b, (D,), f32, dev, "b")
+    mp, rp = _opt(mean, (M,), f32, dev, "mean"), _opt(rstd, (M,), f32, dev, "rstd")
+    _apart((yp, mp, rp), (xp, wp, bp))
+    _run(native.hip().drl_norm_fwd, _NORM.pack(xp, xs, wp, bp, yp, ys, mp, rp, M, D, 0, 0, 0, 0, 0, 0, 0, 0), bf16, float(eps), dev)
 
 
 def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
     """Gradients of :func:`layer_norm_fwd`: dx [rows, D], dw and db (None if the norm has no b) fp32 [D], overwritten. The
     sums over rows run in a fixed order. ``ws`` from :func:`layer_norm_ws`."""
-    _need(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dw=dw, ws=ws)
-    rec, bf16 = _norm_args(x, w, None, None, mean, rstd, dy, dx, dw, db, ws)
-    _ck(native.hip().drl_norm_bwd(rec, bf16, _s()), "layer_norm_bwd")
+    shape, typ, f32 = _norm_shape(x), x.dtype, torch.float32
+    _need(dy=dy, dx=dx, ws=ws)
+    dev, bf16 = _dev(x), _typ(x)
+    M, D = shape
+    xr, dyr, dxr = _rows(x, shape, typ, dev, "x"), _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
+    wp, mp, rp = _vec(w, (D,), f32, dev, "w"), _vec(mean, (M,), f32, dev, "mean"), _vec(rstd, (M,), f32, dev, "rstd")
+    dwp, dbp, wsp = _vec(dw, (D,), f32, dev, "dw"), _opt(db, (D,), f32, dev, "db"), _vec(ws, (ws.numel(),), f32, dev, "ws")
+    _apart((dxr[0], dwp, dbp, wsp), (xr[0], dyr[0], wp, mp, rp))
+    _run(native.hip().drl_norm_bwd, _NORM.pack(*xr, wp, 0, 0, 0, mp, rp, M, D, *dyr, *dxr, dwp, dbp, wsp, ws.numel()), bf16, dev)
+
+
+def _norm_shape(x) -> torch.Size:
+    _need(x=x)
+    shape = x.shape
+    if len(shape) != 2 or not 0 < shape[0] < 1 << 31 or not 0 < shape[1] <= 16384:
+        raise ValueError("layer_norm: x must be [rows, D], D <= 16384 (got %s)" % (tuple(shape),))
+    return shape
 
 
 def short_conv_ws(T: int, B: int, D: int, W: int, device) -> torch.Tensor:
@@ -1150,25 +1167,23 @@ def short_conv_ws(T: int, B: int, D: int, W: int, device) -> torch.Tensor:
 
 def _conv_args(x, w, bias, silu, reset, lengths, y=None, state_in=None, state_out=None, dy=None, dx=None, dw=None, db=None, ws=None,
                dstate_in=None, dstate_out=None):
-    if x.dim() != 3:
-        raise ValueError("x must be [T, B, D] (got %s)" % (tuple(x.shape),))
-    T, B, D = shape = x.shape
-    W = w.shape[-1]
-    if T < 1 or not 1 <= B <= 65535 or D < 1 or not 2 <= W <= 4 or T > 1000000:
+    shape, W = x.shape, w.shape[-1]
+    if len(shape) != 3 or not 0 < shape[0] <= 1000000 or not 0 < shape[1] <= 65535 or shape[2] < 1 or not 2 <= W <= 4:
         raise ValueError("short_conv: unsupported sizes %s with %d taps" % (tuple(shape), W))
+    T, B, D = shape
     dev, typ, f32 = _dev(x), x.dtype, torch.float32
     bf16, st = _typ(x), (B, W - 1, D)
     xr, yr = _rows(x, shape, typ, dev, "x"), _rows(y, shape, typ, dev, "y", True)
     dyr, dxr = _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
-    wp, bp = _vec(w, (D, W), f32, dev, "w"), _vec(bias, (D,), f32, dev, "bias")
-    si, so = _vec(state_in, st, typ, dev, "state_in"), _vec(state_out, st, typ, dev, "state_out")
-    dsi, dso = _vec(dstate_in, st, typ, dev, "dstate_in"), _vec(dstate_out, st, typ, dev, "dstate_out")
-    rp, lp = _vec(reset, (T, B), torch.uint8, dev, "reset"), _vec(lengths, (B,), torch.int32, dev, "lengths")
-    dwp, dbp = _vec(dw, (D, W), f32, dev, "dw"), _vec(db, (D,), f32, dev, "db")
-    wsp = _vec(ws, (ws.numel(),), f32, dev, "ws") if ws is not None else 0
+    wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
+    si, so = _opt(state_in, st, typ, dev, "state_in"), _opt(state_out, st, typ, dev, "state_out")
+    dsi, dso = _opt(dstate_in, st, typ, dev, "dstate_in"), _opt(dstate_out, st, typ, dev, "dstate_out")
+    rp, lp = _opt(reset, (T, B), torch.uint8, dev, "reset"), _opt(lengths, (B,), torch.int32, dev, "lengths")
+    dwp, dbp = _opt(dw, (D, W), f32, dev, "dw"), _opt(db, (D,), f32, dev, "db")
+    wsp, n_ws = (_vec(ws, (ws.numel(),), f32, dev, "ws"), ws.numel()) if ws is not None else (0, 0)
     _apart((yr[0], so, dxr[0], dwp, dbp, dsi, wsp), (xr[0], wp, bp, si, dyr[0], dso, rp, lp))
     return _CONV.pack(xr[0], si, xr[1], xr[2], wp, bp, rp, lp, yr[0], so, yr[1], yr[2], T, B, D, W, 1 if silu else 0, dyr[0], dso,
-                      dyr[1], dyr[2], dxr[0], dsi, dxr[1], dxr[2], dwp, dbp, wsp, ws.numel() if ws is not None else 0), bf16
+                      dyr[1], dyr[2], dxr[0], dsi, dxr[1], dxr[2], dwp, dbp, wsp, n_ws), bf16, dev
 
 
 def short_conv_fwd(x, w, bias, y, state_in=None, state_out=None, reset=None, lengths=None, silu: bool = True) -> None:
@@ -1180,8 +1195,7 @@ def short_conv_fwd(x, w, bias, y, state_in=None, state_out=None, reset=None, len
     cuts step t and all later ones off from the steps before t, the carried state included (episode start). ``lengths``
     int32 [B]: steps from lengths[b] on are padding: not read, and zero in y."""
     _need(x=x, w=w, y=y)
-    rec, bf16 = _conv_args(x, w, bias, silu, reset, lengths, y, state_in, state_out)
-    _ck(native.hip().drl_short_conv_fwd(rec, bf16, _s()), "short_conv_fwd")
+    _run(native.hip().drl_short_conv_fwd, *_conv_args(x, w, bias, silu, reset, lengths, y, state_in, state_out))
 
 
 def short_conv_bwd(dy, x, w, bias, dx, dw, db, ws, state_in=None, dstate_in=None, dstate_out=None, reset=None, lengths=None,
@@ -1190,27 +1204,26 @@ def short_conv_bwd(dy, x, w, bias, dx, dw, db, ws, state_in=None, dstate_in=None
     fp32 [D, W], db fp32 [D] or None, dstate_in [B, W-1, D] or None, all overwritten; ``dstate_out`` adds the gradient that
     arrives at state_out. The sums over rows and steps run in a fixed order. ``ws`` from :func:`short_conv_ws`."""
     _need(dy=dy, x=x, w=w, dx=dx, dw=dw, ws=ws)
-    rec, bf16 = _conv_args(x, w, bias, silu, reset, lengths, None, state_in, None, dy, dx, dw, db, ws, dstate_in, dstate_out)
-    _ck(native.hip().drl_short_conv_bwd(rec, bf16, _s()), "short_conv_bwd")
+    _run(native.hip().drl_short_conv_bwd,
+         *_conv_args(x, w, bias, silu, reset, lengths, None, state_in, None, dy, dx, dw, db, ws, dstate_in, dstate_out))
 
 
 def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None:
     """One step of :func:`short_conv_fwd` for x [B, D]: ``state`` [B, W-1, D] is shifted in place, ``reset`` uint8 [B]."""
-    _need(x=x, w=w, state=state, y=y)
-    if x.dim() != 2:
-        raise ValueError("x must be [B, D] (got %s)" % (tuple(x.shape),))
-    B, D = shape = x.shape
-    W = w.shape[-1]
-    if B < 1 or D < 1 or not 2 <= W <= 4:
-        raise ValueError("short_conv_step: unsupported sizes %s with %d taps" % (tuple(shape), W))
+    _need(x=x, w=w, y=y)
+    shape, W = x.shape, w.shape[-1]
+    if len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or not 2 <= W <= 4:
+        raise ValueError("short_conv_step: x must be [B, D], w [D, 2 .. 4] (got %s, %s)" % (tuple(shape), tuple(w.shape)))
+    B, D = shape
     dev, typ, f32 = _dev(x), x.dtype, torch.float32
     bf16 = _typ(x)
-    xr, yr = _rows(x, shape, typ, dev, "x"), _rows(y, shape, typ, dev, "y", True)
-    sp, rp = _vec(state, (B, W - 1, D), typ, dev, "state"), _vec(reset, (B,), torch.uint8, dev, "reset")
-    wp, bp = _vec(w, (D, W), f32, dev, "w"), _vec(bias, (D,), f32, dev, "bias")
-    _apart((yr[0], sp), (xr[0], wp, bp, rp))
-    rec = _CONV.pack(xr[0], 0, 0, xr[1], wp, bp, rp, 0, yr[0], sp, 0, yr[1], 1, B, D, W, 1 if silu else 0, *(0,) * 12)
-    _ck(native.hip().drl_short_conv_step(rec, bf16, _s()), "short_conv_step")
+    xp, xs = _rows(x, shape, typ, dev, "x")
+    yp, ys = _rows(y, shape, typ, dev, "y", True)
+    sp, rp = _vec(state, (B, W - 1, D), typ, dev, "state"), _opt(reset, (B,), torch.uint8, dev, "reset")
+    wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
+    _apart((yp, sp), (xp, wp, bp, rp))
+    _run(native.hip().drl_short_conv_step, _CONV.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0, 0, 0, 0, 0,
+                                                      0, 0, 0, 0, 0, 0, 0, 0), bf16, dev)
 
 
 SSM_CHUNK = 16              # steps between the states that ssm_scan_fwd saves for ssm_scan_bwd
@@ -1230,32 +1243,33 @@ def ssm_scan_ckpt(T: int, B: int, D: int, N: int, device) -> torch.Tensor:
 
 def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None, ws=None, h0=None, hT=None, ckpt=None, dy=None, dhT=None,
               du=None, ddt=None, dz=None, dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dh0=None):
-    if u.dim() != 3 or Bm.dim() != 3:
-        raise ValueError("u must be [T, B, D] and Bm [T, B, N] (got %s, %s)" % (tuple(u.shape), tuple(Bm.shape)))
-    T, B, Dc = shape = u.shape
-    N = Bm.shape[-1]
-    if T < 1 or not 1 <= B <= 65535 or Dc < 1 or not 1 <= N <= 64 or T >= 1 << 31:
-        raise ValueError("ssm_scan: unsupported sizes %s with %d states" % (tuple(shape), N))
+    shape, bc = u.shape, Bm.shape
+    if len(shape) != 3 or len(bc) != 3 or not 0 < shape[0] < 1 << 31 or not 0 < shape[1] <= 65535 or not 0 < shape[2] < 1 << 25 \
+            or not 0 < bc[2] <= 64 or shape[0] * shape[1] > 1 << 31:
+        raise ValueError("ssm_scan: unsupported sizes: u must be [T, B, D], Bm [T, B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
+    T, B, Dc = shape
+    N = bc[2]
     dev, typ, f32 = _dev(u), u.dtype, torch.float32
-    bf16, bc, st = _typ(u), (T, B, N), (B, Dc, N)
-    ur, dtr, zr = (_rows(t, shape, typ, dev, n) for t, n in ((u, "u"), (dt, "dt"), (z, "z")))
+    bf16, st, bc = _typ(u), (B, Dc, N), (T, B, N)
+    ur, dtr, zr = _rows(u, shape, typ, dev, "u"), _rows(dt, shape, typ, dev, "dt"), _rows(z, shape, typ, dev, "z")
     Br, Cr = _rows(Bm, bc, typ, dev, "Bm"), _rows(Cm, bc, typ, dev, "Cm")
     yr, dyr = _rows(y, shape, typ, dev, "y", True), _rows(dy, shape, typ, dev, "dy")
-    dur, ddtr, dzr = (_rows(t, shape, typ, dev, n, True) for t, n in ((du, "du"), (ddt, "ddt"), (dz, "dz")))
+    dur, ddtr, dzr = _rows(du, shape, typ, dev, "du", True), _rows(ddt, shape, typ, dev, "ddt", True), _rows(dz, shape, typ, dev, "dz", True)
     dBr, dCr = _rows(dB, bc, typ, dev, "dB", True), _rows(dC, bc, typ, dev, "dC", True)
-    Ap, dAp = _vec(A, (Dc, N), f32, dev, "A"), _vec(dA, (Dc, N), f32, dev, "dA")
-    Dp, bp, dDp, dbp = (_vec(t, (Dc,), f32, dev, n) for t, n in ((D, "D"), (dt_bias, "dt_bias"), (dD, "dD"), (ddt_bias, "ddt_bias")))
-    h0p, hTp, dhTp, dh0p = (_vec(t, st, f32, dev, n) for t, n in ((h0, "h0"), (hT, "hT"), (dhT, "dhT"), (dh0, "dh0")))
-    rp, lp = _vec(reset, (T, B), torch.uint8, dev, "reset"), _vec(lengths, (B,), torch.int32, dev, "lengths")
-    ck = _vec(ckpt, ((T + SSM_CHUNK - 1) // SSM_CHUNK, B, Dc, N), f32, dev, "ckpt")
-    wsp = _vec(ws, (ws.numel(),), f32, dev, "ws")
-    if T > 1 and max(r[1] for r in (ur, dtr, zr, Br, Cr, yr, dyr, dur, ddtr, dzr)) >= 1 << 25:
+    Ap, dAp = _vec(A, (Dc, N), f32, dev, "A"), _opt(dA, (Dc, N), f32, dev, "dA")
+    Dp, bp, dDp, dbp = (_opt(t, (Dc,), f32, dev, n) for t, n in ((D, "D"), (dt_bias, "dt_bias"), (dD, "dD"), (ddt_bias, "ddt_bias")))
+    h0p, hTp, dhTp, dh0p = (_opt(t, st, f32, dev, n) for t, n in ((h0, "h0"), (hT, "hT"), (dhT, "dhT"), (dh0, "dh0")))
+    rp, lp = _opt(reset, (T, B), torch.uint8, dev, "reset"), _opt(lengths, (B,), torch.int32, dev, "lengths")
+    ck = _opt(ckpt, ((T + SSM_CHUNK - 1) // SSM_CHUNK, B, Dc, N), f32, dev, "ckpt")
+    n_ws = ws.numel()
+    wsp = _vec(ws, (n_ws,), f32, dev, "ws")
+    if T > 1 and max(ur[1], dtr[1], zr[1], Br[1], Cr[1], yr[1], dyr[1], dur[1], ddtr[1], dzr[1]) >= 1 << 25:
         raise ValueError("ssm_scan: steps of one tensor are 2^25 elements or more apart")
-    ins = (ur[0], dtr[0], zr[0], Br[0], Cr[0], Ap, Dp, bp, h0p, rp, lp, dyr[0], dhTp)
-    _apart((yr[0], hTp, ck, wsp if ws.numel() else 0, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0], dAp, dDp, dbp, dh0p), ins)
+    _apart((yr[0], hTp, ck, wsp if n_ws else 0, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0], dAp, dDp, dbp, dh0p),
+           (ur[0], dtr[0], zr[0], Br[0], Cr[0], Ap, Dp, bp, h0p, rp, lp, dyr[0], dhTp))
     return _SSM.pack(ur[0], dtr[0], zr[0], Br[0], Cr[0], *ur[1:], *dtr[1:], *zr[1:], *Br[1:], *Cr[1:], Ap, Dp, bp, h0p, rp, lp, *yr,
-                     hTp, ck, wsp, ws.numel(), T, B, Dc, N, 1 if softplus else 0, *dyr, dhTp, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0],
-                     *dur[1:], *ddtr[1:], *dzr[1:], *dBr[1:], *dCr[1:], dAp, dDp, dbp, dh0p), bf16
+                     hTp, ck, wsp, n_ws, T, B, Dc, N, 1 if softplus else 0, *dyr, dhTp, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0],
+                     *dur[1:], *ddtr[1:], *dzr[1:], *dBr[1:], *dCr[1:], dAp, dDp, dbp, dh0p), bf16, dev
 
 
 def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None, hT=None, reset=None, lengths=None,
@@ -1271,8 +1285,7 @@ def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None,
     zero in y, and hT is the state after step lengths[b] - 1. ``ckpt`` (:func:`ssm_scan_ckpt`) keeps what
     :func:`ssm_scan_bwd` needs; ``ws`` from :func:`ssm_scan_ws`."""
     _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, y=y, ws=ws)
-    rec, bf16 = _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y, ws, h0, hT, ckpt)
-    _ck(native.hip().drl_ssm_fwd(rec, bf16, _s()), "ssm_scan_fwd")
+    _run(native.hip().drl_ssm_fwd, *_ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y, ws, h0, hT, ckpt))
 
 
 def ssm_scan_bwd(dy, u, dt, A, Bm, Cm, ckpt, du, ddt, dA, dB, dC, ws, D=None, dD=None, z=None, dz=None, dt_bias=None, ddt_bias=None,
@@ -1285,21 +1298,19 @@ def ssm_scan_bwd(dy, u, dt, A, Bm, Cm, ckpt, du, ddt, dA, dB, dC, ws, D=None, dD
     _none_or_both(z, dz, "z and dz")
     if dD is not None and D is None or ddt_bias is not None and dt_bias is None:
         raise ValueError("dD / ddt_bias without D / dt_bias")
-    rec, bf16 = _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, None, ws, None, None, ckpt, dy, dhT, du, ddt, dz,
-                          dB, dC, dA, dD, ddt_bias, dh0)
-    _ck(native.hip().drl_ssm_bwd(rec, bf16, _s()), "ssm_scan_bwd")
+    _run(native.hip().drl_ssm_bwd, *_ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, None, ws, None, None, ckpt, dy, dhT,
+                                              du, ddt, dz, dB, dC, dA, dD, ddt_bias, dh0))
 
 
 def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, softplus: bool = True) -> None:
     """One step of :func:`ssm_scan_fwd` for u, dt, z, y [B, D] and Bm, Cm [B, N]: ``h`` [B, D, N] fp32 is updated in place,
     ``reset`` uint8 [B]."""
-    _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, h=h, y=y)
-    if u.dim() != 2 or Bm.dim() != 2:
-        raise ValueError("u must be [B, D] and Bm [B, N] (got %s, %s)" % (tuple(u.shape), tuple(Bm.shape)))
-    B, Dc = shape = u.shape
-    N = Bm.shape[-1]
-    if B < 1 or Dc < 1 or not 1 <= N <= 64:
-        raise ValueError("ssm_step: unsupported sizes %s with %d states" % (tuple(shape), N))
+    _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, y=y)
+    shape, bc = u.shape, Bm.shape
+    if len(shape) != 2 or len(bc) != 2 or shape[0] < 1 or shape[1] < 1 or not 0 < bc[1] <= 64:
+        raise ValueError("ssm_step: u must be [B, D], Bm [B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
+    B, Dc = shape
+    N = bc[1]
     dev, typ, f32 = _dev(u), u.dtype, torch.float32
     bf16, bc = _typ(u), (B, N)
     up, us = _rows(u, shape, typ, dev, "u")
@@ -1308,9 +1319,11 @@ def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, s
     Bp, Bs = _rows(Bm, bc, typ, dev, "Bm")
     Cp, Cs = _rows(Cm, bc, typ, dev, "Cm")
     yp, ys = _rows(y, shape, typ, dev, "y", True)
-    Ap, hp, rp = _vec(A, (Dc, N), f32, dev, "A"), _vec(h, (B, Dc, N), f32, dev, "h"), _vec(reset, (B,), torch.uint8, dev, "reset")
-    Dp, bp = _vec(D, (Dc,), f32, dev, "D"), _vec(dt_bias, (Dc,), f32, dev, "dt_bias")
+    Ap, hp, rp = _vec(A, (Dc, N), f32, dev, "A"), _vec(h, (B, Dc, N), f32, dev, "h"), _opt(reset, (B,), torch.uint8, dev, "reset")
+    Dp, bp = _opt(D, (Dc,), f32, dev, "D"), _opt(dt_bias, (Dc,), f32, dev, "dt_bias")
     _apart((yp, hp), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, rp))
-    rec = _SSM.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys, hp, 0, 0, 0, 1, B, Dc, N,
-                    1 if softplus else 0, *(0,) * 23)
-    _ck(native.hip().drl_ssm_step(rec, bf16, _s()), "ssm_step")
+    _run(native.hip().drl_ssm_step, _SSM.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys, hp,
+                                              0, 0, 0, 1, B, Dc, N, 1 if softplus else 0, *_ZEROS23), bf16, dev)
+
+
+_ZEROS23 = (0,) * 23

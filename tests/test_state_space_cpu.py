@@ -140,7 +140,7 @@ def test_missing_tensors_are_refused():
 
 def test_rows_of_outputs_may_not_overlap():
     t = torch.zeros(64)
-    cpu = torch.device("cpu")
+    cpu = -1                                                # the ordinal that tensors on the CPU have
     assert hip._rows(t.as_strided((2, 3, 4), (32, 8, 1)), (2, 3, 4), torch.float32, cpu, "y", True)[1:] == (32, 8)
     assert hip._rows(t.as_strided((2, 3, 4), (4, 16, 1)), (2, 3, 4), torch.float32, cpu, "y", True)[1:] == (4, 16)
     assert hip._rows(t.as_strided((2, 3, 4), (0, 0, 1)), (2, 3, 4), torch.float32, cpu, "x")[1:] == (0, 0)
