@@ -4,11 +4,12 @@
 // before t; steps from lengths[b] on are not read and write zeros.
 //
 // Bound by memory: a thread owns V neighbouring channels (16 bytes of fp32, 8 of bf16; 1 where addresses or strides do not
-// allow it) of one row and a run of steps, reads BATCH steps ahead and keeps the last W - 1 inputs in registers. Runs of one
+// allow it) of one row and a run of steps, reads FB (BB) steps ahead and keeps the last W - 1 inputs in registers. Runs of one
 // row are walked side by side; each starts by reading the W - 1 steps before it again.
 #include "ssm_math.h"
 
-#define BATCH 8
+#define FB 16            // steps read ahead by the forward
+#define BB 6             // and by the backward (two tensors)
 
 struct ConvArgs {        // mirrored by ops/hip.py (_conv_args): 64-bit words in this order
     const void *x, *state_in;
@@ -59,6 +60,21 @@ __device__ __forceinline__ int row_end(const ConvArgs& p, int b) {
 }
 __device__ __forceinline__ bool resets(const ConvArgs& p, int b, int t) { return t >= 0 && p.reset && p.reset[(long long)t * p.B + b] != 0; }
 
+// bit q: step t0 + q (< stop) has its reset flag set. With 64 or more threads across the channels a wave has one row and one
+// run: a lane reads a flag. Every lane of the wave takes part.
+template <int N>
+__device__ __forceinline__ unsigned reset_bits(const ConvArgs& p, int L, int b, int t0, int stop) {
+    if (!p.reset) return 0;
+    if (L >= 64) {
+        const int q = threadIdx.x & 63;
+        return (unsigned)__ballot(q < N && t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0);
+    }
+    unsigned rm = 0;
+#pragma unroll
+    for (int q = 0; q < N; ++q) rm |= (t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0 ? 1u : 0u) << q;
+    return rm;
+}
+
 // xw[0 .. W - 2] = the inputs of times ta - W + 1 .. ta - 1 as the step at ta - 1 leaves them (what a reset cut off is 0 and
 // not live); needs ta <= the row's end
 template <typename T, int V, int W>
@@ -88,9 +104,11 @@ __device__ __forceinline__ void load_w(const ConvArgs& p, int d, float (&w)[W][V
 
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
-    const int d = (blockIdx.x * cg.L + threadIdx.x % cg.L) * V, b = blockIdx.y;
-    const int run = blockIdx.z * (256 / cg.L) + threadIdx.x / cg.L, ta = run * cg.seg;
-    if (d >= p.D || run >= cg.n_seg) return;
+    int d = (blockIdx.x * cg.L + threadIdx.x % cg.L) * V, run = blockIdx.z * (256 / cg.L) + threadIdx.x / cg.L;
+    const bool ok = d < p.D && run < cg.n_seg;                                 // idle lanes walk channel 0 or run 0 and write nothing
+    if (d >= p.D) d = 0;
+    if (run >= cg.n_seg) run = 0;                                              // (a whole wave's, where it has one run)
+    const int b = blockIdx.y, ta = run * cg.seg;
     const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), stop = min(tb, end);
     float w[W][V], bias[V], xw[W][V];
     bool live[W];
@@ -102,20 +120,16 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
     if (ta <= end) {
         load_w<V, W>(p, d, w, bias);
         window<T, V, W>(p, b, ta, d, xw, live);
-        if (ta == 0 && end == 0 && p.state_out) put_state();                   // an empty row passes its state on
+        if (ta == 0 && end == 0 && p.state_out && ok) put_state();             // an empty row passes its state on
     }
     const T* x = (const T*)p.x + b * p.x_b + d;
-    for (int t0 = ta; t0 < stop; t0 += BATCH) {
-        float in[BATCH][V];
-        unsigned rm = 0;
+    for (int t0 = ta; t0 < stop; t0 += FB) {
+        float in[FB][V];
 #pragma unroll
-        for (int q = 0; q < BATCH; ++q) {
-            const int t = min(t0 + q, stop - 1);                               // beyond the run: read again, not used
-            cload<T, V>(x + t * p.x_t, in[q]);
-            if (p.reset) rm |= (p.reset[(long long)t * p.B + b] != 0 ? 1u : 0u) << q;
-        }
+        for (int q = 0; q < FB; ++q) cload<T, V>(x + min(t0 + q, stop - 1) * p.x_t, in[q]);      // beyond the run: read again, not used
+        const unsigned rm = reset_bits<FB>(p, cg.L, b, t0, stop);
 #pragma unroll
-        for (int q = 0; q < BATCH; ++q) {
+        for (int q = 0; q < FB; ++q) {
             if (t0 + q >= stop) break;
             if (rm >> q & 1) {
 #pragma unroll
@@ -132,9 +146,10 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
 #pragma unroll
                 for (int k = 0; k < W - 1; ++k) xw[k][i] = xw[k + 1][i];
             }
-            cstore<T, V>(y + (t0 + q) * p.y_t, v);
+            if (ok) cstore<T, V>(y + (t0 + q) * p.y_t, v);
         }
     }
+    if (!ok) return;
     if (stop == end && stop > ta && p.state_out) put_state();                  // the row's last step was this run's
     float zero[V];
     czero(zero);
@@ -148,15 +163,15 @@ template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
     __shared__ float acc[W + 1][256 * V];
     const int lx = threadIdx.x % cg.L, ly = threadIdx.x / cg.L, per = 256 / cg.L;
-    const int d = (blockIdx.x * cg.L + lx) * V;
+    const bool dv = (blockIdx.x * cg.L + lx) * V < p.D;                         // idle lanes walk channel 0 and write nothing
+    const int d = dv ? (blockIdx.x * cg.L + lx) * V : 0;
     float w[W][V], bias[V], dw[W][V], db[V];
-    const bool dv = d < p.D;
-    if (dv) load_w<V, W>(p, d, w, bias);
+    load_w<V, W>(p, d, w, bias);
 #pragma unroll
     for (int k = 0; k < W; ++k) czero(dw[k]);
     czero(db);
     const long long n_runs = (long long)cg.n_seg * p.B;
-    for (long long r = (long long)blockIdx.y * per + ly; dv && r < n_runs; r += (long long)cg.rows * per) {
+    for (long long r = (long long)blockIdx.y * per + ly; r < n_runs; r += (long long)cg.rows * per) {
         const int run = (int)(r / p.B), b = (int)(r - run * p.B), ta = run * cg.seg;
         const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), last = tb + W - 1, stop = min(last, end);
         float xw[W][V], open[W][V];
@@ -170,8 +185,8 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
         const auto emit = [&](int t) {
             const int tau = t - W + 1;
             if (tau < 0) {
-                if (p.dstate_in && ta == 0) cstore<T, V>((T*)p.dstate_in + ((long long)b * (W - 1) + tau + W - 1) * p.D + d, open[0]);
-            } else if (tau >= ta) {
+                if (p.dstate_in && ta == 0 && dv) cstore<T, V>((T*)p.dstate_in + ((long long)b * (W - 1) + tau + W - 1) * p.D + d, open[0]);
+            } else if (tau >= ta && dv) {
                 cstore<T, V>(dx + tau * p.dx_t, open[0]);
             }
 #pragma unroll
@@ -182,18 +197,17 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
             }
             czero(open[W - 1]);
         };
-        for (int t0 = ta; t0 < stop; t0 += BATCH) {
-            float in[BATCH][V], gy[BATCH][V];
-            unsigned rm = 0;
+        for (int t0 = ta; t0 < stop; t0 += BB) {
+            float in[BB][V], gy[BB][V];
 #pragma unroll
-            for (int q = 0; q < BATCH; ++q) {
+            for (int q = 0; q < BB; ++q) {
                 const int t = min(t0 + q, stop - 1);
                 cload<T, V>(x + t * p.x_t, in[q]);
                 cload<T, V>(dy + t * p.dy_t, gy[q]);
-                if (p.reset) rm |= (p.reset[(long long)t * p.B + b] != 0 ? 1u : 0u) << q;
             }
+            const unsigned rm = reset_bits<BB>(p, cg.L, b, t0, stop);
 #pragma unroll
-            for (int q = 0; q < BATCH; ++q) {
+            for (int q = 0; q < BB; ++q) {
                 const int t = t0 + q;
                 if (t >= stop) break;
                 if (rm >> q & 1) {
@@ -309,14 +323,17 @@ static bool conv_ok(long long T, long long B, long long D, long long W) {
     return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && D > 0 && D < (1ll << 29) && W >= 2 && W <= 4;
 }
 
-// Runs of 16 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves. vec: V > 1.
-static ConvGrid conv_grid(long long T, long long B, long long D, bool vec) {
+// Runs of 16 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves. The backward
+// walks W - 1 steps more than a run has: its runs are that much short of 18, 36 or 60. vec: V > 1.
+static ConvGrid conv_grid(long long T, long long B, long long D, bool vec, int extra) {
     const long long cv = vec ? D / 4 : D;
     int L = 1;
     while (L < cv && L < 256) L *= 2;
     const long long waves = (cv + L - 1) / L * L * B / 64;                    // of one run a row
-    int seg = 16;
-    while (seg < 64 && waves * ((T + 2 * seg - 1) / (2 * seg)) >= 4096) seg *= 2;
+    const int choice[2][3] = {{16, 32, 64}, {18 - extra, 36 - extra, 60 - extra}};
+    int k = 0;
+    while (k < 2 && waves * ((T + choice[extra > 0][k + 1] - 1) / choice[extra > 0][k + 1]) >= 4096) ++k;
+    const int seg = choice[extra > 0][k];
     const long long n_seg = (T + seg - 1) / seg, blocks = (n_seg * B + 256 / L - 1) / (256 / L), cols = (cv + L - 1) / L;
     long long rows = (1024 + cols - 1) / cols;
     if (rows > blocks) rows = blocks;
@@ -326,7 +343,7 @@ static ConvGrid conv_grid(long long T, long long B, long long D, bool vec) {
 // floats of scratch of a backward pass, whatever the alignment of its tensors
 DRL_API int drl_short_conv_ws(long long T, long long B, long long D, long long W, long long* n) {
     if (!conv_ok(T, B, D, W)) return -1;
-    const int a = conv_grid(T, B, D, false).rows, b = D % 4 ? 0 : conv_grid(T, B, D, true).rows;
+    const int a = conv_grid(T, B, D, false, W - 1).rows, b = D % 4 ? 0 : conv_grid(T, B, D, true, W - 1).rows;
     *n = (a > b ? a : b) * (W + 1) * D;
     return 0;
 }
@@ -353,7 +370,7 @@ DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(p.T, p.B, p.D, p.W)) return -1;
     const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
-    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec);
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec, 0);
     const long long cv = vec ? p.D / 4 : p.D, per = 256 / cg.L;
     if ((cg.n_seg + per - 1) / per > 65535) return -1;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)p.B, (unsigned)((cg.n_seg + per - 1) / per));
@@ -367,7 +384,7 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
     if (drl_short_conv_ws(p.T, p.B, p.D, p.W, &need)) return -1;
     if (p.ws_n < need) return -2;
     const bool vec = conv_vec(p, bf16 ? 2 : 4, true);
-    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec);
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec, (int)p.W - 1);
     const long long cv = vec ? p.D / 4 : p.D, n = (p.W + 1) * p.D;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)cg.rows);
     CONV_ALL(k_conv_bwd, grid, p, cg)

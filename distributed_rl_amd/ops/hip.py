@@ -1082,6 +1082,15 @@ def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, o
     return (t.data_ptr(),) + st[:-1]
 
 
+def _row2(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, out: bool = False) -> tuple:
+    """``_rows`` of a 2-d tensor that is needed, quick where it is contiguous (single steps are bound by these checks)."""
+    if t is None:
+        _refuse(t, shape, dtype, dev, name)
+    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+        return t.data_ptr(), shape[1]
+    return _rows(t, shape, dtype, dev, name, out)
+
+
 def _apart(outs: tuple, ins: tuple) -> None:
     """No output starts where an input or another output does (0: not given)."""
     for i, a in enumerate(outs):
@@ -1126,11 +1135,10 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
     if not eps >= 0:
         raise ValueError("eps must not be negative (got %r)" % (eps,))
     shape, typ, f32 = _norm_shape(x), x.dtype, torch.float32
-    _need(w=w, y=y)
     dev, bf16 = _dev(x), _typ(x)
     M, D = shape
-    xp, xs = _rows(x, shape, typ, dev, "x")
-    yp, ys = _rows(y, shape, typ, dev, "y", True)
+    xp, xs = _row2(x, shape, typ, dev, "x")
+    yp, ys = _row2(y, shape, typ, dev, "y", True)
     wp, bp = _vec(w, (D,), f32, dev, "w"), _opt(b, (D,), f32, dev, "b")
     mp, rp = _opt(mean, (M,), f32, dev, "mean"), _opt(rstd, (M,), f32, dev, "rstd")
     _apart((yp, mp, rp), (xp, wp, bp))
@@ -1152,7 +1160,8 @@ def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
 
 
 def _norm_shape(x) -> torch.Size:
-    _need(x=x)
+    if x is None:
+        raise ValueError("x is needed")
     shape = x.shape
     if len(shape) != 2 or not 0 < shape[0] < 1 << 31 or not 0 < shape[1] <= 16384:
         raise ValueError("layer_norm: x must be [rows, D], D <= 16384 (got %s)" % (tuple(shape),))
@@ -1210,15 +1219,16 @@ def short_conv_bwd(dy, x, w, bias, dx, dw, db, ws, state_in=None, dstate_in=None
 
 def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None:
     """One step of :func:`short_conv_fwd` for x [B, D]: ``state`` [B, W-1, D] is shifted in place, ``reset`` uint8 [B]."""
-    _need(x=x, w=w, y=y)
+    if x is None or w is None:
+        raise ValueError("x and w are needed")
     shape, W = x.shape, w.shape[-1]
     if len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or not 2 <= W <= 4:
         raise ValueError("short_conv_step: x must be [B, D], w [D, 2 .. 4] (got %s, %s)" % (tuple(shape), tuple(w.shape)))
     B, D = shape
     dev, typ, f32 = _dev(x), x.dtype, torch.float32
     bf16 = _typ(x)
-    xp, xs = _rows(x, shape, typ, dev, "x")
-    yp, ys = _rows(y, shape, typ, dev, "y", True)
+    xp, xs = _row2(x, shape, typ, dev, "x")
+    yp, ys = _row2(y, shape, typ, dev, "y", True)
     sp, rp = _vec(state, (B, W - 1, D), typ, dev, "state"), _opt(reset, (B,), torch.uint8, dev, "reset")
     wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
     _apart((yp, sp), (xp, wp, bp, rp))
@@ -1305,7 +1315,8 @@ def ssm_scan_bwd(dy, u, dt, A, Bm, Cm, ckpt, du, ddt, dA, dB, dC, ws, D=None, dD
 def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, softplus: bool = True) -> None:
     """One step of :func:`ssm_scan_fwd` for u, dt, z, y [B, D] and Bm, Cm [B, N]: ``h`` [B, D, N] fp32 is updated in place,
     ``reset`` uint8 [B]."""
-    _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, y=y)
+    if u is None or Bm is None:
+        raise ValueError("u and Bm are needed")
     shape, bc = u.shape, Bm.shape
     if len(shape) != 2 or len(bc) != 2 or shape[0] < 1 or shape[1] < 1 or not 0 < bc[1] <= 64:
         raise ValueError("ssm_step: u must be [B, D], Bm [B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
@@ -1313,12 +1324,12 @@ def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, s
     N = bc[1]
     dev, typ, f32 = _dev(u), u.dtype, torch.float32
     bf16, bc = _typ(u), (B, N)
-    up, us = _rows(u, shape, typ, dev, "u")
-    dtp, dts = _rows(dt, shape, typ, dev, "dt")
-    zp, zs = _rows(z, shape, typ, dev, "z")
-    Bp, Bs = _rows(Bm, bc, typ, dev, "Bm")
-    Cp, Cs = _rows(Cm, bc, typ, dev, "Cm")
-    yp, ys = _rows(y, shape, typ, dev, "y", True)
+    up, us = _row2(u, shape, typ, dev, "u")
+    dtp, dts = _row2(dt, shape, typ, dev, "dt")
+    zp, zs = _row2(z, shape, typ, dev, "z") if z is not None else (0, 0)
+    Bp, Bs = _row2(Bm, bc, typ, dev, "Bm")
+    Cp, Cs = _row2(Cm, bc, typ, dev, "Cm")
+    yp, ys = _row2(y, shape, typ, dev, "y", True)
     Ap, hp, rp = _vec(A, (Dc, N), f32, dev, "A"), _vec(h, (B, Dc, N), f32, dev, "h"), _opt(reset, (B,), torch.uint8, dev, "reset")
     Dp, bp = _opt(D, (Dc,), f32, dev, "D"), _opt(dt_bias, (Dc,), f32, dev, "dt_bias")
     _apart((yp, hp), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, rp))
