@@ -1041,8 +1041,7 @@ def _typ(t: torch.Tensor) -> int:
 
 
 def _refuse(t, shape, dtype, dev: int, name: str):
-    if t is None:
-        raise ValueError("%s is needed" % name)
+    _need(**{name: t})
     if t.dtype is not dtype or t.get_device() != dev:
         raise TypeError("%s must be a %s tensor on cuda:%d (got %s on %s)" % (name, dtype, dev, t.dtype, t.device))
     raise ValueError("%s must be contiguous of shape %s (got %s, strides %s)" % (name, tuple(shape), tuple(t.shape), t.stride()))
@@ -1131,6 +1130,8 @@ def layer_norm_ws(M: int, D: int, device) -> torch.Tensor:
 def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
     """y[r] = (x[r] - mean) * rstd * w + b over the last axis of x [rows, D], D <= 16384. w fp32 [D], b fp32 [D] or None;
     ``mean`` / ``rstd`` (fp32 [rows], both or neither) keep the statistics for :func:`layer_norm_bwd`."""
+    if x is None or w is None or y is None:
+        _need(x=x, w=w, y=y)
     _none_or_both(mean, rstd, "mean and rstd")
     if not eps >= 0:
         raise ValueError("eps must not be negative (got %r)" % (eps,))
@@ -1148,8 +1149,8 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
 def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
     """Gradients of :func:`layer_norm_fwd`: dx [rows, D], dw and db (None if the norm has no b) fp32 [D], overwritten. The
     sums over rows run in a fixed order. ``ws`` from :func:`layer_norm_ws`."""
+    _need(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dw=dw, ws=ws)
     shape, typ, f32 = _norm_shape(x), x.dtype, torch.float32
-    _need(dy=dy, dx=dx, ws=ws)
     dev, bf16 = _dev(x), _typ(x)
     M, D = shape
     xr, dyr, dxr = _rows(x, shape, typ, dev, "x"), _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
@@ -1160,8 +1161,6 @@ def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
 
 
 def _norm_shape(x) -> torch.Size:
-    if x is None:
-        raise ValueError("x is needed")
     shape = x.shape
     if len(shape) != 2 or not 0 < shape[0] < 1 << 31 or not 0 < shape[1] <= 16384:
         raise ValueError("layer_norm: x must be [rows, D], D <= 16384 (got %s)" % (tuple(shape),))
@@ -1219,8 +1218,8 @@ def short_conv_bwd(dy, x, w, bias, dx, dw, db, ws, state_in=None, dstate_in=None
 
 def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None:
     """One step of :func:`short_conv_fwd` for x [B, D]: ``state`` [B, W-1, D] is shifted in place, ``reset`` uint8 [B]."""
-    if x is None or w is None:
-        raise ValueError("x and w are needed")
+    if x is None or w is None or state is None or y is None:
+        _need(x=x, w=w, state=state, y=y)
     shape, W = x.shape, w.shape[-1]
     if len(shape) != 2 or shape[0] < 1 or shape[1] < 1 or not 2 <= W <= 4:
         raise ValueError("short_conv_step: x must be [B, D], w [D, 2 .. 4] (got %s, %s)" % (tuple(shape), tuple(w.shape)))
@@ -1315,8 +1314,8 @@ def ssm_scan_bwd(dy, u, dt, A, Bm, Cm, ckpt, du, ddt, dA, dB, dC, ws, D=None, dD
 def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, softplus: bool = True) -> None:
     """One step of :func:`ssm_scan_fwd` for u, dt, z, y [B, D] and Bm, Cm [B, N]: ``h`` [B, D, N] fp32 is updated in place,
     ``reset`` uint8 [B]."""
-    if u is None or Bm is None:
-        raise ValueError("u and Bm are needed")
+    if u is None or dt is None or A is None or Bm is None or Cm is None or h is None or y is None:
+        _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, h=h, y=y)
     shape, bc = u.shape, Bm.shape
     if len(shape) != 2 or len(bc) != 2 or shape[0] < 1 or shape[1] < 1 or not 0 < bc[1] <= 64:
         raise ValueError("ssm_step: u must be [B, D], Bm [B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
