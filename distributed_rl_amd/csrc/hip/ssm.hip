@@ -260,7 +260,7 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
             float v = R::value(rv[i]);
             if (BWD && p.z) { const float z = R::value(rz[i]); v *= z * sigmoidf(z); }
             float sp = R::value(rd[i]) + bias;
-            if (p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
+            if (p.softplus) sp = softplus(sp);
             sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
             sum += sp;
             pw_s[w][4 * i + g][j] = make_float2(sp, BWD ? v : sp * v);
@@ -370,7 +370,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
             zz[i] = 1.f;
             if (p.z) { const float z = R::value(rz[i]); zz[i] = z * sigmoidf(z); }
             float sp = R::value(rd[i]) + bias;
-            if (p.softplus) sp = softplus_from(sp, exp_neg_abs(sp));
+            if (p.softplus) sp = softplus(sp);
             sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
             pw_s[w][4 * i + g][j] = make_float2(sp, sp * u[i]);
         }
@@ -591,11 +591,7 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
             const bool ok = dv && t0 + 4 * i + g < end;
             const float u = R::value(ru[i]), dy = R::value(ry[i]);
             float sp = R::value(rd[i]) + bias, ds = dy, sg = 1.f, dz = 0.f;
-            if (soft) {
-                const float e = exp_neg_abs(sp);
-                sg = sigmoid_from(sp, e);
-                sp = softplus_from(sp, e);
-            }
+            if (soft) sp = softplus(sp, &sg);
             sp = ok ? sp : 0.f;
             if (has_z) {
                 const float z = R::value(rz[i]), sz = sigmoidf(z);
@@ -756,7 +752,7 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
     for (int k = 0; k < R; ++k) {
         const long long i = i0 + k * step;
         float s = dt[k], y = 0.f;
-        if (p.softplus) s = softplus_from(s, exp_neg_abs(s));
+        if (p.softplus) s = softplus(s);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const float e = __builtin_amdgcn_exp2f(s * (A[k][v] * LOG2E));
