@@ -236,6 +236,7 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
     const int n_chunks = max(0, (min(tb, end) - ta + KC - 1) / KC);
     float sum = 0.f;
     bool cut = false;
+    const bool has_z = p.z != nullptr, soft = p.softplus != 0;
     unsigned rv[4], rd[4], rz[4], rr;
     const int t_first = BWD ? ta + max(0, n_chunks - 1) * KC : ta;
     R xv(v_p, v_t, v_b, b, t_first), xd(p.dt, p.dt_t, p.dt_b, b, t_first), xz(p.z, p.z_t, p.z_b, b, t_first);
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
             const unsigned bad = dv && t0 + 4 * i + g < end ? 0u : OOB;
             rv[i] = R::load(xv.rsrc(), ov | bad, i * xv.four);
             rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
-            if (BWD && p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
+            if (BWD && has_z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
         }
         st.fetch(end - t0);
         rr = fetch_resets(p, b, t0, end, lane);
@@ -255,15 +256,23 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
     if (n_chunks) fetch(t_first);
     for (int c = 0; c < n_chunks; ++c) {
         const int t0 = ta + (BWD ? n_chunks - 1 - c : c) * KC;
+        // the flags are asked once, outside: the four elements' chains of operations then overlap
+        float v[4], sp[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = R::value(rv[i]); sp[i] = R::value(rd[i]) + bias; }
+        if (BWD && has_z) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const float z = R::value(rz[i]); v[i] *= z * sigmoidf(z); }
+        }
+        if (soft) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sp[i] = softplus(sp[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float v = R::value(rv[i]);
-            if (BWD && p.z) { const float z = R::value(rz[i]); v *= z * sigmoidf(z); }
-            float sp = R::value(rd[i]) + bias;
-            if (p.softplus) sp = softplus(sp);
-            sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
-            sum += sp;
-            pw_s[w][4 * i + g][j] = make_float2(sp, BWD ? v : sp * v);
+            sp[i] = dv && t0 + 4 * i + g < end ? sp[i] : 0.f;
+            sum += sp[i];
+            pw_s[w][4 * i + g][j] = make_float2(sp[i], BWD ? v[i] : sp[i] * v[i]);
         }
         float* bcb = bc_s[c & 1];
         st.put(bcb);
@@ -345,6 +354,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     for (int i = 0; i < NS; ++i) A2[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
     const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.y_t, g, d);
+    const bool has_z = p.z != nullptr, soft = p.softplus != 0;
     unsigned ru[4], rd[4], rz[4], rr;
     R xu(p.u, p.u_t, p.u_b, b, ta), xd(p.dt, p.dt_t, p.dt_b, b, ta), xz(p.z, p.z_t, p.z_b, b, ta), xy(p.y, p.y_t, p.y_b, b, ta);
     StageBC<T, NS, 3> st(p, b, ta);
@@ -354,7 +364,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
             const unsigned bad = dv && t0 + 4 * i + g < end ? 0u : OOB;
             ru[i] = R::load(xu.rsrc(), ou | bad, i * xu.four);
             rd[i] = R::load(xd.rsrc(), od | bad, i * xd.four);
-            if (p.z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
+            if (has_z) rz[i] = R::load(xz.rsrc(), oz | bad, i * xz.four);
         }
         st.fetch(end - t0);
         rr = fetch_resets(p, b, t0, end, lane);
@@ -363,16 +373,21 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     const int live = min(tb, end);                          // padding is not walked: its rows are zeroed below
     if (live > ta) fetch(ta);
     for (int t0 = ta, c = 0; t0 < live; t0 += KC, ++c) {
-        float u[4], zz[4];
+        float u[4], zz[4], sp[4];                           // flags outside: see k_ssm_carry
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { u[i] = R::value(ru[i]); zz[i] = 1.f; sp[i] = R::value(rd[i]) + bias; }
+        if (has_z) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { const float z = R::value(rz[i]); zz[i] = z * sigmoidf(z); }
+        }
+        if (soft) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sp[i] = softplus(sp[i]);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            u[i] = R::value(ru[i]);
-            zz[i] = 1.f;
-            if (p.z) { const float z = R::value(rz[i]); zz[i] = z * sigmoidf(z); }
-            float sp = R::value(rd[i]) + bias;
-            if (p.softplus) sp = softplus(sp);
-            sp = dv && t0 + 4 * i + g < end ? sp : 0.f;
-            pw_s[w][4 * i + g][j] = make_float2(sp, sp * u[i]);
+            sp[i] = dv && t0 + 4 * i + g < end ? sp[i] : 0.f;
+            pw_s[w][4 * i + g][j] = make_float2(sp[i], sp[i] * u[i]);
         }
         float* bcb = bc_s[c & 1];
         st.put(bcb);
@@ -586,20 +601,29 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     if (live > ta) fetch(t_last);
     int c = 0;
     for (int t0 = live > ta ? t_last : ta - 1; t0 >= ta; t0 -= KC, ++c) {
+        {
+            float sp[4], ds[4], sg[4], dz[4];               // flags outside: see k_ssm_carry
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bool ok = dv && t0 + 4 * i + g < end;
-            const float u = R::value(ru[i]), dy = R::value(ry[i]);
-            float sp = R::value(rd[i]) + bias, ds = dy, sg = 1.f, dz = 0.f;
-            if (soft) sp = softplus(sp, &sg);
-            sp = ok ? sp : 0.f;
+            for (int i = 0; i < 4; ++i) { sp[i] = R::value(rd[i]) + bias; ds[i] = R::value(ry[i]); sg[i] = 1.f; dz[i] = 0.f; }
             if (has_z) {
-                const float z = R::value(rz[i]), sz = sigmoidf(z);
-                ds = dy * (z * sz);
-                dz = dy * sz * fmaf(z, 1.f - sz, 1.f);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float z = R::value(rz[i]), sz = sigmoidf(z);
+                    dz[i] = ds[i] * sz * fmaf(z, 1.f - sz, 1.f);
+                    ds[i] *= z * sz;
+                }
             }
-            pw_s[w][4 * i + g][j] = make_float4(sp * LOG2E, sp * u, ds, u);
-            ex_s[w][4 * i + g][j] = make_float4(dz, 0.f, sg, 0.f);
+            if (soft) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sp[i] = softplus(sp[i], &sg[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = R::value(ru[i]);
+                sp[i] = dv && t0 + 4 * i + g < end ? sp[i] : 0.f;
+                pw_s[w][4 * i + g][j] = make_float4(sp[i] * LOG2E, sp[i] * u, ds[i], u);
+                ex_s[w][4 * i + g][j] = make_float4(dz[i], 0.f, sg[i], 0.f);
+            }
         }
         float* bcb = bc_s[c & 1];
         st.put(bcb);
