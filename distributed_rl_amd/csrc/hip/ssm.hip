@@ -125,6 +125,28 @@ __device__ __forceinline__ unsigned reset_mask(unsigned flag) { return (unsigned
 
 __device__ __forceinline__ int row_end(const SsmArgs& p, int b) { return p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T; }
 
+// The row of a block. Rows of unequal length are taken longest first, so that no long one starts when the others are through
+// (120 x 64 x 1024 with lengths of 30 .. 120: see k_ssm_bwd): slot k of the grid gets the row with k longer ones, found by
+// counting, 256 rows at most.
+#define SORT_ROWS 256
+__device__ __forceinline__ int block_row(const SsmArgs& p, int* len_s) {
+    const int slot = blockIdx.y, B = (int)p.B;
+    if (!p.lengths || B > SORT_ROWS) return slot;
+    const int r = threadIdx.x;
+    if (r < B) len_s[r] = p.lengths[r];
+    __syncthreads();
+    if (r < B) {
+        const int mine = len_s[r];
+        int rank = 0;
+        for (int k = 0; k < B; ++k) rank += len_s[k] > mine || (len_s[k] == mine && k < r);
+        if (rank == slot) len_s[SORT_ROWS] = r;
+    }
+    __syncthreads();
+    const int b = __builtin_amdgcn_readfirstlane(len_s[SORT_ROWS]);
+    __syncthreads();                                        // len_s is another array's memory
+    return b;
+}
+
 // the states of a lane in a [.., B, D, N] tensor, four at a time (v4: N and the tensor's address allow it, see vec4)
 __host__ __device__ __forceinline__ bool vec4(const float* q, long long N) { return (N & 3) == 0 && ((uintptr_t)q & 15) == 0; }
 template <int NS>
@@ -341,7 +363,8 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     __shared__ __align__(16) float2 pw_s[4][KC][16];
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    const int b = blockIdx.y;
+    static_assert(sizeof(bc_s) > SORT_ROWS * sizeof(int), "block_row");
+    const int b = block_row(p, (int*)bc_s);
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
     const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
@@ -535,7 +558,8 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
     __shared__ float mid_s[KH < KC ? 4 : 1][KH < KC ? KC / KH - 1 : 1][KH < KC ? NS : 1][64];      // states before each piece
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    const int b = blockIdx.y;
+    static_assert(sizeof(bc_s) > SORT_ROWS * sizeof(int), "block_row");
+    const int b = block_row(p, (int*)bc_s);
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
     const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
