@@ -206,7 +206,7 @@ __device__ __forceinline__ float sum_rows2(const float* be, const float* ce, con
         : "v"(be[0]), "v"(be[1]), "v"(bo[0]), "v"(bo[1]), "v"(ce[0]), "v"(ce[1]), "v"(co[0]), "v"(co[1]));
     asm volatile("s_nop 1\n"
         DPP(0, 2, "row_half_mirror", "0x5") DPP(1, 3, "row_half_mirror", "0x5")
-        DPP(0, 4, "row_half_mirror", "0xa") DPP(1, 5, "row_half_mirror", "0xa")
+        DPP(0, 4, "row_half_mirror", "0xa") DPP(1, 5, "row_half_mirror", "0xa") "s_nop 1\n"
         : "=&v"(r0), "=&v"(r1) : "v"(t0), "v"(t1), "v"(t2), "v"(t3));
     float v = quad_fold<QUAD_XOR1>(j & 1, r0, r1);
     return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), QUAD_XOR2, 0xf, 0xf, true));
@@ -224,6 +224,7 @@ __device__ __forceinline__ float sum_rows4(const float* be, const float* ce, con
     asm volatile("s_nop 1\n"
         DPP(0, 4, "row_half_mirror", "0x5") DPP(1, 5, "row_half_mirror", "0x5") DPP(2, 6, "row_half_mirror", "0x5") DPP(3, 7, "row_half_mirror", "0x5")
         DPP(0, 8, "row_half_mirror", "0xa") DPP(1, 9, "row_half_mirror", "0xa") DPP(2, 10, "row_half_mirror", "0xa") DPP(3, 11, "row_half_mirror", "0xa")
+        "s_nop 1\n"                               // what follows may read the sums across lanes
         : "=&v"(r[0]), "=&v"(r[1]), "=&v"(r[2]), "=&v"(r[3])
         : "v"(t[0]), "v"(t[1]), "v"(t[2]), "v"(t[3]), "v"(t[4]), "v"(t[5]), "v"(t[6]), "v"(t[7]));
     return quad_fold<QUAD_XOR2>(j & 2, quad_fold<QUAD_XOR1>(j & 1, r[0], r[1]), quad_fold<QUAD_XOR1>(j & 1, r[2], r[3]));

@@ -1020,6 +1020,8 @@ def add2(a, b, out) -> None:
 # may not share memory with an input. Scratch (``*_ws``) belongs to the caller: calls that may run at the same time (two
 # streams, two graphs) need one each.
 _NORM, _CONV, _SSM = (struct.Struct("<%dq" % n) for n in (18, 29, 56))
+_NORM_FWD, _CONV_STEP, _SSM_STEP = (struct.Struct("<%dq%dx" % (n, 8 * m)) for n, m in ((10, 8), (17, 12), (33, 23)))     # the rest zero
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dev(t: torch.Tensor) -> int:
@@ -1081,19 +1083,19 @@ def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, o
     return (t.data_ptr(),) + st[:-1]
 
 
-def _row2(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, out: bool = False) -> tuple:
-    """``_rows`` of a 2-d tensor that is needed, quick where it is contiguous (single steps are bound by these checks)."""
-    if t is None:
+def _row2(t: torch.Tensor, shape: tuple, dtype, dev: int, name: str, out: bool = False) -> tuple:
+    """``_rows`` of a 2-d tensor, quick where it is contiguous: small single steps are bound by these checks."""
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
         _refuse(t, shape, dtype, dev, name)
-    if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == dev:
+    if t.is_contiguous():
         return t.data_ptr(), shape[1]
     return _rows(t, shape, dtype, dev, name, out)
 
 
 def _apart(outs: tuple, ins: tuple) -> None:
     """No output starts where an input or another output does (0: not given)."""
-    for i, a in enumerate(outs):
-        if a and (a in ins or a in outs[i + 1:]):
+    for a in outs:
+        if a and (a in ins or outs.count(a) > 1):
             raise ValueError("an output shares its memory with an input or another output")
 
 
@@ -1114,9 +1116,9 @@ def _ws_numel(rc: int, n: ctypes.c_longlong, what: str, sizes) -> int:
     return n.value
 
 
-def _run(fn, *args) -> None:
-    """Launch on the current stream of the tensors' device (the last argument is its ordinal)."""
-    rc = fn(*args[:-1], torch._C._cuda_getCurrentRawStream(args[-1]))
+def _run(fn, rec: bytes, bf16: int, dev: int) -> None:
+    """Launch on the current stream of the tensors' device."""
+    rc = fn(rec, bf16, _raw_stream(dev))
     if rc != 0:
         raise RuntimeError("%s failed with code %d%s" % (fn.__name__, rc, " (workspace too small)" if rc == -2 else ""))
 
@@ -1143,7 +1145,7 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
     wp, bp = _vec(w, (D,), f32, dev, "w"), _opt(b, (D,), f32, dev, "b")
     mp, rp = _opt(mean, (M,), f32, dev, "mean"), _opt(rstd, (M,), f32, dev, "rstd")
     _apart((yp, mp, rp), (xp, wp, bp))
-    _run(native.hip().drl_norm_fwd, _NORM.pack(xp, xs, wp, bp, yp, ys, mp, rp, M, D, 0, 0, 0, 0, 0, 0, 0, 0), bf16, float(eps), dev)
+    _ck(native.hip().drl_norm_fwd(_NORM_FWD.pack(xp, xs, wp, bp, yp, ys, mp, rp, M, D), bf16, eps, _raw_stream(dev)), "layer_norm_fwd")
 
 
 def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
@@ -1231,8 +1233,7 @@ def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None
     sp, rp = _vec(state, (B, W - 1, D), typ, dev, "state"), _opt(reset, (B,), torch.uint8, dev, "reset")
     wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
     _apart((yp, sp), (xp, wp, bp, rp))
-    _run(native.hip().drl_short_conv_step, _CONV.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0, 0, 0, 0, 0,
-                                                      0, 0, 0, 0, 0, 0, 0, 0), bf16, dev)
+    _run(native.hip().drl_short_conv_step, _CONV_STEP.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0), bf16, dev)
 
 
 SSM_CHUNK = 16              # steps between the states that ssm_scan_fwd saves for ssm_scan_bwd
@@ -1332,8 +1333,5 @@ def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, s
     Ap, hp, rp = _vec(A, (Dc, N), f32, dev, "A"), _vec(h, (B, Dc, N), f32, dev, "h"), _opt(reset, (B,), torch.uint8, dev, "reset")
     Dp, bp = _opt(D, (Dc,), f32, dev, "D"), _opt(dt_bias, (Dc,), f32, dev, "dt_bias")
     _apart((yp, hp), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, rp))
-    _run(native.hip().drl_ssm_step, _SSM.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys, hp,
-                                              0, 0, 0, 1, B, Dc, N, 1 if softplus else 0, *_ZEROS23), bf16, dev)
-
-
-_ZEROS23 = (0,) * 23
+    _run(native.hip().drl_ssm_step, _SSM_STEP.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys,
+                                                   hp, 0, 0, 0, 1, B, Dc, N, 1 if softplus else 0), bf16, dev)

@@ -277,6 +277,23 @@ def test_scan_long_and_few_rows(T, B, D, N, dtype):
     check_scan(scan_case(T, B, D, N, dtype, reset=0, ragged=False, shift=-4.0, scale=0.3))
 
 
+@pytest.mark.parametrize("T,B,D", [(20, 3, 40), (600, 1, 16)])                              # one segment, and several
+def test_scan_state_of_a_finished_episode_is_never_used(T, B, D):
+    v = scan_case(T, B, D, 16, F32, ragged=False, reset=0.01, shift=-4.0, scale=0.3)
+    v["reset"][0] = 1
+    v["h0"].zero_()
+    a = run_scan(v)
+    v["h0"].fill_(float("nan"))
+    b = run_scan(v)
+    assert all(torch.equal(a[k], b[k]) for k in a)
+    assert bool((b["dh0"] == 0).all())
+
+
+@pytest.mark.parametrize("B", [255, 256, 257, 300])
+def test_scan_padded_rows_around_the_sorted_count(B):
+    check_scan(scan_case(18, B, 5, 3, F32))
+
+
 def test_scan_of_views():
     g = Gen(11)
     T, B, D, N = 25, 3, 40, 16
@@ -350,6 +367,57 @@ def test_step_of_views():
     assert torch.equal(y[:, :D], y2) and torch.equal(h, h2) and bool((y[:, D:] == 7).all())
 
 
+# ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
+def test_norm_past_32_bits():
+    M, D = 150000, 16384                                    # 2.46e9 elements
+    x = torch.empty(M, D, dtype=BF, device=DEV)
+    x.random_(-8, 9)
+    y, w = torch.empty_like(x), torch.ones(D, device=DEV)
+    mean, rstd = torch.empty(M, device=DEV), torch.empty(M, device=DEV)
+    H.layer_norm_fwd(x, w, None, y, mean=mean, rstd=rstd)
+    part = torch.empty(3, D, dtype=BF, device=DEV)
+    H.layer_norm_fwd(x[-3:], w, None, part)
+    assert torch.equal(y[-3:], part)
+    dw = torch.empty(D, device=DEV)
+    H.layer_norm_bwd(x, x, w, mean, rstd, y, dw, None, H.layer_norm_ws(M, D, DEV))
+    dx = torch.empty_like(part)
+    H.layer_norm_bwd(x[-3:], x[-3:], w, mean[-3:], rstd[-3:], dx, dw, None, H.layer_norm_ws(3, D, DEV))
+    assert torch.equal(y[-3:], dx)
+
+
+def test_conv_and_scan_past_32_bits():
+    T, B, D, N = 2100, 1024, 1024, 2                        # 2.2e9 elements a tensor
+    g = Gen(0)
+    x = torch.empty(T, B, D, dtype=BF, device=DEV)
+    x.random_(-2, 3)
+    y, dx = torch.empty_like(x), torch.empty_like(x)
+    w, dw = g.n(D, 4), torch.empty(D, 4, device=DEV)
+    last = x[:, -1:].contiguous()
+    p, q = torch.empty_like(last), torch.empty_like(last)
+    H.short_conv_fwd(x, w, None, y)
+    H.short_conv_fwd(last, w, None, p)
+    assert torch.equal(y[:, -1:], p)
+    H.short_conv_bwd(x, x, w, None, dx, dw, None, H.short_conv_ws(T, B, D, 4, DEV))
+    H.short_conv_bwd(last, last, w, None, q, dw, None, H.short_conv_ws(T, 1, D, 4, DEV))
+    assert torch.equal(dx[:, -1:], q)
+    A, bc = -g.u(D, N) - 0.5, g.n(T, B, 2 * N, dtype=BF)
+    ws, ck = H.ssm_scan_ws(T, B, D, N, DEV), H.ssm_scan_ckpt(T, B, D, N, DEV)
+    H.ssm_scan_fwd(x, x, A, bc[..., :N], bc[..., N:], y, ws, ckpt=ck)
+    dA, dB, dC = torch.empty(D, N, device=DEV), torch.empty(T, B, N, dtype=BF, device=DEV), torch.empty(T, B, N, dtype=BF, device=DEV)
+    ddt = torch.empty_like(x)
+    H.ssm_scan_bwd(x, x, x, A, bc[..., :N], bc[..., N:], ck, dx, ddt, dA, dB, dC, ws)
+    # the last row by itself: cut into segments there, so equal up to rounding (2 100 steps, decays of at most exp(-0.06))
+    bl = bc[:, -1:].contiguous()
+    o = [torch.empty_like(last) for _ in range(3)]
+    oB, oC = torch.empty(T, 1, N, dtype=BF, device=DEV), torch.empty(T, 1, N, dtype=BF, device=DEV)
+    ws, ck = H.ssm_scan_ws(T, 1, D, N, DEV), H.ssm_scan_ckpt(T, 1, D, N, DEV)
+    H.ssm_scan_fwd(last, last, A, bl[..., :N], bl[..., N:], o[0], ws, ckpt=ck)
+    H.ssm_scan_bwd(last, last, last, A, bl[..., :N], bl[..., N:], ck, o[1], o[2], dA, oB, oC, ws)
+    for a, b in ((y[:, -1:], o[0]), (dx[:, -1:], o[1]), (ddt[:, -1:], o[2]), (dB[:, -1:], oB), (dC[:, -1:], oC)):
+        a, b = a.double(), b.double()
+        assert float((a - b).norm() / b.norm()) < 2.0 ** -8                # each is rounded to bf16 once: 2^-8 between the two
+
+
 # ---- same inputs, same bits; streams; graphs ----------------------------------------------------------------------------
 def test_results_do_not_change_from_call_to_call():
     for v in (scan_case(70, 5, 96, 16, BF), scan_case(523, 1, 40, 8, F32)):
@@ -421,7 +489,7 @@ def test_the_operators_together_against_autograd_in_64_bits():
                  dh0=p["h0"].grad)
     for k, ref in pairs.items():
         # the longest chain: 2 x 40 steps of (14 + exponents) roundings and sums over 160 rows; 2e-4 = 3 400 half steps
-        got = s[k].cpu().double()
+        got, ref = s[k].cpu().double(), ref.detach()
         assert float((got - ref).norm() / ref.norm()) < 2e-4, k
 
 
@@ -471,6 +539,17 @@ def test_captured_and_replayed_on_new_inputs():
 
 
 # ---- refusals on the GPU ------------------------------------------------------------------------------------------------
+def test_tensors_of_another_device_than_the_current_one_are_refused(monkeypatch):
+    x, w = torch.zeros(2, 8, device=DEV), torch.ones(8, device=DEV)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        H.layer_norm_fwd(x, w, w, torch.empty_like(x))
+    with pytest.raises(ValueError, match="current device"):
+        H.short_conv_step(x, torch.zeros(8, 4, device=DEV), w, torch.zeros(2, 3, 8, device=DEV), torch.empty_like(x))
+    with pytest.raises(ValueError, match="current device"):
+        H.ssm_step(x, x.clone(), torch.zeros(8, 2, device=DEV), x[:, :2], x[:, 2:4], torch.zeros(2, 8, 2, device=DEV), torch.empty_like(x))
+
+
 def test_refusals():
     g = Gen(0)
     T, B, D, N = 5, 2, 8, 4
