@@ -7,6 +7,7 @@
 // allow it) of one row and a run of steps, reads FB (BB) steps ahead and keeps the last W - 1 inputs in registers. Runs of one
 // row are walked side by side; each starts by reading the W - 1 steps before it again.
 #include "ssm_math.h"
+#include <type_traits>
 
 #define FB 16            // steps read ahead by the forward
 #define BB 6             // and by the backward (two tensors)
@@ -60,36 +61,40 @@ __device__ __forceinline__ int row_end(const ConvArgs& p, int b) {
 }
 __device__ __forceinline__ bool resets(const ConvArgs& p, int b, int t) { return t >= 0 && p.reset && p.reset[(long long)t * p.B + b] != 0; }
 
-// bit q: step t0 + q (< stop) has its reset flag set. With 64 or more threads across the channels a wave has one row and one
-// run: a lane reads a flag. Every lane of the wave takes part.
-template <int N>
-__device__ __forceinline__ unsigned reset_bits(const ConvArgs& p, int L, int b, int t0, int stop) {
+// WIDE: 64 or more threads across the channels, so a wave has one row and one run, whose steps and flags are scalars.
+template <bool WIDE>
+__device__ __forceinline__ int uniform(int v) { return WIDE ? __builtin_amdgcn_readfirstlane(v) : v; }
+
+// bit q: step t0 + q (0 <= it < stop) has its reset flag set. WIDE: a lane reads a flag, every lane of the wave takes part.
+template <int N, bool WIDE>
+__device__ __forceinline__ unsigned reset_bits(const ConvArgs& p, int b, int t0, int stop) {
     if (!p.reset) return 0;
-    if (L >= 64) {
+    if constexpr (WIDE) {
         const int q = threadIdx.x & 63;
-        return (unsigned)__ballot(q < N && t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0);
+        return (unsigned)__ballot(q < N && t0 + q >= 0 && t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0);
     }
     unsigned rm = 0;
 #pragma unroll
-    for (int q = 0; q < N; ++q) rm |= (t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0 ? 1u : 0u) << q;
+    for (int q = 0; q < N; ++q) rm |= (t0 + q >= 0 && t0 + q < stop && p.reset[(long long)(t0 + q) * p.B + b] != 0 ? 1u : 0u) << q;
     return rm;
 }
 
 // xw[0 .. W - 2] = the inputs of times ta - W + 1 .. ta - 1 as the step at ta - 1 leaves them (what a reset cut off is 0 and
 // not live); needs ta <= the row's end
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool WIDE>
 __device__ __forceinline__ void window(const ConvArgs& p, int b, int ta, int d, float (&xw)[W][V], bool (&live)[W]) {
+    const unsigned rm = reset_bits<W - 1, WIDE>(p, b, ta - W + 1, ta);
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) {
         const int t = ta - W + 1 + k;
-        live[k] = true;
-        if (resets(p, b, t)) {
-#pragma unroll
-            for (int q = 0; q < k; ++q) { czero(xw[q]); live[q] = false; }
-        }
         if (t >= 0) cload<T, V>((const T*)p.x + t * p.x_t + b * p.x_b + d, xw[k]);
         else if (p.state_in) cload<T, V>((const T*)p.state_in + ((long long)b * (W - 1) + (t + W - 1)) * p.D + d, xw[k]);
         else czero(xw[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) {
+        live[k] = rm >> (k + 1) == 0;                                          // no episode starts behind it
+        if (!live[k]) czero(xw[k]);
     }
 }
 template <int V, int W>
@@ -102,16 +107,18 @@ __device__ __forceinline__ void load_w(const ConvArgs& p, int d, float (&w)[W][V
     }
 }
 
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool WIDE>
 __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
     int d = (blockIdx.x * cg.L + threadIdx.x % cg.L) * V, run = blockIdx.z * (256 / cg.L) + threadIdx.x / cg.L;
     const bool ok = d < p.D && run < cg.n_seg;                                 // idle lanes walk channel 0 or run 0 and write nothing
     if (d >= p.D) d = 0;
     if (run >= cg.n_seg) run = 0;                                              // (a whole wave's, where it has one run)
+    run = uniform<WIDE>(run);
     const int b = blockIdx.y, ta = run * cg.seg;
     const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), stop = min(tb, end);
     float w[W][V], bias[V], xw[W][V];
     bool live[W];
+    const bool silu = p.silu != 0;
     T* y = (T*)p.y + b * p.y_b + d;
     const auto put_state = [&] {
 #pragma unroll
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
     };
     if (ta <= end) {
         load_w<V, W>(p, d, w, bias);
-        window<T, V, W>(p, b, ta, d, xw, live);
+        window<T, V, W, WIDE>(p, b, ta, d, xw, live);
         if (ta == 0 && end == 0 && p.state_out && ok) put_state();             // an empty row passes its state on
     }
     const T* x = (const T*)p.x + b * p.x_b + d;
@@ -127,27 +134,31 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
         float in[FB][V];
 #pragma unroll
         for (int q = 0; q < FB; ++q) cload<T, V>(x + min(t0 + q, stop - 1) * p.x_t, in[q]);      // beyond the run: read again, not used
-        const unsigned rm = reset_bits<FB>(p, cg.L, b, t0, stop);
+        const unsigned rm = reset_bits<FB, WIDE>(p, b, t0, stop);
+        // a whole batch without a reset is straight code, in which the window moves by renaming
+        const auto steps = [&](auto plain) {
 #pragma unroll
-        for (int q = 0; q < FB; ++q) {
-            if (t0 + q >= stop) break;
-            if (rm >> q & 1) {
+            for (int q = 0; q < FB; ++q) {
+                if (!plain && t0 + q >= stop) break;
+                if (!plain && (rm >> q & 1)) {
 #pragma unroll
-                for (int k = 0; k < W - 1; ++k) czero(xw[k]);
+                    for (int k = 0; k < W - 1; ++k) czero(xw[k]);
+                }
+                float v[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    xw[W - 1][i] = in[q][i];
+                    v[i] = bias[i];
+#pragma unroll
+                    for (int k = 0; k < W; ++k) v[i] = fmaf(w[k][i], xw[k][i], v[i]);
+                    if (silu) v[i] *= sigmoidf(v[i]);
+#pragma unroll
+                    for (int k = 0; k < W - 1; ++k) xw[k][i] = xw[k + 1][i];
+                }
+                if (ok) cstore<T, V>(y + (t0 + q) * p.y_t, v);
             }
-            float v[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                xw[W - 1][i] = in[q][i];
-                v[i] = bias[i];
-#pragma unroll
-                for (int k = 0; k < W; ++k) v[i] = fmaf(w[k][i], xw[k][i], v[i]);
-                if (p.silu) v[i] *= sigmoidf(v[i]);
-#pragma unroll
-                for (int k = 0; k < W - 1; ++k) xw[k][i] = xw[k + 1][i];
-            }
-            if (ok) cstore<T, V>(y + (t0 + q) * p.y_t, v);
-        }
+        };
+        if (__all(rm == 0 && t0 + FB <= stop)) steps(std::true_type{}); else steps(std::false_type{});
     }
     if (!ok) return;
     if (stop == end && stop > ta && p.state_out) put_state();                  // the row's last step was this run's
@@ -159,7 +170,7 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
 // dx[tau] collects w[k] dpre[tau + W - 1 - k]: one walk forward in time with W open sums. A run emits its steps ta .. tb - 1
 // and goes W - 1 steps further for them; dw and db count its own steps only and stay in registers over all the runs that a
 // thread takes (every cg.rows-th).
-template <typename T, int V, int W>
+template <typename T, int V, int W, bool WIDE>
 __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
     __shared__ float acc[W + 1][256 * V];
     const int lx = threadIdx.x % cg.L, ly = threadIdx.x / cg.L, per = 256 / cg.L;
@@ -170,15 +181,16 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
 #pragma unroll
     for (int k = 0; k < W; ++k) czero(dw[k]);
     czero(db);
+    const bool silu = p.silu != 0;
     const long long n_runs = (long long)cg.n_seg * p.B;
     for (long long r = (long long)blockIdx.y * per + ly; r < n_runs; r += (long long)cg.rows * per) {
-        const int run = (int)(r / p.B), b = (int)(r - run * p.B), ta = run * cg.seg;
+        const int run = uniform<WIDE>((int)(r / p.B)), b = uniform<WIDE>((int)(r - run * p.B)), ta = run * cg.seg;
         const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), last = tb + W - 1, stop = min(last, end);
         float xw[W][V], open[W][V];
         bool live[W];
 #pragma unroll
         for (int k = 0; k < W; ++k) { czero(open[k]); czero(xw[k]); live[k] = true; }
-        if (ta < end) window<T, V, W>(p, b, ta, d, xw, live);
+        if (ta < end) window<T, V, W, WIDE>(p, b, ta, d, xw, live);
         const T *x = (const T*)p.x + b * p.x_b + d, *dy = (const T*)p.dy + b * p.dy_b + d;
         T* dx = (T*)p.dx + b * p.dx_b + d;
         // tau = t - W + 1 is complete once step t is through: no later step reaches back to it
@@ -205,34 +217,41 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
                 cload<T, V>(x + t * p.x_t, in[q]);
                 cload<T, V>(dy + t * p.dy_t, gy[q]);
             }
-            const unsigned rm = reset_bits<BB>(p, cg.L, b, t0, stop);
+            const unsigned rm = reset_bits<BB, WIDE>(p, b, t0, stop);
+            // a whole batch of the run's own steps in one episode is straight code, see k_conv_fwd
+            const auto steps = [&](auto plain) {
 #pragma unroll
-            for (int q = 0; q < BB; ++q) {
-                const int t = t0 + q;
-                if (t >= stop) break;
-                if (rm >> q & 1) {
+                for (int q = 0; q < BB; ++q) {
+                    const int t = t0 + q;
+                    if (!plain && t >= stop) break;
+                    if (!plain && (rm >> q & 1)) {
 #pragma unroll
-                    for (int k = 0; k < W - 1; ++k) { czero(xw[k]); live[k] = false; }
-                }
-                live[W - 1] = true;
-                const bool mine = t < tb;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    xw[W - 1][i] = in[q][i];
-                    float v = bias[i], g = gy[q][i];
-#pragma unroll
-                    for (int k = 0; k < W; ++k) v = fmaf(w[k][i], xw[k][i], v);
-                    if (p.silu) { const float s = sigmoidf(v); g *= s * fmaf(v, 1.f - s, 1.f); }
-#pragma unroll
-                    for (int k = 0; k < W; ++k) open[k][i] = live[k] ? fmaf(w[k][i], g, open[k][i]) : open[k][i];
-                    if (mine) {
-                        db[i] += g;
-#pragma unroll
-                        for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, xw[k][i], dw[k][i]);
+                        for (int k = 0; k < W - 1; ++k) { czero(xw[k]); live[k] = false; }
                     }
+                    live[W - 1] = true;
+                    const bool mine = plain || t < tb;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        xw[W - 1][i] = in[q][i];
+                        float v = bias[i], g = gy[q][i];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) v = fmaf(w[k][i], xw[k][i], v);
+                        if (silu) { const float s = sigmoidf(v); g *= s * fmaf(v, 1.f - s, 1.f); }
+#pragma unroll
+                        for (int k = 0; k < W; ++k) open[k][i] = plain || live[k] ? fmaf(w[k][i], g, open[k][i]) : open[k][i];
+                        if (mine) {
+                            db[i] += g;
+#pragma unroll
+                            for (int k = 0; k < W; ++k) dw[k][i] = fmaf(g, xw[k][i], dw[k][i]);
+                        }
+                    }
+                    emit(t);
                 }
-                emit(t);
-            }
+            };
+            bool whole = rm == 0 && t0 + BB <= min(stop, tb);
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) whole = whole && live[k];
+            if (__all(whole)) steps(std::true_type{}); else steps(std::false_type{});
         }
         for (int t = max(ta, stop); t < last; ++t) {
             if (t == end && p.dstate_out) {           // the state the row left = its last W - 1 inputs: their gradient comes in here
@@ -356,15 +375,25 @@ static bool conv_vec(const ConvArgs& p, long long e, bool bwd) {
     return p.D % 4 == 0 && (m & (4 * e - 1)) == 0;
 }
 
-#define CONV_W(NAME, T, V, GRID, ...)                                          \
-    switch (p.W) {                                                              \
-        case 2: NAME<T, V, 2><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;         \
-        case 3: NAME<T, V, 3><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;         \
-        default: NAME<T, V, 4><<<GRID, 256, 0, s>>>(__VA_ARGS__); break;        \
+template <typename T, int V, int W, bool WIDE>
+static void launch_conv(const ConvArgs& p, const ConvGrid& cg, bool bwd, dim3 grid, hipStream_t s) {
+    if (bwd) k_conv_bwd<T, V, W, WIDE><<<grid, 256, 0, s>>>(p, cg);
+    else k_conv_fwd<T, V, W, WIDE><<<grid, 256, 0, s>>>(p, cg);
+}
+template <typename T, int V, int W>
+static void launch_conv_step(const ConvArgs& p, dim3 grid, hipStream_t s) { k_conv_step<T, V, W><<<grid, 256, 0, s>>>(p); }
+// F<T, V, W>(...) for the call's type, alignment and taps
+#define CONV_W(F, T, V, ...)                                           \
+    switch (p.W) {                                                      \
+        case 2: F(T, V, 2, __VA_ARGS__); break;                         \
+        case 3: F(T, V, 3, __VA_ARGS__); break;                         \
+        default: F(T, V, 4, __VA_ARGS__); break;                        \
     }
-#define CONV_ALL(NAME, GRID, ...)                                                                                       \
-    if (bf16) { if (vec) { CONV_W(NAME, bf16_t, 4, GRID, __VA_ARGS__) } else { CONV_W(NAME, bf16_t, 1, GRID, __VA_ARGS__) } }    \
-    else { if (vec) { CONV_W(NAME, float, 4, GRID, __VA_ARGS__) } else { CONV_W(NAME, float, 1, GRID, __VA_ARGS__) } }
+#define CONV_ALL(F, ...)                                                                                            \
+    if (bf16) { if (vec) { CONV_W(F, bf16_t, 4, __VA_ARGS__) } else { CONV_W(F, bf16_t, 1, __VA_ARGS__) } }         \
+    else { if (vec) { CONV_W(F, float, 4, __VA_ARGS__) } else { CONV_W(F, float, 1, __VA_ARGS__) } }
+#define CONV_SEQ(T, V, W, BWD) cg.L >= 64 ? launch_conv<T, V, W, true>(p, cg, BWD, grid, s) : launch_conv<T, V, W, false>(p, cg, BWD, grid, s)
+#define CONV_ONE(T, V, W, _) launch_conv_step<T, V, W>(p, grid, s)
 
 DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
@@ -374,7 +403,7 @@ DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const long long cv = vec ? p.D / 4 : p.D, per = 256 / cg.L;
     if ((cg.n_seg + per - 1) / per > 65535) return -1;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)p.B, (unsigned)((cg.n_seg + per - 1) / per));
-    CONV_ALL(k_conv_fwd, grid, p, cg)
+    CONV_ALL(CONV_SEQ, false)
     return (int)hipGetLastError();
 }
 
@@ -387,7 +416,7 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec, (int)p.W - 1);
     const long long cv = vec ? p.D / 4 : p.D, n = (p.W + 1) * p.D;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)cg.rows);
-    CONV_ALL(k_conv_bwd, grid, p, cg)
+    CONV_ALL(CONV_SEQ, true)
     k_conv_sum<<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(p.ws, cg.rows, (int)p.W, p.D, p.dw, p.db);
     return (int)hipGetLastError();
 }
@@ -399,6 +428,6 @@ DRL_API int drl_short_conv_step(const ConvArgs* a, int bf16, hipStream_t s) {
     const long long nb = (p.B * p.D / (vec ? 4 : 1) + 255) / 256;
     if (nb > 0x7fffffffll) return -1;
     const dim3 grid((unsigned)nb);
-    CONV_ALL(k_conv_step, grid, p)
+    CONV_ALL(CONV_ONE, 0)
     return (int)hipGetLastError();
 }
