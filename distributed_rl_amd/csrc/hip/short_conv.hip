@@ -9,7 +9,7 @@
 #include "ssm_math.h"
 #include <type_traits>
 
-#define FB 16            // steps read ahead by the forward
+#define FB 8             // steps read ahead by the forward
 #define BB 6             // and by the backward (two tensors)
 
 struct ConvArgs {        // mirrored by ops/hip.py (_conv_args): 64-bit words in this order
@@ -182,9 +182,9 @@ __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
     for (int k = 0; k < W; ++k) czero(dw[k]);
     czero(db);
     const bool silu = p.silu != 0;
-    const long long n_runs = (long long)cg.n_seg * p.B;
-    for (long long r = (long long)blockIdx.y * per + ly; r < n_runs; r += (long long)cg.rows * per) {
-        const int run = uniform<WIDE>((int)(r / p.B)), b = uniform<WIDE>((int)(r - run * p.B)), ta = run * cg.seg;
+    const unsigned B = (unsigned)p.B, n_runs = (unsigned)cg.n_seg * B;      // T B <= 2^31
+    for (unsigned r = blockIdx.y * per + ly; r < n_runs; r += cg.rows * per) {
+        const int run = uniform<WIDE>((int)(r / B)), b = uniform<WIDE>((int)(r % B)), ta = run * cg.seg;
         const int end = row_end(p, b), tb = min(ta + cg.seg, (int)p.T), last = tb + W - 1, stop = min(last, end);
         float xw[W][V], open[W][V];
         bool live[W];
@@ -339,19 +339,21 @@ __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
 }
 
 static bool conv_ok(long long T, long long B, long long D, long long W) {
-    return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && D > 0 && D < (1ll << 29) && W >= 2 && W <= 4;
+    return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && T * B <= (1ll << 31) && D > 0 && D < (1ll << 29) && W >= 2 && W <= 4;
 }
 
-// Runs of 16 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves. The backward
-// walks W - 1 steps more than a run has: its runs are that much short of 18, 36 or 60. vec: V > 1.
+// Runs of 8 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves: 120 x 64 x
+// 1 024 bf16 forward 11.3 us in runs of 8, 12.8 in runs of 16, 14.6 of 32. The backward walks W - 1 steps more than a run has:
+// its runs are that much short of 12 (below 1 024 waves: 30 x 64 x 256 11.8 us against 13.8), 18 (the above: 22.6 us against 30.2
+// with 12, whose partial rows are twice as many), 36 or 60. vec: V > 1.
 static ConvGrid conv_grid(long long T, long long B, long long D, bool vec, int extra) {
     const long long cv = vec ? D / 4 : D;
     int L = 1;
     while (L < cv && L < 256) L *= 2;
     const long long waves = (cv + L - 1) / L * L * B / 64;                    // of one run a row
-    const int choice[2][3] = {{16, 32, 64}, {18 - extra, 36 - extra, 60 - extra}};
+    const int choice[2][4] = {{8, 16, 32, 64}, {12 - extra, 18 - extra, 36 - extra, 60 - extra}};
     int k = 0;
-    while (k < 2 && waves * ((T + choice[extra > 0][k + 1] - 1) / choice[extra > 0][k + 1]) >= 4096) ++k;
+    while (k < 3 && waves * ((T + choice[extra > 0][k + 1] - 1) / choice[extra > 0][k + 1]) >= (extra && k == 0 ? 1024 : 4096)) ++k;
     const int seg = choice[extra > 0][k];
     const long long n_seg = (T + seg - 1) / seg, blocks = (n_seg * B + 256 / L - 1) / (256 / L), cols = (cv + L - 1) / L;
     long long rows = (1024 + cols - 1) / cols;

@@ -1178,7 +1178,8 @@ def short_conv_ws(T: int, B: int, D: int, W: int, device) -> torch.Tensor:
 def _conv_args(x, w, bias, silu, reset, lengths, y=None, state_in=None, state_out=None, dy=None, dx=None, dw=None, db=None, ws=None,
                dstate_in=None, dstate_out=None):
     shape, W = x.shape, w.shape[-1]
-    if len(shape) != 3 or not 0 < shape[0] <= 1000000 or not 0 < shape[1] <= 65535 or shape[2] < 1 or not 2 <= W <= 4:
+    if len(shape) != 3 or not 0 < shape[0] <= 1000000 or not 0 < shape[1] <= 65535 or shape[2] < 1 or not 2 <= W <= 4 \
+            or shape[0] * shape[1] > 1 << 31:
         raise ValueError("short_conv: unsupported sizes %s with %d taps" % (tuple(shape), W))
     T, B, D = shape
     dev, typ, f32 = _dev(x), x.dtype, torch.float32
