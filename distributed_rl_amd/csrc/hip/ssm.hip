@@ -10,7 +10,8 @@
 #include "ssm_math.h"
 #include <type_traits>
 
-#define KC 16            // steps per chunk = distance of the saved states
+#define KC 16            // steps per chunk
+#define SAVE 8           // distance of the states that the forward saves for the backward (ops/hip.py SSM_SAVE)
 
 struct SsmArgs {         // mirrored by ops/hip.py (_ssm_args): 64-bit words in this order
     const void *u, *dt, *z, *Bm, *Cm;
@@ -378,7 +379,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     for (int i = 0; i < NS; ++i) A2[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
     const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.y_t, g, d);
-    const bool has_z = p.z != nullptr, soft = p.softplus != 0;
+    const bool has_z = p.z != nullptr, soft = p.softplus != 0, ck4 = vec4(p.ckpt, p.N);
     unsigned ru[4], rd[4], rz[4], rr;
     R xu(p.u, p.u_t, p.u_b, b, ta), xd(p.dt, p.dt_t, p.dt_b, b, ta), xz(p.z, p.z_t, p.z_b, b, ta), xy(p.y, p.y_t, p.y_b, b, ta);
     StageBC<T, NS, 3> st(p, b, ta);
@@ -418,11 +419,12 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
         const unsigned rm = reset_mask(rr);
         if (t0 + KC < live) fetch(t0 + KC);
         block_sync_lds();                 // B and C of this chunk are there; the image of the chunk before last is free again
-        if (p.ckpt && dv) put_states<NS>(p.ckpt + (t0 / KC) * BDN + so, h, g * NS, p.N, vec4(p.ckpt, p.N));
         float y[4];
         auto steps = [&](auto has) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
+                if (4 * q % SAVE == 0 && p.ckpt && dv && t0 + 4 * q < p.T)
+                    put_states<NS>(p.ckpt + (t0 / SAVE + 4 * q / SAVE) * BDN + so, h, g * NS, p.N, ck4);
                 float part[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
@@ -510,7 +512,7 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
     for (int k = KH - 2; k >= 0; k -= 2) {          // two steps at a time: k + 1, then k
         float vB[2][NS], vC[2][NS];
         __builtin_amdgcn_sched_barrier(0);
-        if (k == KH / 2 - 2 || (KH == 4 && k == 0)) mid();
+        if (k == (KH == 4 ? 0 : KH / 2 - 2)) mid();
         In nx[2];
         if (k >= 2) { nx[1] = load(s0 + k - 1, again); nx[0] = load(s0 + k - 2, again); }
 #pragma unroll
@@ -551,13 +553,12 @@ template <typename T, int NS, bool HAS>
 __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
                                                     float* __restrict__ part_bc, float* __restrict__ part_a) {
     constexpr int NP = 4 * NS;
-    constexpr int KH = NS > 4 ? 4 : NS == 4 ? 8 : KC;                   // steps whose states are held at a time
+    constexpr int KH = NS > 4 ? 4 : 8;                      // steps whose states are held at a time
     using R = Rows<T>;
     __shared__ __align__(16) float4 pw_s[4][KC][16];        // s log2(e), s u, ds, u
     __shared__ __align__(16) float4 ex_s[4][KC][16];        // dy silu'(z), -, ds/d(pre), sum_n C h
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
-    __shared__ float mid_s[KH < KC ? 4 : 1][KH < KC ? KC / KH - 1 : 1][KH < KC ? NS : 1][64];      // states before each piece
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
     static_assert(sizeof(bc_s) > SORT_ROWS * sizeof(int), "block_row");
     const int b = block_row(p, (int*)bc_s);
@@ -580,12 +581,12 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.dy_t, g, d);
     const unsigned odu = R::offset(p.du_t, g, d), odd = R::offset(p.ddt_t, g, d), odz = R::offset(p.dz_t, g, d);
     unsigned ru[4], rd[4], rz[4], ry[4], rr;
-    float hc[NS];
+    float hc0[NS], hc1[NS];                                 // the saved states before steps 0 and 8 of the chunk
     const int live = min(tb, end), t_last = ta + max(live - ta - 1, 0) / KC * KC;       // padding is not walked, see below
     R xu(p.u, p.u_t, p.u_b, b, t_last), xd(p.dt, p.dt_t, p.dt_b, b, t_last), xz(p.z, p.z_t, p.z_b, b, t_last), xy(p.dy, p.dy_t, p.dy_b, b, t_last);
     R wu(p.du, p.du_t, p.du_b, b, t_last), wd(p.ddt, p.ddt_t, p.ddt_b, b, t_last), wz(p.dz, p.dz_t, p.dz_b, b, t_last);
     StageBC<T, NS, 3> st(p, b, t_last);
-    const float* ck = p.ckpt + t_last / KC * BDN;
+    const float* ck = p.ckpt + t_last / SAVE * BDN;
     const bool ck4 = vec4(p.ckpt, p.N);
     auto fetch = [&](int t0) {
 #pragma unroll
@@ -598,8 +599,9 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
         }
         st.fetch(end - t0);
         if (HAS) rr = fetch_resets(p, b, t0, end, lane);
-        get_states<NS>(ck + so, hc, g * NS, p.N, dv, ck4);
-        xu.back(); xd.back(); xz.back(); xy.back(); st.B.back(); st.C.back(); ck -= BDN;
+        get_states<NS>(ck + so, hc0, g * NS, p.N, dv, ck4);
+        get_states<NS>(ck + BDN + so, hc1, g * NS, p.N, dv && t0 + SAVE < live, ck4);
+        xu.back(); xd.back(); xz.back(); xy.back(); st.B.back(); st.C.back(); ck -= 2 * BDN;
     };
     // sums of the block's four waves over a finished chunk's dB, dC
     const long long prow = p.B * gridDim.x * 2 * NP;        // partials of a step
@@ -653,9 +655,9 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
         float* bcb = bc_s[c & 1];
         st.put(bcb);
         const unsigned rm = HAS ? reset_mask(rr) : 0;
-        float hs[KH + 1][NS];
+        float hs[KH + 1][NS], h0[NS];
 #pragma unroll
-        for (int i = 0; i < NS; ++i) hs[0][i] = HAS && (rm & 1) ? 0.f : hc[i];
+        for (int i = 0; i < NS; ++i) h0[i] = HAS && (rm & 1) ? 0.f : hc0[i];
         auto next = [&] {
             asm volatile("" ::: "memory");                  // not earlier
             if (t0 > ta) fetch(t0 - KC);
@@ -677,30 +679,33 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
             R::store(wd.rsrc(), odd | bad, (unsigned)(s / 4) * wd.four, dpre);
             if (has_z) R::store(wz.rsrc(), odz | bad, (unsigned)(s / 4) * wz.four, t < end ? ex.x * fmaf(Dd, pw.w, ex.w) : 0.f);
         };
-        if constexpr (KH == KC) {
-            bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, 0, g, j, An, hs, G, dAc, ex_s[w], next, emit);
-        } else {
-#pragma unroll 1
-            for (int s = 0; s < KC - KH; ++s) {             // the states before each piece
-                if (s % KH == 0) {
+        auto from = [&](const float (&h)[NS]) {
 #pragma unroll
-                    for (int i = 0; i < NS; ++i) mid_s[w][s / KH][i][lane] = hs[0][i];
+            for (int i = 0; i < NS; ++i) hs[0][i] = h[i];
+        };
+        auto piece = [&](int s0, auto mid) { bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], mid, emit); };
+        auto nothing = [] {};
+        if constexpr (KH == SAVE) {
+            from(hc1);
+            piece(SAVE, nothing);
+            from(h0);
+            piece(0, next);
+        } else {                                            // two pieces from each saved state: its steps are run up to the second
+            auto run = [&](int s0) {
+#pragma unroll
+                for (int s = s0; s < s0 + KH; ++s) {
+                    const float4 pw = pw_s[w][s][j];
+                    float Bv[NS];
+                    lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
+                    const bool rs = HAS && (rm >> s & 1);
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * An[i]), rs ? 0.f : hs[0][i], pw.y * Bv[i]);
                 }
-                const float4 pw = pw_s[w][s][j];
-                float Bv[NS];
-                lds_row<NS>(bcb + s * 2 * NP + g * NS, Bv);
-                const bool rs = HAS && (rm >> s & 1);
-#pragma unroll
-                for (int i = 0; i < NS; ++i) hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * An[i]), rs ? 0.f : hs[0][i], pw.y * Bv[i]);
-            }
-#pragma unroll 1
-            for (int s0 = KC - KH; s0 >= 0; s0 -= KH) {
-                bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], [&] { if (!s0) next(); }, emit);
-                if (s0) {
-#pragma unroll
-                    for (int i = 0; i < NS; ++i) hs[0][i] = mid_s[w][s0 / KH - 1][i][lane];
-                }
-            }
+            };
+            from(hc1); run(SAVE); piece(SAVE + KH, nothing);
+            from(hc1); piece(SAVE, nothing);
+            from(h0); run(0); piece(KH, nothing);
+            from(h0); piece(0, next);
         }
 #pragma unroll
         for (int i = 0; i < NS; ++i) dA[i] += dAc[i];

@@ -1237,7 +1237,7 @@ def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None
     _run(native.hip().drl_short_conv_step, _CONV_STEP.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0), bf16, dev)
 
 
-SSM_CHUNK = 16              # steps between the states that ssm_scan_fwd saves for ssm_scan_bwd
+SSM_SAVE = 8                # steps between the states that ssm_scan_fwd saves for ssm_scan_bwd
 
 
 def ssm_scan_ws(T: int, B: int, D: int, N: int, device, train: bool = True) -> torch.Tensor:
@@ -1248,8 +1248,8 @@ def ssm_scan_ws(T: int, B: int, D: int, N: int, device, train: bool = True) -> t
 
 
 def ssm_scan_ckpt(T: int, B: int, D: int, N: int, device) -> torch.Tensor:
-    """The states that :func:`ssm_scan_fwd` keeps for :func:`ssm_scan_bwd`: one per 16 steps, fp32."""
-    return torch.empty((T + SSM_CHUNK - 1) // SSM_CHUNK, B, D, N, device=device)
+    """The states that :func:`ssm_scan_fwd` keeps for :func:`ssm_scan_bwd`: one per 8 steps, fp32."""
+    return torch.empty((T + SSM_SAVE - 1) // SSM_SAVE, B, D, N, device=device)
 
 
 def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None, ws=None, h0=None, hT=None, ckpt=None, dy=None, dhT=None,
@@ -1271,7 +1271,7 @@ def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None,
     Dp, bp, dDp, dbp = (_opt(t, (Dc,), f32, dev, n) for t, n in ((D, "D"), (dt_bias, "dt_bias"), (dD, "dD"), (ddt_bias, "ddt_bias")))
     h0p, hTp, dhTp, dh0p = (_opt(t, st, f32, dev, n) for t, n in ((h0, "h0"), (hT, "hT"), (dhT, "dhT"), (dh0, "dh0")))
     rp, lp = _opt(reset, (T, B), torch.uint8, dev, "reset"), _opt(lengths, (B,), torch.int32, dev, "lengths")
-    ck = _opt(ckpt, ((T + SSM_CHUNK - 1) // SSM_CHUNK, B, Dc, N), f32, dev, "ckpt")
+    ck = _opt(ckpt, ((T + SSM_SAVE - 1) // SSM_SAVE, B, Dc, N), f32, dev, "ckpt")
     n_ws = ws.numel()
     wsp = _vec(ws, (n_ws,), f32, dev, "ws")
     if T > 1 and max(ur[1], dtr[1], zr[1], Br[1], Cr[1], yr[1], dyr[1], dur[1], ddtr[1], dzr[1]) >= 1 << 25:
