@@ -385,6 +385,18 @@ def test_norm_past_32_bits():
     assert torch.equal(y[-3:], dx)
 
 
+def test_norm_of_more_rows_than_a_launch_takes():
+    M, D = (1 << 21) * 64 + 5, 4
+    x = torch.empty(M, D, dtype=BF, device=DEV)
+    x.random_(-8, 9)
+    y, w, mean, rstd = torch.empty_like(x), torch.ones(D, device=DEV), torch.empty(M, device=DEV), torch.empty(M, device=DEV)
+    H.layer_norm_fwd(x, w, None, y, mean=mean, rstd=rstd)
+    for cut in (slice(0, 7), slice(M - 9, M)):
+        part = [torch.empty_like(x[cut]), torch.empty_like(mean[cut]), torch.empty_like(mean[cut])]
+        H.layer_norm_fwd(x[cut], w, None, part[0], mean=part[1], rstd=part[2])
+        assert torch.equal(y[cut], part[0]) and torch.equal(mean[cut], part[1]) and torch.equal(rstd[cut], part[2])
+
+
 def test_conv_and_scan_past_32_bits():
     T, B, D, N = 2100, 1024, 1024, 2                        # 2.2e9 elements a tensor
     g = Gen(0)
