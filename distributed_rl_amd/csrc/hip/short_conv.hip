@@ -12,7 +12,7 @@
 #define FB 8             // steps read ahead by the forward
 #define BB 6             // and by the backward (two tensors)
 
-struct ConvArgs {        // mirrored by ops/hip.py (_conv_args): 64-bit words in this order
+struct ConvArgs {        // mirrored by ops/hip.py (_CONV): 64-bit words in this order
     const void *x, *state_in;
     long long x_t, x_b;
     const float *w, *bias;
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(1024) void k_conv_sum(const float* __restrict__ par
 // One step. A thread per V channels of a row.
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * V;
+    const long long i = (((long long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x) * V;
     if (i >= p.B * p.D) return;
     const long long b = i / p.D, d = i - b * p.D;
     T* s = (T*)p.state_out + b * (W - 1) * p.D + d;
@@ -339,7 +339,7 @@ __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
 }
 
 static bool conv_ok(long long T, long long B, long long D, long long W) {
-    return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && T * B <= (1ll << 31) && D > 0 && D < (1ll << 29) && W >= 2 && W <= 4;
+    return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && T * B <= (1ll << 31) && D > 0 && D <= (1ll << 22) && W >= 2 && W <= 4;
 }
 
 // Runs of 8 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves: 120 x 64 x
@@ -428,8 +428,9 @@ DRL_API int drl_short_conv_step(const ConvArgs* a, int bf16, hipStream_t s) {
     if (!conv_ok(1, 1, p.D, p.W) || p.B <= 0) return -1;
     const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
     const long long nb = (p.B * p.D / (vec ? 4 : 1) + 255) / 256;
-    if (nb > 0x7fffffffll) return -1;
-    const dim3 grid((unsigned)nb);
+    if (nb >= 1ll << 38) return -1;
+    const long long x = nb < (1 << 23) ? nb : 1 << 23;
+    const dim3 grid((unsigned)x, (unsigned)((nb + x - 1) / x));
     CONV_ALL(CONV_ONE, 0)
     return (int)hipGetLastError();
 }

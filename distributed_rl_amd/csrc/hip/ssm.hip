@@ -13,7 +13,7 @@
 #define KC 16            // steps per chunk
 #define SAVE 8           // distance of the states that the forward saves for the backward (ops/hip.py SSM_SAVE)
 
-struct SsmArgs {         // mirrored by ops/hip.py (_ssm_args): 64-bit words in this order
+struct SsmArgs {         // mirrored by ops/hip.py (_SSM): 64-bit words in this order
     const void *u, *dt, *z, *Bm, *Cm;
     long long u_t, u_b, dt_t, dt_b, z_t, z_b, B_t, B_b, C_t, C_b;
     const float *A, *Dp, *bias, *h0;
@@ -736,19 +736,20 @@ template <typename T>
 __global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __restrict__ part_bc, int nblk, int NP, unsigned n_bc,
                                                     const float* __restrict__ part_a, int rows) {
     if (blockIdx.x < n_bc) {
-        const long long i = (long long)blockIdx.x * 256 + threadIdx.x, row = i / (2 * p.N);
-        if (row >= p.T * p.B) return;
-        const int c = (int)(i - row * 2 * p.N), isC = c >= p.N, n = isC ? c - (int)p.N : c;
-        const float* q = part_bc + row * nblk * 2 * NP + isC * NP + n;
-        const long long t = row / p.B, b = row - t * p.B;
-        float v = 0.f;
-        if (t < row_end(p, (int)b)) {                       // padding has no partials
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x;; i += (long long)n_bc * 256) {
+            const long long row = i / (2 * p.N);
+            if (row >= p.T * p.B) return;
+            const int c = (int)(i - row * 2 * p.N), isC = c >= p.N, n = isC ? c - (int)p.N : c;
+            const float* q = part_bc + row * nblk * 2 * NP + isC * NP + n;
+            const long long t = row / p.B, b = row - t * p.B;
+            float v = 0.f;
+            if (t < row_end(p, (int)b)) {                   // padding has no partials
 #pragma unroll 4
-            for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
+                for (int k = 0; k < nblk; ++k) v += q[(long long)k * 2 * NP];
+            }
+            if (isC) st((T*)p.dCm + t * p.dC_t + b * p.dC_b + n, v);
+            else st((T*)p.dBm + t * p.dB_t + b * p.dB_b + n, v);
         }
-        if (isC) st((T*)p.dCm + t * p.dC_t + b * p.dC_b + n, v);
-        else st((T*)p.dBm + t * p.dB_t + b * p.dB_b + n, v);
-        return;
     }
     __shared__ float acc[8][33];
     const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
@@ -776,8 +777,8 @@ __global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __re
 template <typename T, int V, int L, int R>
 __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
     const int lane = threadIdx.x % L, n0 = lane * V, N = (int)p.N, D = (int)p.D;
-    const long long total = p.B * p.D, step = (long long)gridDim.x * (256 / L);
-    const long long i0 = (long long)blockIdx.x * (256 / L) + threadIdx.x / L;
+    const long long total = p.B * p.D, step = (long long)gridDim.x * gridDim.y * (256 / L);
+    const long long i0 = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (256 / L) + threadIdx.x / L;
     float h[R][V], A[R][V], Bv[R][V], Cv[R][V], u[R], dt[R], z[R], Dd[R];
     bool rs[R];
 #pragma unroll
@@ -850,11 +851,21 @@ static Segs segments(long long T, long long B, long long D) {
 
 // floats of scratch that a forward (train = 0) or a forward and its backward (1) need
 DRL_API int drl_ssm_ws(long long T, long long B, long long D, long long N, int train, long long* n) {
-    if (T <= 0 || T >= (1ll << 31) || B <= 0 || D <= 0 || D >= (1ll << 25) || N <= 0 || N > 64 || B > 65535 || T * B > (1ll << 31)) return -1;
+    if (T <= 0 || T > (1ll << 30) || B <= 0 || D <= 0 || D > (1ll << 22) || N <= 0 || N > 64 || B > 65535 || T * B > (1ll << 31)) return -1;
     const long long nblk = (D + 63) / 64, S = segments(T, B, D).n;
     *n = S > 1 ? S * B * D * (N + 1) : 0;
     if (train) *n += T * B * nblk * 8 * ns_of(N) + S * B * D * (N + 2);
     return 0;
+}
+
+// Offsets inside a chunk are 32-bit: 16 steps of any tensor lie under 2^31 bytes. The stride of a single step says nothing and
+// may be anything; it becomes 0.
+static bool steps_ok(SsmArgs& p) {
+    for (long long* q : {&p.u_t, &p.dt_t, &p.z_t, &p.B_t, &p.C_t, &p.y_t, &p.dy_t, &p.du_t, &p.ddt_t, &p.dz_t}) {
+        if (p.T == 1) *q = 0;
+        else if (*q < 0 || *q >= (1ll << 25)) return false;
+    }
+    return true;
 }
 
 template <typename T, int NS, bool BWD>
@@ -884,7 +895,8 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
     const dim3 grid((unsigned)nblk, (unsigned)p.B, (unsigned)sg.n);
     if (p.reset) k_ssm_bwd<T, NS, true><<<grid, 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
     else k_ssm_bwd<T, NS, false><<<grid, 256, 0, s>>>(p, sg.len, carry, part_bc, part_a);
-    const unsigned n_bc = (unsigned)((p.T * p.B * 2 * p.N + 255) / 256), n_a = (unsigned)((p.D * (p.N + 2) + 31) / 32);
+    const long long n = (p.T * p.B * 2 * p.N + 255) / 256;
+    const unsigned n_bc = (unsigned)(n < (1 << 22) ? n : 1 << 22), n_a = (unsigned)((p.D * (p.N + 2) + 31) / 32);
     k_ssm_finish<T><<<n_bc + n_a, 256, 0, s>>>(p, part_bc, nblk, NP, n_bc, part_a, (int)rows);
 }
 
@@ -898,18 +910,18 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
     }
 
 DRL_API int drl_ssm_fwd(const SsmArgs* a, int bf16, hipStream_t s) {
-    const SsmArgs p = *a;
+    SsmArgs p = *a;
     long long need;
-    if (drl_ssm_ws(p.T, p.B, p.D, p.N, 0, &need)) return -1;
+    if (drl_ssm_ws(p.T, p.B, p.D, p.N, 0, &need) || !steps_ok(p)) return -1;
     if (p.ws_n < need) return -2;
     if (bf16) { SSM_NS(launch_fwd, bf16_t) } else { SSM_NS(launch_fwd, float) }
     return (int)hipGetLastError();
 }
 
 DRL_API int drl_ssm_bwd(const SsmArgs* a, int bf16, hipStream_t s) {
-    const SsmArgs p = *a;
+    SsmArgs p = *a;
     long long need;
-    if (drl_ssm_ws(p.T, p.B, p.D, p.N, 1, &need) || !p.ckpt) return -1;
+    if (drl_ssm_ws(p.T, p.B, p.D, p.N, 1, &need) || !p.ckpt || !steps_ok(p)) return -1;
     if (p.ws_n < need) return -2;
     if (bf16) { SSM_NS(launch_bwd, bf16_t) } else { SSM_NS(launch_bwd, float) }
     return (int)hipGetLastError();
@@ -917,8 +929,8 @@ DRL_API int drl_ssm_bwd(const SsmArgs* a, int bf16, hipStream_t s) {
 
 template <typename T, int V, int L>
 static void launch_step(const SsmArgs& p, hipStream_t s) {
-    const long long ch = p.B * p.D, nb = (ch + 256 / L - 1) / (256 / L);
-    if (nb >= 8192) k_ssm_step<T, V, L, 4><<<(unsigned)((nb + 3) / 4), 256, 0, s>>>(p);
+    const long long ch = p.B * p.D, nb = (ch + 256 / L - 1) / (256 / L), n4 = (nb + 3) / 4, x = n4 < (1 << 23) ? n4 : 1 << 23;
+    if (nb >= 8192) k_ssm_step<T, V, L, 4><<<dim3((unsigned)x, (unsigned)((n4 + x - 1) / x)), 256, 0, s>>>(p);
     else k_ssm_step<T, V, L, 1><<<(unsigned)nb, 256, 0, s>>>(p);
 }
 template <typename T>

@@ -1178,7 +1178,7 @@ def short_conv_ws(T: int, B: int, D: int, W: int, device) -> torch.Tensor:
 def _conv_args(x, w, bias, silu, reset, lengths, y=None, state_in=None, state_out=None, dy=None, dx=None, dw=None, db=None, ws=None,
                dstate_in=None, dstate_out=None):
     shape, W = x.shape, w.shape[-1]
-    if len(shape) != 3 or not 0 < shape[0] <= 1000000 or not 0 < shape[1] <= 65535 or shape[2] < 1 or not 2 <= W <= 4 \
+    if len(shape) != 3 or not 0 < shape[0] <= 1000000 or not 0 < shape[1] <= 65535 or not 0 < shape[2] <= 1 << 22 or not 2 <= W <= 4 \
             or shape[0] * shape[1] > 1 << 31:
         raise ValueError("short_conv: unsupported sizes %s with %d taps" % (tuple(shape), W))
     T, B, D = shape
@@ -1204,7 +1204,7 @@ def short_conv_fwd(x, w, bias, y, state_in=None, state_out=None, reset=None, len
     ``state_in`` [B, W-1, D] holds the inputs before step 0 (None: zeros) and ``state_out`` receives the last W-1 inputs of
     every row, so that a sequence can be cut anywhere (burn-in / training window). ``reset`` uint8 [T, B]: a non-zero flag
     cuts step t and all later ones off from the steps before t, the carried state included (episode start). ``lengths``
-    int32 [B]: steps from lengths[b] on are padding: not read, and zero in y."""
+    int32 [B]: steps from lengths[b] on are padding: not read, and zero in y. T <= 10^6, B <= 65535, D <= 2^22."""
     _need(x=x, w=w, y=y)
     _run(native.hip().drl_short_conv_fwd, *_conv_args(x, w, bias, silu, reset, lengths, y, state_in, state_out))
 
@@ -1255,7 +1255,7 @@ def ssm_scan_ckpt(T: int, B: int, D: int, N: int, device) -> torch.Tensor:
 def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None, ws=None, h0=None, hT=None, ckpt=None, dy=None, dhT=None,
               du=None, ddt=None, dz=None, dB=None, dC=None, dA=None, dD=None, ddt_bias=None, dh0=None):
     shape, bc = u.shape, Bm.shape
-    if len(shape) != 3 or len(bc) != 3 or not 0 < shape[0] < 1 << 31 or not 0 < shape[1] <= 65535 or not 0 < shape[2] < 1 << 25 \
+    if len(shape) != 3 or len(bc) != 3 or not 0 < shape[0] <= 1 << 30 or not 0 < shape[1] <= 65535 or not 0 < shape[2] <= 1 << 22 \
             or not 0 < bc[2] <= 64 or shape[0] * shape[1] > 1 << 31:
         raise ValueError("ssm_scan: unsupported sizes: u must be [T, B, D], Bm [T, B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
     T, B, Dc = shape
@@ -1285,7 +1285,7 @@ def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None,
 
 def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None, hT=None, reset=None, lengths=None,
                  softplus: bool = True, ckpt=None) -> None:
-    """Selective state-space scan of u [T, B, D] with N <= 64 states per channel:
+    """Selective state-space scan of u [T, B, D] with N <= 64 states per channel (B <= 65535, D <= 2^22, T B <= 2^31):
 
         s = softplus(dt + dt_bias)                 (``softplus=False``: s = dt + dt_bias)
         h = exp(s A) h + s u Bm                    h [B, D, N] fp32, A fp32 [D, N], Bm [T, B, N]

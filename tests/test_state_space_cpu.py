@@ -120,6 +120,16 @@ def test_sizes_are_refused(T, B, D, N):
         hip.layer_norm_fwd(torch.empty(T * 0, 16385), torch.empty(16385), None, torch.empty(0, 16385))
 
 
+def test_sizes_past_the_limits_are_refused():
+    big = lambda *shape: torch.empty(1).expand(shape)                       # noqa: E731
+    for T, B, D in (((1 << 30) + 1, 1, 1), (2, 65536, 1), (1, 1, (1 << 22) + 1), (40000, 65535, 1)):
+        u, bc = big(T, B, D), big(T, B, 4)
+        with pytest.raises(ValueError, match="unsupported sizes"):
+            hip.ssm_scan_fwd(u, u, big(D, 4), bc, bc, u, torch.empty(0))
+        with pytest.raises(ValueError, match="unsupported sizes"):
+            hip.short_conv_fwd(u, big(D, 4), None, u)
+
+
 def test_missing_tensors_are_refused():
     x, w = torch.zeros(4, 8), torch.ones(8)
     with pytest.raises(ValueError, match="w is needed"):

@@ -430,6 +430,70 @@ def test_conv_and_scan_past_32_bits():
         assert float((a - b).norm() / b.norm()) < 2.0 ** -8                # each is rounded to bf16 once: 2^-8 between the two
 
 
+def test_scan_of_one_step_of_many_rows():
+    # the stride of the one step is 1.3e8 elements: offsets inside a chunk must not count it
+    B, D = 65535, 2048
+    g = Gen(0)
+    u = torch.empty(1, B, D, dtype=BF, device=DEV)
+    u.random_(-2, 3)
+    A, bc = -g.u(D, 1) - 0.5, g.n(1, B, 2, dtype=BF)
+    y, hT, ws = torch.empty_like(u), torch.empty(B, D, 1, device=DEV), H.ssm_scan_ws(1, B, D, 1, DEV)
+    ck = H.ssm_scan_ckpt(1, B, D, 1, DEV)
+    o = [torch.empty_like(u) for _ in range(2)] + [torch.empty(D, 1, device=DEV)] + [torch.empty(1, B, 1, dtype=BF, device=DEV) for _ in range(2)]
+    H.ssm_scan_fwd(u, u, A, bc[..., :1], bc[..., 1:], y, ws, hT=hT, ckpt=ck)
+    H.ssm_scan_bwd(u, u, u, A, bc[..., :1], bc[..., 1:], ck, *o, ws)
+    for cut in (slice(0, 3), slice(B - 3, B)):
+        v, b = u[:, cut].contiguous(), bc[:, cut].contiguous()
+        p, q = torch.empty_like(v), [torch.empty_like(v) for _ in range(2)] + [o[2].clone()] + [torch.empty(1, 3, 1, dtype=BF, device=DEV) for _ in range(2)]
+        h, w, c = torch.empty(3, D, 1, device=DEV), H.ssm_scan_ws(1, 3, D, 1, DEV), H.ssm_scan_ckpt(1, 3, D, 1, DEV)
+        H.ssm_scan_fwd(v, v, A, b[..., :1], b[..., 1:], p, w, hT=h, ckpt=c)
+        H.ssm_scan_bwd(v, v, v, A, b[..., :1], b[..., 1:], c, *q, w)
+        assert torch.equal(y[:, cut], p) and torch.equal(hT[cut], h)
+        assert torch.equal(o[0][:, cut], q[0]) and torch.equal(o[1][:, cut], q[1]) and torch.equal(o[3][:, cut], q[3]) and torch.equal(o[4][:, cut], q[4])
+
+
+def test_gradients_of_more_elements_than_a_launch_takes():
+    # 1.1e9 elements of dB and dC. Every step starts an episode, so dB = dy C s u and dC = dy s u B by themselves.
+    T, N = (1 << 23) + 70, 64
+    g = Gen(0)
+    u, dy = g.n(T, 1, 1, dtype=BF), g.n(T, 1, 1, dtype=BF)
+    bc = torch.empty(T, 1, 2 * N, dtype=BF, device=DEV)
+    bc.random_(-2, 3)
+    dt, A, one = torch.full_like(u, 0.5), -torch.ones(1, N, device=DEV), torch.ones(T, 1, dtype=torch.uint8, device=DEV)
+    y, ws, ck = torch.empty_like(u), H.ssm_scan_ws(T, 1, 1, N, DEV), H.ssm_scan_ckpt(T, 1, 1, N, DEV)
+    o = [torch.empty_like(u) for _ in range(2)] + [torch.empty(1, N, device=DEV)] + [torch.empty(T, 1, N, dtype=BF, device=DEV) for _ in range(2)]
+    H.ssm_scan_fwd(u, dt, A, bc[..., :N], bc[..., N:], y, ws, reset=one, softplus=False, ckpt=ck)
+    H.ssm_scan_bwd(dy, u, dt, A, bc[..., :N], bc[..., N:], ck, *o, ws, reset=one, softplus=False)
+    for cut in (slice(0, 1000), slice(T - 1000, T)):
+        f = (dy[cut].double() * 0.5 * u[cut].double())
+        for got, x in ((o[3], bc[cut, :, N:]), (o[4], bc[cut, :, :N])):
+            want = f * x.double()
+            assert bool(((got[cut].double() - want).abs() <= want.abs() * 2.0 ** -8 * 1.01).all())      # one rounding to bf16
+
+
+def test_steps_of_more_channels_than_a_launch_takes():
+    B, D, N = 70000, 2048, 33                               # 1.4e8 channels of 64 lanes
+    g = Gen(0)
+    u = torch.empty(B, D, dtype=BF, device=DEV)
+    u.random_(-2, 3)
+    A, bc, y, h = -g.u(D, N), g.n(B, 2 * N, dtype=BF), torch.empty_like(u), torch.ones(B, D, N, device=DEV)
+    H.ssm_step(u, u, A, bc[:, :N], bc[:, N:], h, y)
+    for cut in (slice(0, 2), slice(B - 2, B)):
+        p, k = torch.empty_like(u[cut]), torch.ones(2, D, N, device=DEV)
+        H.ssm_step(u[cut], u[cut], A, bc[cut, :N], bc[cut, N:], k, p)
+        assert torch.equal(p, y[cut]) and torch.equal(k, h[cut])
+    del u, y, h
+    B, D, W = 2100000, 1025, 2                              # 2.2e9 channels, one a thread
+    x, s = torch.empty(B, D, dtype=BF, device=DEV), torch.empty(B, 1, D, dtype=BF, device=DEV)
+    x.random_(-2, 3); s.fill_(0.5)
+    w, y = g.n(D, W), torch.empty_like(x)
+    H.short_conv_step(x, w, None, s, y)
+    for cut in (slice(0, 2), slice(B - 2, B)):
+        p, k = torch.empty_like(x[cut]), torch.full((2, 1, D), 0.5, dtype=BF, device=DEV)
+        H.short_conv_step(x[cut], w, None, k, p)
+        assert torch.equal(p, y[cut]) and torch.equal(k, s[cut])
+
+
 # ---- same inputs, same bits; streams; graphs ----------------------------------------------------------------------------
 def test_results_do_not_change_from_call_to_call():
     for v in (scan_case(70, 5, 96, 16, BF), scan_case(523, 1, 40, 8, F32)):
