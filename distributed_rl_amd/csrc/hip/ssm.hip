@@ -110,9 +110,11 @@ __device__ __forceinline__ void lds_row(const float* q, float (&v)[NS]) {
     if constexpr (NS % 4 == 0) {
 #pragma unroll
         for (int i = 0; i < NS; i += 4) { const float4 x = *reinterpret_cast<const float4*>(q + i); v[i] = x.x; v[i + 1] = x.y; v[i + 2] = x.z; v[i + 3] = x.w; }
-    } else {
+    } else if constexpr (NS == 2) {
         const float2 x = *reinterpret_cast<const float2*>(q);
         v[0] = x.x; v[1] = x.y;
+    } else {
+        v[0] = *q;
     }
 }
 
@@ -186,7 +188,7 @@ __device__ __forceinline__ float sum_groups(float v0, float v1, float v2, float 
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
 // Sums over the 16 lanes of a row, NS x 4 of them at a time: quad 0 holds the sums of be, quad 1 bo, quad 2 ce, quad 3 co, and
-// lane q of a quad the one of index q (index q & 1 where there are two). Every level folds two values into one register - by
+// lane q of a quad the one of index q (q & 1 where there are two, any lane where there is one). Every level folds two values into one register - by
 // bank masks, which write half of the quads each, or within quads by exchanging what the other lane keeps - so a value costs
 // 2 to 2.3 instructions instead of 4 adds. Between a write and a cross-lane read of it there are 2 wait states: the other
 // registers' adds, or s_nop.
@@ -198,6 +200,17 @@ __device__ __forceinline__ float quad_fold(bool odd, float v0, float v1) {
 }
 #define QUAD_XOR1 0xB1
 #define QUAD_XOR2 0x4E
+template <int CTRL>
+__device__ __forceinline__ float quad_add(float v) { return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true)); }
+__device__ __forceinline__ float sum_rows1(const float* be, const float* ce, const float* bo, const float* co) {
+    float t0, t1, r;
+    asm volatile("s_nop 1\n"
+        DPP(0, 2, "row_mirror", "0x3") DPP(1, 3, "row_mirror", "0x3") DPP(0, 4, "row_mirror", "0xc") DPP(1, 5, "row_mirror", "0xc")
+        : "=&v"(t0), "=&v"(t1) : "v"(be[0]), "v"(bo[0]), "v"(ce[0]), "v"(co[0]));
+    asm volatile("s_nop 1\n" DPP(0, 1, "row_half_mirror", "0x5") DPP(0, 2, "row_half_mirror", "0xa") "s_nop 1\n"
+        : "=&v"(r) : "v"(t0), "v"(t1));
+    return quad_add<QUAD_XOR2>(quad_add<QUAD_XOR1>(r));
+}
 __device__ __forceinline__ float sum_rows2(const float* be, const float* ce, const float* bo, const float* co, int j) {
     float t0, t1, t2, t3, r0, r1;
     asm volatile("s_nop 1\n"
@@ -209,8 +222,7 @@ __device__ __forceinline__ float sum_rows2(const float* be, const float* ce, con
         DPP(0, 2, "row_half_mirror", "0x5") DPP(1, 3, "row_half_mirror", "0x5")
         DPP(0, 4, "row_half_mirror", "0xa") DPP(1, 5, "row_half_mirror", "0xa") "s_nop 1\n"
         : "=&v"(r0), "=&v"(r1) : "v"(t0), "v"(t1), "v"(t2), "v"(t3));
-    float v = quad_fold<QUAD_XOR1>(j & 1, r0, r1);
-    return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), QUAD_XOR2, 0xf, 0xf, true));
+    return quad_add<QUAD_XOR2>(quad_fold<QUAD_XOR1>(j & 1, r0, r1));
 }
 __device__ __forceinline__ float sum_rows4(const float* be, const float* ce, const float* bo, const float* co, int j) {
     float t[8], r[4];
@@ -365,8 +377,8 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     __shared__ __align__(16) float2 pw_s[4][KC][16];
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    static_assert(sizeof(bc_s) > SORT_ROWS * sizeof(int), "block_row");
-    const int b = block_row(p, (int*)bc_s);
+    static_assert(sizeof(pw_s) > SORT_ROWS * sizeof(int), "block_row");
+    const int b = block_row(p, (int*)pw_s);
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
     const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
@@ -538,8 +550,10 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
         if constexpr (NS % 4 == 0) {
 #pragma unroll
             for (int i = 0; i < NS; i += 4) red[i + (j & 3)] = sum_rows4(vB[0] + i, vC[0] + i, vB[1] + i, vC[1] + i, j);
-        } else {
+        } else if constexpr (NS == 2) {
             red[j & 1] = sum_rows2(vB[0], vC[0], vB[1], vC[1], j);
+        } else {
+            red[0] = sum_rows1(vB[0], vC[0], vB[1], vC[1]);
         }
         if ((k & 3) == 0) {
             emit(s0 + k, sum_groups(pb[0], pb[1], pb[2], pb[3]), sum_groups(pa[0], pa[1], pa[2], pa[3]));
@@ -560,8 +574,8 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
-    static_assert(sizeof(bc_s) > SORT_ROWS * sizeof(int), "block_row");
-    const int b = block_row(p, (int*)bc_s);
+    static_assert(sizeof(pw_s) > SORT_ROWS * sizeof(int), "block_row");
+    const int b = block_row(p, (int*)pw_s);
     const int d = (blockIdx.x * 4 + w) * 16 + j;
     const bool dv = d < p.D;
     const int end = row_end(p, b), ta = blockIdx.z * seg_len, tb = min(ta + seg_len, (int)p.T);
@@ -832,7 +846,9 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
     }
 }
 
-static int ns_of(long long N) { return N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 48 ? 12 : 16; }
+// States a lane, of the four lanes a channel has. Up to 4 states one each: 120 x 64 x 1024 bf16 forward 29 us and both passes 98,
+// with two each (half of them empty) 33 and 124.
+static int ns_of(long long N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : N <= 48 ? 12 : 16; }
 
 // Segments: one where the rows alone give the chip 768 waves, else as many as bring it to 4 096, of at least 64 steps. A cut
 // costs the carry pass (the recurrence without its read-out), so rows that fill the chip are never cut.
@@ -902,6 +918,7 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
 
 #define SSM_NS(NAME, T)                       \
     switch (ns_of(p.N)) {                     \
+        case 1: NAME<T, 1>(p, s); break;      \
         case 2: NAME<T, 2>(p, s); break;      \
         case 4: NAME<T, 4>(p, s); break;      \
         case 8: NAME<T, 8>(p, s); break;      \

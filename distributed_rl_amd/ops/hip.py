@@ -1089,6 +1089,10 @@ def _row2(t: torch.Tensor, shape: tuple, dtype, dev: int, name: str, out: bool =
         _refuse(t, shape, dtype, dev, name)
     if t.is_contiguous():
         return t.data_ptr(), shape[1]
+    if not out:
+        step, last = t.stride()
+        if last == 1:
+            return t.data_ptr(), step
     return _rows(t, shape, dtype, dev, name, out)
 
 

@@ -271,7 +271,7 @@ def test_scan_rows_without_a_step():
     assert all(torch.equal(a[k], b[k]) for k in a)
 
 
-@pytest.mark.parametrize("T,B,D,N,dtype", [(300, 1, 16, 16, F32), (523, 1, 40, 8, BF), (1100, 2, 17, 5, F32), (260, 1, 64, 40, F32)])
+@pytest.mark.parametrize("T,B,D,N,dtype", [(300, 1, 16, 16, F32), (523, 1, 40, 8, BF), (1100, 2, 17, 5, F32), (260, 1, 64, 40, F32), (701, 1, 33, 3, BF)])
 def test_scan_long_and_few_rows(T, B, D, N, dtype):
     check_scan(scan_case(T, B, D, N, dtype, reset=0.004, shift=-4.0, scale=0.3))
     check_scan(scan_case(T, B, D, N, dtype, reset=0, ragged=False, shift=-4.0, scale=0.3))
