@@ -1132,8 +1132,19 @@ struct NoBody {
     static __device__ __forceinline__ void run(const Args&, int, uint8_t*) {}
 };
 
+// Waves a SIMD that a fused launch is held to (0: as they come). conv2's backward with a two-step pipeline needs 126 to 130
+// registers, as the compiler happens to allot them, and 128 is where a fourth wave fits: 512 frames 28.7 us with it, 38.5 with three.
 template <class B0, class B1, class B2, class B3>
-__global__ __launch_bounds__(NTHREADS) void k_multi(typename B0::Args a0, typename B1::Args a1, typename B2::Args a2,
+inline constexpr int multi_waves = 0;
+template <class AOp, class BOp, class AOp2, class BOp2>
+inline constexpr int multi_waves<TreeBody, ColsumBody, GemmBody<64, 64, 64, 2, 2, true, true, 2, AOp, BOp>,
+                                 GemmBody<128, 32, 64, 4, 1, false, true, 2, AOp2, BOp2>> = 4;
+template <class AOp, class BOp, class AOp2, class BOp2>
+inline constexpr int multi_waves<TreeBody, ColsumBody, GemmBody<128, 32, 64, 4, 1, false, true, 2, AOp2, BOp2>,
+                                 GemmBody<64, 64, 64, 2, 2, true, true, 2, AOp, BOp>> = 4;
+
+template <class B0, class B1, class B2, class B3>
+__global__ __launch_bounds__(NTHREADS, (multi_waves<B0, B1, B2, B3>)) void k_multi(typename B0::Args a0, typename B1::Args a1, typename B2::Args a2,
                                                     typename B3::Args a3, int e0, int e1, int e2) {
     extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
     const int b = blockIdx.x;
