@@ -1020,7 +1020,7 @@ def add2(a, b, out) -> None:
 # may not share memory with an input. Scratch (``*_ws``) belongs to the caller: calls that may run at the same time (two
 # streams, two graphs) need one each.
 _NORM, _CONV, _SSM = (struct.Struct("<%dq" % n) for n in (18, 29, 56))
-_NORM_FWD, _CONV_STEP, _SSM_STEP = (struct.Struct("<%dq%dx" % (n, 8 * m)) for n, m in ((10, 8), (17, 12), (33, 23)))     # the rest zero
+_NORM_FWD, _CONV_FWD, _SSM_FWD = (struct.Struct("<%dq%dx" % (n, 8 * m)) for n, m in ((10, 8), (17, 12), (33, 23)))        # the rest zero
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -1070,7 +1070,7 @@ def _rows(t: Optional[torch.Tensor], shape: tuple, dtype, dev: int, name: str, o
         _refuse(t, shape, dtype, dev, name)
     st = t.stride()
     if t.is_contiguous():
-        return (t.data_ptr(),) + st[:-1]
+        return (t.data_ptr(), *st[:-1])
     if st[-1] != 1 and shape[-1] > 1:
         raise ValueError("%s: the last dimension must be contiguous (strides %s)" % (name, st))
     if out:
@@ -1096,11 +1096,27 @@ def _row2(t: torch.Tensor, shape: tuple, dtype, dev: int, name: str, out: bool =
     return _rows(t, shape, dtype, dev, name, out)
 
 
+def _rows3(t: Optional[torch.Tensor], shape: tuple, lead: tuple, dtype, dev: int, name: str, out: bool = False) -> tuple:
+    """``_rows`` of a 3-d tensor; ``lead``: the strides of a contiguous one (and an axis of one step has any stride)."""
+    if t is None:
+        return 0, 0, 0
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev:
+        _refuse(t, shape, dtype, dev, name)
+    if t.is_contiguous():
+        return (t.data_ptr(), *lead)
+    if not out:
+        a, b, last = t.stride()
+        if last == 1:
+            return t.data_ptr(), a, b
+    return _rows(t, shape, dtype, dev, name, out)
+
+
 def _apart(outs: tuple, ins: tuple) -> None:
     """No output starts where an input or another output does (0: not given)."""
-    for a in outs:
-        if a and (a in ins or outs.count(a) > 1):
-            raise ValueError("an output shares its memory with an input or another output")
+    given = {*outs}
+    given.discard(0)
+    if len(given) != len(outs) - outs.count(0) or not given.isdisjoint(ins):
+        raise ValueError("an output shares its memory with an input or another output")
 
 
 def _need(**tensors) -> None:
@@ -1155,15 +1171,17 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
 def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:
     """Gradients of :func:`layer_norm_fwd`: dx [rows, D], dw and db (None if the norm has no b) fp32 [D], overwritten. The
     sums over rows run in a fixed order. ``ws`` from :func:`layer_norm_ws`."""
-    _need(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dw=dw, ws=ws)
+    if dy is None or x is None or w is None or mean is None or rstd is None or dx is None or dw is None or ws is None:
+        _need(dy=dy, x=x, w=w, mean=mean, rstd=rstd, dx=dx, dw=dw, ws=ws)
     shape, typ, f32 = _norm_shape(x), x.dtype, torch.float32
     dev, bf16 = _dev(x), _typ(x)
     M, D = shape
-    xr, dyr, dxr = _rows(x, shape, typ, dev, "x"), _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
-    wp, mp, rp = _vec(w, (D,), f32, dev, "w"), _vec(mean, (M,), f32, dev, "mean"), _vec(rstd, (M,), f32, dev, "rstd")
-    dwp, dbp, wsp = _vec(dw, (D,), f32, dev, "dw"), _opt(db, (D,), f32, dev, "db"), _vec(ws, (ws.numel(),), f32, dev, "ws")
+    xr, dyr, dxr = _row2(x, shape, typ, dev, "x"), _row2(dy, shape, typ, dev, "dy"), _row2(dx, shape, typ, dev, "dx", True)
+    d, m, n_ws = (D,), (M,), ws.numel()
+    wp, mp, rp = _vec(w, d, f32, dev, "w"), _vec(mean, m, f32, dev, "mean"), _vec(rstd, m, f32, dev, "rstd")
+    dwp, dbp, wsp = _vec(dw, d, f32, dev, "dw"), _vec(db, d, f32, dev, "db") if db is not None else 0, _vec(ws, (n_ws,), f32, dev, "ws")
     _apart((dxr[0], dwp, dbp, wsp), (xr[0], dyr[0], wp, mp, rp))
-    _run(native.hip().drl_norm_bwd, _NORM.pack(*xr, wp, 0, 0, 0, mp, rp, M, D, *dyr, *dxr, dwp, dbp, wsp, ws.numel()), bf16, dev)
+    _run(native.hip().drl_norm_bwd, _NORM.pack(*xr, wp, 0, 0, 0, mp, rp, M, D, *dyr, *dxr, dwp, dbp, wsp, n_ws), bf16, dev)
 
 
 def _norm_shape(x) -> torch.Size:
@@ -1187,17 +1205,23 @@ def _conv_args(x, w, bias, silu, reset, lengths, y=None, state_in=None, state_ou
         raise ValueError("short_conv: unsupported sizes %s with %d taps" % (tuple(shape), W))
     T, B, D = shape
     dev, typ, f32 = _dev(x), x.dtype, torch.float32
-    bf16, st = _typ(x), (B, W - 1, D)
-    xr, yr = _rows(x, shape, typ, dev, "x"), _rows(y, shape, typ, dev, "y", True)
-    dyr, dxr = _rows(dy, shape, typ, dev, "dy"), _rows(dx, shape, typ, dev, "dx", True)
-    wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
-    si, so = _opt(state_in, st, typ, dev, "state_in"), _opt(state_out, st, typ, dev, "state_out")
-    dsi, dso = _opt(dstate_in, st, typ, dev, "dstate_in"), _opt(dstate_out, st, typ, dev, "dstate_out")
-    rp, lp = _opt(reset, (T, B), torch.uint8, dev, "reset"), _opt(lengths, (B,), torch.int32, dev, "lengths")
-    dwp, dbp = _opt(dw, (D, W), f32, dev, "dw"), _opt(db, (D,), f32, dev, "db")
-    wsp, n_ws = (_vec(ws, (ws.numel(),), f32, dev, "ws"), ws.numel()) if ws is not None else (0, 0)
-    _apart((yr[0], so, dxr[0], dwp, dbp, dsi, wsp), (xr[0], wp, bp, si, dyr[0], dso, rp, lp))
-    return _CONV.pack(xr[0], si, xr[1], xr[2], wp, bp, rp, lp, yr[0], so, yr[1], yr[2], T, B, D, W, 1 if silu else 0, dyr[0], dso,
+    bf16, lead, st, wd, d = _typ(x), (B * D, D), (B, W - 1, D), (D, W), (D,)
+    xr = _rows3(x, shape, lead, typ, dev, "x")
+    wp, bp = _vec(w, wd, f32, dev, "w"), _vec(bias, d, f32, dev, "bias") if bias is not None else 0
+    si = _vec(state_in, st, typ, dev, "state_in") if state_in is not None else 0
+    rp = _vec(reset, (T, B), torch.uint8, dev, "reset") if reset is not None else 0
+    lp = _vec(lengths, (B,), torch.int32, dev, "lengths") if lengths is not None else 0
+    if dy is None:
+        yr, so = _rows3(y, shape, lead, typ, dev, "y", True), _opt(state_out, st, typ, dev, "state_out")
+        _apart((yr[0], so), (xr[0], wp, bp, si, rp, lp))
+        return _CONV_FWD.pack(xr[0], si, xr[1], xr[2], wp, bp, rp, lp, yr[0], so, yr[1], yr[2], T, B, D, W, 1 if silu else 0), bf16, dev
+    dyr, dxr = _rows3(dy, shape, lead, typ, dev, "dy"), _rows3(dx, shape, lead, typ, dev, "dx", True)
+    dsi = _vec(dstate_in, st, typ, dev, "dstate_in") if dstate_in is not None else 0
+    dso = _vec(dstate_out, st, typ, dev, "dstate_out") if dstate_out is not None else 0
+    dwp, dbp, n_ws = _vec(dw, wd, f32, dev, "dw"), _vec(db, d, f32, dev, "db") if db is not None else 0, ws.numel()
+    wsp = _vec(ws, (n_ws,), f32, dev, "ws")
+    _apart((dxr[0], dwp, dbp, dsi, wsp), (xr[0], wp, bp, si, dyr[0], dso, rp, lp))
+    return _CONV.pack(xr[0], si, xr[1], xr[2], wp, bp, rp, lp, 0, 0, 0, 0, T, B, D, W, 1 if silu else 0, dyr[0], dso,
                       dyr[1], dyr[2], dxr[0], dsi, dxr[1], dxr[2], dwp, dbp, wsp, n_ws), bf16, dev
 
 
@@ -1209,7 +1233,8 @@ def short_conv_fwd(x, w, bias, y, state_in=None, state_out=None, reset=None, len
     every row, so that a sequence can be cut anywhere (burn-in / training window). ``reset`` uint8 [T, B]: a non-zero flag
     cuts step t and all later ones off from the steps before t, the carried state included (episode start). ``lengths``
     int32 [B]: steps from lengths[b] on are padding: not read, and zero in y. T <= 10^6, B <= 65535, D <= 2^22."""
-    _need(x=x, w=w, y=y)
+    if x is None or w is None or y is None:
+        _need(x=x, w=w, y=y)
     _run(native.hip().drl_short_conv_fwd, *_conv_args(x, w, bias, silu, reset, lengths, y, state_in, state_out))
 
 
@@ -1218,7 +1243,8 @@ def short_conv_bwd(dy, x, w, bias, dx, dw, db, ws, state_in=None, dstate_in=None
     """Gradients of :func:`short_conv_fwd` (same x, w, bias, state_in, reset, lengths): dx [T, B, D] (zero on padding), dw
     fp32 [D, W], db fp32 [D] or None, dstate_in [B, W-1, D] or None, all overwritten; ``dstate_out`` adds the gradient that
     arrives at state_out. The sums over rows and steps run in a fixed order. ``ws`` from :func:`short_conv_ws`."""
-    _need(dy=dy, x=x, w=w, dx=dx, dw=dw, ws=ws)
+    if dy is None or x is None or w is None or dx is None or dw is None or ws is None:
+        _need(dy=dy, x=x, w=w, dx=dx, dw=dw, ws=ws)
     _run(native.hip().drl_short_conv_bwd,
          *_conv_args(x, w, bias, silu, reset, lengths, None, state_in, None, dy, dx, dw, db, ws, dstate_in, dstate_out))
 
@@ -1238,7 +1264,7 @@ def short_conv_step(x, w, bias, state, y, reset=None, silu: bool = True) -> None
     sp, rp = _vec(state, (B, W - 1, D), typ, dev, "state"), _opt(reset, (B,), torch.uint8, dev, "reset")
     wp, bp = _vec(w, (D, W), f32, dev, "w"), _opt(bias, (D,), f32, dev, "bias")
     _apart((yp, sp), (xp, wp, bp, rp))
-    _run(native.hip().drl_short_conv_step, _CONV_STEP.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0), bf16, dev)
+    _run(native.hip().drl_short_conv_step, _CONV_FWD.pack(xp, 0, 0, xs, wp, bp, rp, 0, yp, sp, 0, ys, 1, B, D, W, 1 if silu else 0), bf16, dev)
 
 
 SSM_SAVE = 8                # steps between the states that ssm_scan_fwd saves for ssm_scan_bwd
@@ -1265,26 +1291,44 @@ def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None,
     T, B, Dc = shape
     N = bc[2]
     dev, typ, f32 = _dev(u), u.dtype, torch.float32
-    bf16, st, bc = _typ(u), (B, Dc, N), (T, B, N)
-    ur, dtr, zr = _rows(u, shape, typ, dev, "u"), _rows(dt, shape, typ, dev, "dt"), _rows(z, shape, typ, dev, "z")
-    Br, Cr = _rows(Bm, bc, typ, dev, "Bm"), _rows(Cm, bc, typ, dev, "Cm")
-    yr, dyr = _rows(y, shape, typ, dev, "y", True), _rows(dy, shape, typ, dev, "dy")
-    dur, ddtr, dzr = _rows(du, shape, typ, dev, "du", True), _rows(ddt, shape, typ, dev, "ddt", True), _rows(dz, shape, typ, dev, "dz", True)
-    dBr, dCr = _rows(dB, bc, typ, dev, "dB", True), _rows(dC, bc, typ, dev, "dC", True)
-    Ap, dAp = _vec(A, (Dc, N), f32, dev, "A"), _opt(dA, (Dc, N), f32, dev, "dA")
-    Dp, bp, dDp, dbp = (_opt(t, (Dc,), f32, dev, n) for t, n in ((D, "D"), (dt_bias, "dt_bias"), (dD, "dD"), (ddt_bias, "ddt_bias")))
-    h0p, hTp, dhTp, dh0p = (_opt(t, st, f32, dev, n) for t, n in ((h0, "h0"), (hT, "hT"), (dhT, "dhT"), (dh0, "dh0")))
-    rp, lp = _opt(reset, (T, B), torch.uint8, dev, "reset"), _opt(lengths, (B,), torch.int32, dev, "lengths")
-    ck = _opt(ckpt, ((T + SSM_SAVE - 1) // SSM_SAVE, B, Dc, N), f32, dev, "ckpt")
-    n_ws = ws.numel()
-    wsp = _vec(ws, (n_ws,), f32, dev, "ws")
-    if T > 1 and max(ur[1], dtr[1], zr[1], Br[1], Cr[1], yr[1], dyr[1], dur[1], ddtr[1], dzr[1]) >= 1 << 25:
+    bf16, st, ld, lb, dn, d, n_ws = _typ(u), (B, Dc, N), (B * Dc, Dc), (B * N, N), (Dc, N), (Dc,), ws.numel()
+    up, ut, ub = _rows3(u, shape, ld, typ, dev, "u")
+    dtp, dtt, dtb = _rows3(dt, shape, ld, typ, dev, "dt")
+    zp, zt, zb = _rows3(z, shape, ld, typ, dev, "z")
+    Bp, Bt, Bb = _rows3(Bm, bc, lb, typ, dev, "Bm")
+    Cp, Ct, Cb = _rows3(Cm, bc, lb, typ, dev, "Cm")
+    Ap, wsp = _vec(A, dn, f32, dev, "A"), _vec(ws, (n_ws,), f32, dev, "ws")
+    Dp = _vec(D, d, f32, dev, "D") if D is not None else 0
+    bp = _vec(dt_bias, d, f32, dev, "dt_bias") if dt_bias is not None else 0
+    rp = _vec(reset, (T, B), torch.uint8, dev, "reset") if reset is not None else 0
+    lp = _vec(lengths, (B,), torch.int32, dev, "lengths") if lengths is not None else 0
+    ck = _vec(ckpt, ((T + SSM_SAVE - 1) // SSM_SAVE, B, Dc, N), f32, dev, "ckpt") if ckpt is not None else 0
+    far = max(ut, dtt, zt, Bt, Ct)
+    if dy is None:
+        yp, yt, yb = _rows3(y, shape, ld, typ, dev, "y", True)
+        h0p, hTp = _opt(h0, st, f32, dev, "h0"), _opt(hT, st, f32, dev, "hT")
+        if T > 1 and max(far, yt) >= 1 << 25:
+            raise ValueError("ssm_scan: steps of one tensor are 2^25 elements or more apart")
+        _apart((yp, hTp, ck, wsp if n_ws else 0), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, h0p, rp, lp))
+        return _SSM_FWD.pack(up, dtp, zp, Bp, Cp, ut, ub, dtt, dtb, zt, zb, Bt, Bb, Ct, Cb, Ap, Dp, bp, h0p, rp, lp, yp, yt, yb, hTp, ck, wsp,
+                             n_ws, T, B, Dc, N, 1 if softplus else 0), bf16, dev
+    dyp, dyt, dyb = _rows3(dy, shape, ld, typ, dev, "dy")
+    dup, dut, dub = _rows3(du, shape, ld, typ, dev, "du", True)
+    ddp, ddt_, ddb = _rows3(ddt, shape, ld, typ, dev, "ddt", True)
+    dzp, dzt, dzb = _rows3(dz, shape, ld, typ, dev, "dz", True)
+    dBp, dBt, dBb = _rows3(dB, bc, lb, typ, dev, "dB", True)
+    dCp, dCt, dCb = _rows3(dC, bc, lb, typ, dev, "dC", True)
+    dAp = _vec(dA, dn, f32, dev, "dA")
+    dDp = _vec(dD, d, f32, dev, "dD") if dD is not None else 0
+    dbp = _vec(ddt_bias, d, f32, dev, "ddt_bias") if ddt_bias is not None else 0
+    dhTp = _vec(dhT, st, f32, dev, "dhT") if dhT is not None else 0
+    dh0p = _vec(dh0, st, f32, dev, "dh0") if dh0 is not None else 0
+    if T > 1 and max(far, dyt, dut, ddt_, dzt) >= 1 << 25:
         raise ValueError("ssm_scan: steps of one tensor are 2^25 elements or more apart")
-    _apart((yr[0], hTp, ck, wsp if n_ws else 0, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0], dAp, dDp, dbp, dh0p),
-           (ur[0], dtr[0], zr[0], Br[0], Cr[0], Ap, Dp, bp, h0p, rp, lp, dyr[0], dhTp))
-    return _SSM.pack(ur[0], dtr[0], zr[0], Br[0], Cr[0], *ur[1:], *dtr[1:], *zr[1:], *Br[1:], *Cr[1:], Ap, Dp, bp, h0p, rp, lp, *yr,
-                     hTp, ck, wsp, n_ws, T, B, Dc, N, 1 if softplus else 0, *dyr, dhTp, dur[0], ddtr[0], dzr[0], dBr[0], dCr[0],
-                     *dur[1:], *ddtr[1:], *dzr[1:], *dBr[1:], *dCr[1:], dAp, dDp, dbp, dh0p), bf16, dev
+    _apart((wsp, dup, ddp, dzp, dBp, dCp, dAp, dDp, dbp, dh0p), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, rp, lp, ck, dyp, dhTp))
+    return _SSM.pack(up, dtp, zp, Bp, Cp, ut, ub, dtt, dtb, zt, zb, Bt, Bb, Ct, Cb, Ap, Dp, bp, 0, rp, lp, 0, 0, 0, 0, ck, wsp, n_ws, T, B, Dc, N,
+                     1 if softplus else 0, dyp, dyt, dyb, dhTp, dup, ddp, dzp, dBp, dCp, dut, dub, ddt_, ddb, dzt, dzb, dBt, dBb, dCt, dCb,
+                     dAp, dDp, dbp, dh0p), bf16, dev
 
 
 def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None, hT=None, reset=None, lengths=None,
@@ -1299,7 +1343,8 @@ def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None,
     [T, B]: a non-zero flag starts step t from h = 0. ``lengths`` int32 [B]: steps from lengths[b] on are padding: not read,
     zero in y, and hT is the state after step lengths[b] - 1. ``ckpt`` (:func:`ssm_scan_ckpt`) keeps what
     :func:`ssm_scan_bwd` needs; ``ws`` from :func:`ssm_scan_ws`."""
-    _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, y=y, ws=ws)
+    if u is None or dt is None or A is None or Bm is None or Cm is None or y is None or ws is None:
+        _need(u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, y=y, ws=ws)
     _run(native.hip().drl_ssm_fwd, *_ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y, ws, h0, hT, ckpt))
 
 
@@ -1309,7 +1354,9 @@ def ssm_scan_bwd(dy, u, dt, A, Bm, Cm, ckpt, du, ddt, dA, dB, dC, ws, D=None, dD
     dB, dC [T, B, N] (all zero on padding), dA fp32 [D, N], dD, ddt_bias fp32 [D], dh0 fp32 [B, D, N], all overwritten;
     ``dhT`` [B, D, N] is the gradient that arrives at hT (None: zero). dz is needed where z is given, the other optional
     gradients are not. Sums over rows, steps and channels run in a fixed order."""
-    _need(dy=dy, u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, ckpt=ckpt, du=du, ddt=ddt, dA=dA, dB=dB, dC=dC, ws=ws)
+    if dy is None or u is None or dt is None or A is None or Bm is None or Cm is None or ckpt is None or du is None or ddt is None \
+            or dA is None or dB is None or dC is None or ws is None:
+        _need(dy=dy, u=u, dt=dt, A=A, Bm=Bm, Cm=Cm, ckpt=ckpt, du=du, ddt=ddt, dA=dA, dB=dB, dC=dC, ws=ws)
     _none_or_both(z, dz, "z and dz")
     if dD is not None and D is None or ddt_bias is not None and dt_bias is None:
         raise ValueError("dD / ddt_bias without D / dt_bias")
@@ -1338,5 +1385,5 @@ def ssm_step(u, dt, A, Bm, Cm, h, y, D=None, z=None, dt_bias=None, reset=None, s
     Ap, hp, rp = _vec(A, (Dc, N), f32, dev, "A"), _vec(h, (B, Dc, N), f32, dev, "h"), _opt(reset, (B,), torch.uint8, dev, "reset")
     Dp, bp = _opt(D, (Dc,), f32, dev, "D"), _opt(dt_bias, (Dc,), f32, dev, "dt_bias")
     _apart((yp, hp), (up, dtp, zp, Bp, Cp, Ap, Dp, bp, rp))
-    _run(native.hip().drl_ssm_step, _SSM_STEP.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys,
+    _run(native.hip().drl_ssm_step, _SSM_FWD.pack(up, dtp, zp, Bp, Cp, 0, us, 0, dts, 0, zs, 0, Bs, 0, Cs, Ap, Dp, bp, 0, rp, 0, yp, 0, ys,
                                                    hp, 0, 0, 0, 1, B, Dc, N, 1 if softplus else 0), bf16, dev)
