@@ -431,10 +431,11 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
         const unsigned rm = reset_mask(rr);
         if (t0 + KC < live) fetch(t0 + KC);
         block_sync_lds();                 // B and C of this chunk are there; the image of the chunk before last is free again
-        float y[4];
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
         auto steps = [&](auto has) {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
+                if (q == 2 && t0 + 8 >= live) break;        // the row ends in the chunk's first half
                 if (4 * q % SAVE == 0 && p.ckpt && dv && t0 + 4 * q < p.T)
                     put_states<NS>(p.ckpt + (t0 / SAVE + 4 * q / SAVE) * BDN + so, h, g * NS, p.N, ck4);
                 float part[4];
@@ -699,9 +700,21 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
         };
         auto piece = [&](int s0, auto mid) { bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], mid, emit); };
         auto nothing = [] {};
+        const bool half = t0 + SAVE >= live;                // the row ends in the chunk's first half: the other is zeros
+        if (half) {
+#pragma unroll
+            for (int i = 2; i < 4; ++i) {
+                const unsigned bad = dv && t0 + 4 * i + g < n_t ? 0u : OOB;
+                R::store(wu.rsrc(), odu | bad, i * wu.four, 0.f);
+                R::store(wd.rsrc(), odd | bad, i * wd.four, 0.f);
+                if (has_z) R::store(wz.rsrc(), odz | bad, i * wz.four, 0.f);
+            }
+        }
         if constexpr (KH == SAVE) {
-            from(hc1);
-            piece(SAVE, nothing);
+            if (!half) {
+                from(hc1);
+                piece(SAVE, nothing);
+            }
             from(h0);
             piece(0, next);
         } else {                                            // two pieces from each saved state: its steps are run up to the second
@@ -716,8 +729,10 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
                     for (int i = 0; i < NS; ++i) hs[0][i] = fmaf(__builtin_amdgcn_exp2f(pw.x * An[i]), rs ? 0.f : hs[0][i], pw.y * Bv[i]);
                 }
             };
-            from(hc1); run(SAVE); piece(SAVE + KH, nothing);
-            from(hc1); piece(SAVE, nothing);
+            if (!half) {
+                from(hc1); run(SAVE); piece(SAVE + KH, nothing);
+                from(hc1); piece(SAVE, nothing);
+            }
             from(h0); run(0); piece(KH, nothing);
             from(h0); piece(0, next);
         }
