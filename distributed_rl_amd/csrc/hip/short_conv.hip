@@ -3,9 +3,11 @@
 // Steps before the first come from state_in [B, W - 1, D]; a set reset flag at t cuts every tap from t on off from the steps
 // before t; steps from lengths[b] on are not read and write zeros.
 //
-// Bound by memory: a thread owns V neighbouring channels (16 bytes of fp32, 8 of bf16; 1 where addresses or strides do not
-// allow it) of one row and a run of steps, reads FB (BB) steps ahead and keeps the last W - 1 inputs in registers. Runs of one
-// row are walked side by side; each starts by reading the W - 1 steps before it again.
+// Bound by memory: a thread owns V neighbouring channels of one row (4 of fp32, 2 of bf16, at any alignment; 1 where there are
+// fewer) and a run of steps, reads FB (BB) steps ahead and keeps the last W - 1 inputs in registers. The last vector ends at
+// the last channel: the channels that it has twice come out alike. Runs of one row are walked side by side; each starts by
+// reading the W - 1 steps before it again. More channels a thread means fewer loads but also fewer waves on a SIMD: both
+// passes of 120 x 64 x 1024 bf16 29 us with 2, 30 with 1, 33 with 4; of 1021 x 9 x 771 fp32 46 with 4, 51 with 2, 54 with 1.
 #include "ssm_math.h"
 #include <type_traits>
 
@@ -35,20 +37,42 @@ template <typename T, int V>
 __device__ __forceinline__ void cload(const T* q, float (&v)[V]) {
     if constexpr (V == 1) {
         v[0] = ld(q);
+    } else if constexpr (V == 2 && sizeof(T) == 2) {
+        uint32_t r;
+        __builtin_memcpy(&r, q, 4);
+        v[0] = __uint_as_float(r << 16); v[1] = __uint_as_float(r & 0xffff0000u);
+    } else if constexpr (V == 2) {
+        float2 r;
+        __builtin_memcpy(&r, q, 8);
+        v[0] = r.x; v[1] = r.y;
     } else if constexpr (sizeof(T) == 2) {
-        const uint2 r = *reinterpret_cast<const uint2*>(q);
+        uint2 r;
+        __builtin_memcpy(&r, q, 8);
         v[0] = __uint_as_float(r.x << 16); v[1] = __uint_as_float(r.x & 0xffff0000u);
         v[2] = __uint_as_float(r.y << 16); v[3] = __uint_as_float(r.y & 0xffff0000u);
     } else {
-        const float4 r = *reinterpret_cast<const float4*>(q);
+        float4 r;
+        __builtin_memcpy(&r, q, 16);
         v[0] = r.x; v[1] = r.y; v[2] = r.z; v[3] = r.w;
     }
 }
 template <typename T, int V>
 __device__ __forceinline__ void cstore(T* q, const float (&v)[V]) {
-    if constexpr (V == 1) st(q, v[0]);
-    else if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(q) = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
-    else *reinterpret_cast<float4*>(q) = make_float4(v[0], v[1], v[2], v[3]);
+    if constexpr (V == 1) {
+        st(q, v[0]);
+    } else if constexpr (V == 2 && sizeof(T) == 2) {
+        const uint32_t r = pack_bf2(v[0], v[1]);
+        __builtin_memcpy(q, &r, 4);
+    } else if constexpr (V == 2) {
+        const float2 r = make_float2(v[0], v[1]);
+        __builtin_memcpy(q, &r, 8);
+    } else if constexpr (sizeof(T) == 2) {
+        const uint2 r = make_uint2(pack_bf2(v[0], v[1]), pack_bf2(v[2], v[3]));
+        __builtin_memcpy(q, &r, 8);
+    } else {
+        const float4 r = make_float4(v[0], v[1], v[2], v[3]);
+        __builtin_memcpy(q, &r, 16);
+    }
 }
 template <int V>
 __device__ __forceinline__ void czero(float (&v)[V]) {
@@ -107,11 +131,13 @@ __device__ __forceinline__ void load_w(const ConvArgs& p, int d, float (&w)[W][V
     }
 }
 
+// 120 x 64 x 1024 bf16 10.5 us (3.0 TB/s), 1021 x 9 x 771 fp32 12.7 us (4.5 TB/s): bound by the three memory latencies that a
+// wave's run has one after the other (flags and window, steps, stores), of which too few waves are on the way at a time.
 template <typename T, int V, int W, bool WIDE>
 __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
     int d = (blockIdx.x * cg.L + threadIdx.x % cg.L) * V, run = blockIdx.z * (256 / cg.L) + threadIdx.x / cg.L;
-    const bool ok = d < p.D && run < cg.n_seg;                                 // idle lanes walk channel 0 or run 0 and write nothing
-    if (d >= p.D) d = 0;
+    const bool ok = d < p.D && run < cg.n_seg;                                 // idle lanes walk the last channels or run 0 and write nothing
+    d = min(d, (int)p.D - V);
     if (run >= cg.n_seg) run = 0;                                              // (a whole wave's, where it has one run)
     run = uniform<WIDE>(run);
     const int b = blockIdx.y, ta = run * cg.seg;
@@ -169,13 +195,13 @@ __global__ __launch_bounds__(256) void k_conv_fwd(ConvArgs p, ConvGrid cg) {
 
 // dx[tau] collects w[k] dpre[tau + W - 1 - k]: one walk forward in time with W open sums. A run emits its steps ta .. tb - 1
 // and goes W - 1 steps further for them; dw and db count its own steps only and stay in registers over all the runs that a
-// thread takes (every cg.rows-th).
+// thread takes (every cg.rows-th). Bound as the forward is, with half of its waves (the sums' registers).
 template <typename T, int V, int W, bool WIDE>
 __global__ __launch_bounds__(256) void k_conv_bwd(ConvArgs p, ConvGrid cg) {
     __shared__ float acc[W + 1][256 * V];
     const int lx = threadIdx.x % cg.L, ly = threadIdx.x / cg.L, per = 256 / cg.L;
-    const bool dv = (blockIdx.x * cg.L + lx) * V < p.D;                         // idle lanes walk channel 0 and write nothing
-    const int d = dv ? (blockIdx.x * cg.L + lx) * V : 0;
+    const bool dv = (blockIdx.x * cg.L + lx) * V < p.D;                         // idle lanes walk the last channels and write nothing
+    const int d = min((int)(blockIdx.x * cg.L + lx) * V, (int)p.D - V);
     float w[W][V], bias[V], dw[W][V], db[V];
     load_w<V, W>(p, d, w, bias);
 #pragma unroll
@@ -310,12 +336,13 @@ __global__ __launch_bounds__(1024) void k_conv_sum(const float* __restrict__ par
     }
 }
 
-// One step. A thread per V channels of a row.
+// One step. A thread per V channels of a row. Bound by memory: 4096 x 1024 bf16 12 us (5.5 TB/s).
 template <typename T, int V, int W>
 __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
-    const long long i = (((long long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x) * V;
-    if (i >= p.B * p.D) return;
-    const long long b = i / p.D, d = i - b * p.D;
+    const long long i = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * 256 + threadIdx.x, cv = (p.D + V - 1) / V;
+    if (i >= p.B * cv) return;
+    const long long b = i / cv, c = (i - b * cv) * V, d = min(c, p.D - V);
+    const int dup = (int)(c - d);           // the state changes in place: what the vector before has is not written twice
     T* s = (T*)p.state_out + b * (W - 1) * p.D + d;
     const bool rs = p.reset && p.reset[b] != 0;
     float row[W][V], w[W][V], v[V];
@@ -333,21 +360,40 @@ __global__ __launch_bounds__(256) void k_conv_step(ConvArgs p) {
         for (int k = 0; k < W; ++k) v[q] = fmaf(w[k][q], row[k][q], v[q]);
         if (p.silu) v[q] *= sigmoidf(v[q]);
     }
+    T* y = (T*)p.y + b * p.y_b + d;
+    if (dup == 0) {
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) cstore<T, V>(s + k * p.D, row[k + 1]);
-    cstore<T, V>((T*)p.y + b * p.y_b + d, v);
+        for (int k = 0; k < W - 1; ++k) cstore<T, V>(s + k * p.D, row[k + 1]);
+        cstore<T, V>(y, v);
+        return;
+    }
+#pragma unroll
+    for (int q = 1; q < V; ++q) {
+        if (q < dup) continue;
+#pragma unroll
+        for (int k = 0; k < W - 1; ++k) st(s + k * p.D + q, row[k + 1][q]);
+        st(y + q, v[q]);
+    }
 }
 
 static bool conv_ok(long long T, long long B, long long D, long long W) {
     return T > 0 && T <= 1000000 && B > 0 && B <= 65535 && T * B <= (1ll << 31) && D > 0 && D <= (1ll << 22) && W >= 2 && W <= 4;
 }
 
-// Runs of 8 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves: 120 x 64 x
-// 1 024 bf16 forward 11.3 us in runs of 8, 12.8 in runs of 16, 14.6 of 32. The backward walks W - 1 steps more than a run has:
-// its runs are that much short of 12 (below 1 024 waves: 30 x 64 x 256 11.8 us against 13.8), 18 (the above: 22.6 us against 30.2
-// with 12, whose partial rows are twice as many), 36 or 60. vec: V > 1.
-static ConvGrid conv_grid(long long T, long long B, long long D, bool vec, int extra) {
-    const long long cv = vec ? D / 4 : D;
+// channels a thread of the sequence kernels, see above; a single step has two (4 096 x 1 024: bf16 12 us against 14 with one and
+// 17 with four, fp32 21 against 23 with four)
+#define V_BF16 2
+#define V_F32 4
+#define V_STEP 2
+static long long conv_cols(long long D, int V) { return D < V ? D : (D + V - 1) / V; }
+static int conv_v(int bf16) { return bf16 ? V_BF16 : V_F32; }
+
+// Runs of 8 steps, longer ones (up to 64: fewer steps are read twice) where they still give the chip 4 096 waves: the forward of
+// 120 x 64 x 1024 bf16 takes 10.5 us in runs of 16 and 10.7 of 8. The backward walks W - 1 steps more than a run has: its
+// runs are that much short of 12 (below 1 024 waves), 18 (both passes of the above 29.5 us against 31.7 with 12), 36 or 60.
+// A block of the backward takes every rows-th run: 1 024 rows of partials at most (29.5 us; 512 33, 2 048 29.5).
+static ConvGrid conv_grid(long long T, long long B, long long D, int bf16, int extra) {
+    const long long cv = conv_cols(D, conv_v(bf16));
     int L = 1;
     while (L < cv && L < 256) L *= 2;
     const long long waves = (cv + L - 1) / L * L * B / 64;                    // of one run a row
@@ -361,20 +407,12 @@ static ConvGrid conv_grid(long long T, long long B, long long D, bool vec, int e
     return {L, seg, (int)n_seg, (int)rows};
 }
 
-// floats of scratch of a backward pass, whatever the alignment of its tensors
+// floats of scratch of a backward pass
 DRL_API int drl_short_conv_ws(long long T, long long B, long long D, long long W, long long* n) {
     if (!conv_ok(T, B, D, W)) return -1;
-    const int a = conv_grid(T, B, D, false, W - 1).rows, b = D % 4 ? 0 : conv_grid(T, B, D, true, W - 1).rows;
+    const int a = conv_grid(T, B, D, 0, (int)W - 1).rows, b = conv_grid(T, B, D, 1, (int)W - 1).rows;
     *n = (a > b ? a : b) * (W + 1) * D;
     return 0;
-}
-
-// whether 4 channels travel at once: every address and stride a multiple of their size
-static bool conv_vec(const ConvArgs& p, long long e, bool bwd) {
-    long long m = (long long)((uintptr_t)p.x | (uintptr_t)p.state_in | (uintptr_t)p.state_out) | ((p.x_t | p.x_b) * e);
-    m |= bwd ? (long long)((uintptr_t)p.dy | (uintptr_t)p.dx | (uintptr_t)p.dstate_in | (uintptr_t)p.dstate_out) | ((p.dy_t | p.dy_b | p.dx_t | p.dx_b) * e)
-             : (long long)(uintptr_t)p.y | ((p.y_t | p.y_b) * e);
-    return p.D % 4 == 0 && (m & (4 * e - 1)) == 0;
 }
 
 template <typename T, int V, int W, bool WIDE>
@@ -384,28 +422,27 @@ static void launch_conv(const ConvArgs& p, const ConvGrid& cg, bool bwd, dim3 gr
 }
 template <typename T, int V, int W>
 static void launch_conv_step(const ConvArgs& p, dim3 grid, hipStream_t s) { k_conv_step<T, V, W><<<grid, 256, 0, s>>>(p); }
-// F<T, V, W>(...) for the call's type, alignment and taps
+// F<T, V, W>(...) for the call's type, channels and taps
 #define CONV_W(F, T, V, ...)                                           \
     switch (p.W) {                                                      \
         case 2: F(T, V, 2, __VA_ARGS__); break;                         \
         case 3: F(T, V, 3, __VA_ARGS__); break;                         \
         default: F(T, V, 4, __VA_ARGS__); break;                        \
     }
-#define CONV_ALL(F, ...)                                                                                            \
-    if (bf16) { if (vec) { CONV_W(F, bf16_t, 4, __VA_ARGS__) } else { CONV_W(F, bf16_t, 1, __VA_ARGS__) } }         \
-    else { if (vec) { CONV_W(F, float, 4, __VA_ARGS__) } else { CONV_W(F, float, 1, __VA_ARGS__) } }
+#define CONV_ALL(F, VB, VF, ...)                                                                                            \
+    if (bf16) { if (p.D >= VB) { CONV_W(F, bf16_t, VB, __VA_ARGS__) } else { CONV_W(F, bf16_t, 1, __VA_ARGS__) } }         \
+    else { if (p.D >= VF) { CONV_W(F, float, VF, __VA_ARGS__) } else { CONV_W(F, float, 1, __VA_ARGS__) } }
 #define CONV_SEQ(T, V, W, BWD) cg.L >= 64 ? launch_conv<T, V, W, true>(p, cg, BWD, grid, s) : launch_conv<T, V, W, false>(p, cg, BWD, grid, s)
 #define CONV_ONE(T, V, W, _) launch_conv_step<T, V, W>(p, grid, s)
 
 DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(p.T, p.B, p.D, p.W)) return -1;
-    const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
-    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec, 0);
-    const long long cv = vec ? p.D / 4 : p.D, per = 256 / cg.L;
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, bf16, 0);
+    const long long cv = conv_cols(p.D, conv_v(bf16)), per = 256 / cg.L;
     if ((cg.n_seg + per - 1) / per > 65535) return -1;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)p.B, (unsigned)((cg.n_seg + per - 1) / per));
-    CONV_ALL(CONV_SEQ, false)
+    CONV_ALL(CONV_SEQ, V_BF16, V_F32, false)
     return (int)hipGetLastError();
 }
 
@@ -414,11 +451,10 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
     long long need;
     if (drl_short_conv_ws(p.T, p.B, p.D, p.W, &need)) return -1;
     if (p.ws_n < need) return -2;
-    const bool vec = conv_vec(p, bf16 ? 2 : 4, true);
-    const ConvGrid cg = conv_grid(p.T, p.B, p.D, vec, (int)p.W - 1);
-    const long long cv = vec ? p.D / 4 : p.D, n = (p.W + 1) * p.D;
+    const ConvGrid cg = conv_grid(p.T, p.B, p.D, bf16, (int)p.W - 1);
+    const long long cv = conv_cols(p.D, conv_v(bf16)), n = (p.W + 1) * p.D;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)cg.rows);
-    CONV_ALL(CONV_SEQ, true)
+    CONV_ALL(CONV_SEQ, V_BF16, V_F32, true)
     k_conv_sum<<<(unsigned)((n + 31) / 32), 1024, 0, s>>>(p.ws, cg.rows, (int)p.W, p.D, p.dw, p.db);
     return (int)hipGetLastError();
 }
@@ -426,11 +462,10 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
 DRL_API int drl_short_conv_step(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(1, 1, p.D, p.W) || p.B <= 0) return -1;
-    const bool vec = conv_vec(p, bf16 ? 2 : 4, false);
-    const long long nb = (p.B * p.D / (vec ? 4 : 1) + 255) / 256;
+    const long long nb = (p.B * conv_cols(p.D, V_STEP) + 255) / 256;
     if (nb >= 1ll << 38) return -1;
     const long long x = nb < (1 << 23) ? nb : 1 << 23;
     const dim3 grid((unsigned)x, (unsigned)((nb + x - 1) / x));
-    CONV_ALL(CONV_ONE, 0)
+    CONV_ALL(CONV_ONE, V_STEP, V_STEP, 0)
     return (int)hipGetLastError();
 }

@@ -122,7 +122,7 @@ def check_conv(v, silu=True):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("T,B,D,W", [(1, 1, 1, 4), (1, 3, 5, 2), (2, 4, 64, 4), (3, 2, 16, 4), (15, 3, 7, 3), (16, 2, 256, 4), (17, 5, 8, 4),
-                                     (31, 3, 130, 2), (33, 2, 264, 3), (65, 4, 40, 4)])
+                                     (31, 3, 130, 2), (33, 2, 264, 3), (65, 4, 40, 4), (4, 3, 2, 4), (9, 3, 3, 2), (40, 2, 515, 3), (19, 2, 1027, 4)])
 def test_conv(T, B, D, W, dtype):
     check_conv(conv_case(T, B, D, W, dtype))
 
@@ -168,7 +168,24 @@ def test_conv_in_pieces_and_in_steps_is_the_whole(dtype):
     assert torch.equal(st, whole["state_out"])
 
 
-@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (5, 33, 3), (3, 1024, 4), (257, 40, 4)])
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("D", [1, 3, 7, 510, 1025])
+def test_conv_writes_nothing_beside_its_rows(D, dtype):
+    T, B, W, g = 21, 3, 4, Gen(D)
+    x, w, dy = g.n(T, B, D + 5, dtype=dtype)[..., 2:D + 2], g.n(D, W), g.n(T, B, D, dtype=dtype)
+    y, dx = (torch.full((T, B, D + 7), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+    dw, ref, rx = torch.empty_like(w), torch.empty_like(dy), torch.empty_like(dy)
+    ws = H.short_conv_ws(T, B, D, W, DEV)
+    H.short_conv_fwd(x, w, None, y[..., 3:D + 3])
+    H.short_conv_bwd(dy, x, w, None, dx[..., 3:D + 3], dw, None, ws)
+    H.short_conv_fwd(x.contiguous(), w, None, ref)
+    H.short_conv_bwd(dy, x.contiguous(), w, None, rx, dw, None, ws)
+    for got, want in ((y, ref), (dx, rx)):
+        assert torch.equal(got[..., 3:D + 3], want)
+        assert bool((got[..., :3] == 7).all()) and bool((got[..., D + 3:] == 7).all())
+
+
+@pytest.mark.parametrize("B,D,W", [(1, 1, 2), (5, 33, 3), (3, 1024, 4), (257, 40, 4), (150, 257, 4), (3, 2, 2)])
 def test_conv_step_strided(B, D, W):
     g = Gen(B + D)
     wide = g.n(B, 2 * D + 3, dtype=BF)
