@@ -16,13 +16,12 @@ struct NormArgs {        // mirrored by ops/hip.py (_NORM): 64-bit words in this
     long long ws_n;
 };
 
-// A team of L lanes (4, 16, or 64 x TW waves) owns a row and keeps it in registers, 16 values a lane at most: one read, the
+// A team of L lanes (4 to 64, or 64 x TW of TW waves) owns a row and keeps it in registers, NV vectors a lane: one read, the
 // mean, the spread around it, one write. V values (16 bytes) travel per load. AL: every vector lies at a multiple of 16 bytes
 // and D is a multiple of V; otherwise vectors start anywhere (the memory system takes them), and a row's last one ends at the
 // row's end: its first `dup` columns are the vector before's, left out of the sums and stored twice with the same value.
-// Bound by memory. Forward and backward of 20 M values, a wave a row and one value a load where nothing is aligned -> this:
-// bf16 D = 17 875 -> 115 us, 100 240 -> 80, 511 176 -> 73, 2047 177 -> 73, 4001 199 -> 81; fp32 769 -> 278, 150 -> 153,
-// 121 -> 95, 113 -> 92, 110 -> 100. Aligned: bf16 512 55 us (3.7 TB/s), fp32 512 83, 4096 88 (4.6 to 4.8 TB/s).
+// Bound by memory. Forward and backward of 10 M values, bf16 / fp32: D = 17 55 / 86 us, 40 33 / 58, 100 36 / 51, 130 41 / 59,
+// 256 28 / 45, 350 36 / 53, 511 37 / 47, 768 30 / 46; of 20 M values 512 55 / 83, 4001 81 / 100, 4096 69 / 88 (4.6 TB/s).
 template <typename T, int V, bool AL>
 __device__ __forceinline__ void load_v(const T* q, int n, float (&v)[V]) {
     if (AL || n >= V) {
@@ -279,12 +278,19 @@ __global__ __launch_bounds__(1024) void k_norm_sum(const float* __restrict__ par
 }
 
 static bool norm_ok(long long M, long long D) { return M > 0 && M < (1ll << 31) && D > 0 && D <= 16384; }
-// Lanes and vectors of a row's team: the fewest lanes with at most 16 values each, so that short rows share a wave.
+// Lanes and vectors of a row's team: as few idle lanes as the powers of two allow, one vector a lane where they are full, three
+// where that saves a quarter of them (10 M fp32 values: D = 130 59 us with 3 x 16 lanes, 92 with 64; 17 86 with 8, 144 with
+// 16), four waves beyond 1 024 columns and 16 beyond 4 096.
 struct Team { int L, TW, NV; };
 static Team team_of(long long D, int V) {
     const long long n = (D + V - 1) / V;               // vectors a row
     if (n <= 4) return {4, 1, 1};
-    if (n <= 32 && (V == 8 || n <= 16)) return {16, 1, n <= 16 ? 1 : 2};
+    if (n <= 8) return {8, 1, 1};
+    if (n <= 16) return {16, 1, 1};
+    if (n <= 24) return {8, 1, 3};
+    if (n <= 32) return {32, 1, 1};
+    if (n <= 48) return {16, 1, 3};
+    if (n > 64 && n <= 96) return {32, 1, 3};
     const int TW = D <= 1024 ? 1 : D <= 4096 ? 4 : 16;
     const int nv = (int)((n + 64 * TW - 1) / (64 * TW));
     return {64, TW, nv > 2 ? 4 : nv};
@@ -328,10 +334,9 @@ template <typename T, bool AL>
 static void norm_team(const NormArgs& p, bool bwd, float eps, hipStream_t s) {
     const Team t = team_of(p.D, 16 / sizeof(T));
     if (t.L == 4) return norm_launch<T, 1, 4, 1, AL>(p, bwd, eps, s);
-    if (t.L == 16) {
-        if constexpr (sizeof(T) == 2) { if (t.NV == 2) return norm_launch<T, 2, 16, 1, AL>(p, bwd, eps, s); }
-        return norm_launch<T, 1, 16, 1, AL>(p, bwd, eps, s);
-    }
+    if (t.L == 8) return t.NV == 1 ? norm_launch<T, 1, 8, 1, AL>(p, bwd, eps, s) : norm_launch<T, 3, 8, 1, AL>(p, bwd, eps, s);
+    if (t.L == 16) return t.NV == 1 ? norm_launch<T, 1, 16, 1, AL>(p, bwd, eps, s) : norm_launch<T, 3, 16, 1, AL>(p, bwd, eps, s);
+    if (t.L == 32) return t.NV == 1 ? norm_launch<T, 1, 32, 1, AL>(p, bwd, eps, s) : norm_launch<T, 3, 32, 1, AL>(p, bwd, eps, s);
 #define NORM_NV(TW)                                                                                                   \
     if (t.NV == 1) return norm_launch<T, 1, 64, TW, AL>(p, bwd, eps, s);                                              \
     if constexpr (sizeof(T) == 4) { if (t.NV == 4) return norm_launch<T, 4, 64, TW, AL>(p, bwd, eps, s); }            \

@@ -44,19 +44,15 @@ template <int CTRL>
 __device__ __forceinline__ float add_dpp(float v) {
     return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(v), CTRL, 0xf, 0xf, true));
 }
-// sum over groups of L = 4, 16 or 64 neighbouring lanes, in every lane: adds across neighbours, then row swaps, no trip
+// sum over groups of L = 4, 8, 16, 32 or 64 neighbouring lanes, in every lane: adds across neighbours, then row swaps, no trip
 // through LDS
 template <int L>
 __device__ __forceinline__ float lane_sum(float v) {
     v = add_dpp<0xB1>(v);                              // quad: lane ^ 1
     v = add_dpp<0x4E>(v);                              // quad: lane ^ 2
-    if constexpr (L > 4) {
-        v = add_dpp<0x141>(v);                         // row_half_mirror: the other quad of 8 lanes
-        v = add_dpp<0x140>(v);                         // row_mirror: the other 8 lanes
-    }
-    if constexpr (L > 16) {
-        v = add_swap16(v, v);
-        v = add_swap32(v, v);
-    }
+    if constexpr (L > 4) v = add_dpp<0x141>(v);        // row_half_mirror: the other quad of 8 lanes
+    if constexpr (L > 8) v = add_dpp<0x140>(v);        // row_mirror: the other 8 lanes
+    if constexpr (L > 16) v = add_swap16(v, v);
+    if constexpr (L > 32) v = add_swap32(v, v);
     return v;
 }

@@ -57,7 +57,8 @@ def check_norm(v, eps=1e-5):
 
 @pytest.mark.parametrize("dtype", [F32, BF])
 @pytest.mark.parametrize("M,D", [(1, 1), (3, 2), (1, 512), (5, 63), (4, 64), (7, 100), (257, 8), (33, 513), (9, 1024), (6, 1032), (5, 3136),
-                                 (2, 4099), (3, 8192), (2, 16384), (1030, 40)])
+                                 (2, 4099), (3, 8192), (2, 16384), (1030, 40),
+                                 (70, 20), (35, 29), (41, 70), (37, 93), (19, 100), (21, 130), (23, 185), (9, 270), (11, 381), (5, 600), (3, 765)])
 def test_norm(M, D, dtype):
     g = Gen(M * 31 + D)
     check_norm(dict(x=g.n(M, D, dtype=dtype, scale=2.0, shift=0.7), w=g.n(D, shift=1.0), b=g.n(D), dy=g.n(M, D, dtype=dtype)))
