@@ -1021,7 +1021,7 @@ def add2(a, b, out) -> None:
 # streams, two graphs) need one each.
 _NORM, _CONV, _SSM = (struct.Struct("<%dq" % n) for n in (18, 29, 56))
 _NORM_FWD, _CONV_FWD, _SSM_FWD = (struct.Struct("<%dq%dx" % (n, 8 * m)) for n, m in ((10, 8), (17, 12), (33, 23)))        # the rest zero
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # (torch without GPU support: no GPU tensors either)
 
 
 def _dev(t: torch.Tensor) -> int:
