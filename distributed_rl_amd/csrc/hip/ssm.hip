@@ -375,7 +375,7 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
     }
 }
 
-// 120 x 64 x 1024 bf16, 16 states: 40 us (45 under a profiler, its vector units 92 % busy there), 1.6 TB/s; 32 states 68 us, 4
+// 120 x 64 x 1024 bf16, 16 states: 40 to 45 us, its vector units busy 88 % of the time, 1.6 TB/s; 32 states 68 us, 4
 // states 28 us.
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const float* __restrict__ carry) {
@@ -486,7 +486,8 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
 // Backward. g_t = C ds + a_{t+1} g_{t+1} runs against the time; the states it needs are recomputed chunk by chunk from the
 // saved ones and kept in registers (16 steps x NS, next to the decays). The sums over channels of dB and dC leave as partials
 // of 64 channels (a block), the sums over rows of dA, dD and the bias as partials of a row: a second launch adds them in a
-// fixed order. 120 x 64 x 1024 bf16, 16 states, resets and lengths of 30 .. 120: 99 to 105 us, vector units 86 % busy.
+// fixed order. 120 x 64 x 1024 bf16, 16 states, resets and lengths of 30 .. 120: 99 to 105 us, vector units busy 74 % of the
+// time with two waves a SIMD. Three fit 168 registers only with spills or with LDS reads one step at a time: 3 to 8 % slower.
 //
 // KH steps of a chunk, s0 .. s0 + KH - 1, from the state before them: forward with the states and decays kept, then back.
 // mid() is called half way back, when half of those registers are free again: the next chunk's loads start there. emit(s, gB, wA)
