@@ -495,7 +495,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
 template <int NS, int KH, bool RS, typename F, typename E>
 __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const float* bcb, float* red_w, unsigned rm, int s0, int g, int j,
                                           const float (&An)[NS], float (&hs)[KH + 1][NS], float (&G)[NS], float (&dAc)[NS],
-                                          float4 (&ex_w)[KC][16], F mid, E emit) {
+                                          float (&y_w)[KC][16], F mid, E emit) {
     constexpr int NP = 4 * NS;
     // What a step reads from LDS. Forward a step ahead; back as it is needed: two steps ahead took registers that 32 states do
     // not have (120 x 64 x 1024 both passes 340 us, so 297) and gained nothing with fewer.
@@ -525,7 +525,7 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
             acc = fmaf(x.C[i], hs[k + 1][i], acc);
         }
         part[k & 3] = acc;
-        if ((k & 3) == 3) ex_w[s - 3 + g][j].w = sum_groups(part[0], part[1], part[2], part[3]);
+        if ((k & 3) == 3) y_w[s - 3 + g][j] = sum_groups(part[0], part[1], part[2], part[3]);
         if (k + 1 < KH) x = nx;
     }
     int again = 0;                                  // hides that B, C and the step's scalars are read a second time:
@@ -579,7 +579,8 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
     constexpr int KH = NS > 4 ? 4 : 8;                      // steps whose states are held at a time
     using R = Rows<T>;
     __shared__ __align__(16) float4 pw_s[4][KC][16];        // s log2(e), s u, ds, u
-    __shared__ __align__(16) float4 ex_s[4][KC][16];        // dy silu'(z), -, ds/d(pre), sum_n C h
+    __shared__ __align__(16) float2 ex_s[4][KC][16];        // dy silu'(z), ds/d(pre)
+    __shared__ float y_s[4][KC][16];                        // sum_n C h
     __shared__ __align__(16) float bc_s[2][KC * 2 * NP];
     __shared__ __align__(16) float red_s[2][4][KC * 2 * NP];
     const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, j = lane & 15;
@@ -672,7 +673,7 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
                 const float u = R::value(ru[i]);
                 sp[i] = dv && t0 + 4 * i + g < end ? sp[i] : 0.f;
                 pw_s[w][4 * i + g][j] = make_float4(sp[i] * LOG2E, sp[i] * u, ds[i], u);
-                ex_s[w][4 * i + g][j] = make_float4(dz[i], 0.f, sg[i], 0.f);
+                ex_s[w][4 * i + g][j] = make_float2(dz[i], sg[i]);
             }
         }
         float* bcb = bc_s[c & 1];
@@ -692,21 +693,23 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int 
         for (int i = 0; i < NS; ++i) dAc[i] = 0.f;
         float* red = red_s[c & 1][w];
         auto emit = [&](int s, float gB, float wA) {
-            const float4 pw = pw_s[w][s + g][j], ex = ex_s[w][s + g][j];
+            const float4 pw = pw_s[w][s + g][j];
+            const float2 ex = ex_s[w][s + g][j];
+            const float yq = y_s[w][s + g][j];
             const int t = t0 + s + g;
-            const float dpre = t < end ? fmaf(pw.w, gB, wA) * ex.z : 0.f;
+            const float dpre = t < end ? fmaf(pw.w, gB, wA) * ex.y : 0.f;
             dDc = fmaf(pw.z, pw.w, dDc);
             dbc += dpre;
             const unsigned bad = dv && t < n_t ? 0u : OOB;
             R::store(wu.rsrc(), odu | bad, (unsigned)(s / 4) * wu.four, t < end ? fmaf(Dd, pw.z, pw.x * LN2 * gB) : 0.f);
             R::store(wd.rsrc(), odd | bad, (unsigned)(s / 4) * wd.four, dpre);
-            if (has_z) R::store(wz.rsrc(), odz | bad, (unsigned)(s / 4) * wz.four, t < end ? ex.x * fmaf(Dd, pw.w, ex.w) : 0.f);
+            if (has_z) R::store(wz.rsrc(), odz | bad, (unsigned)(s / 4) * wz.four, t < end ? ex.x * fmaf(Dd, pw.w, yq) : 0.f);
         };
         auto from = [&](const float (&h)[NS]) {
 #pragma unroll
             for (int i = 0; i < NS; ++i) hs[0][i] = h[i];
         };
-        auto piece = [&](int s0, auto mid) { bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, ex_s[w], mid, emit); };
+        auto piece = [&](int s0, auto mid) { bwd_piece<NS, KH, HAS>(pw_s[w], bcb, red, rm, s0, g, j, An, hs, G, dAc, y_s[w], mid, emit); };
         auto nothing = [] {};
         const bool half = t0 + SAVE >= live;                // the row ends in the chunk's first half: the other is zeros
         if (half) {
