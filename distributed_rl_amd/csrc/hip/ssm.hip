@@ -571,9 +571,10 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
     }
 }
 
+// Four waves a SIMD for up to 8 states: 120 x 64 x 1024 both passes 130 -> 117 us, though the form with resets spills 7 registers.
 // HAS: the call has reset flags. (A branch on each chunk's flags instead holds the registers of both paths: spills.)
 template <typename T, int NS, bool HAS>
-__global__ __launch_bounds__(256, NS > 8 ? 1 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
+__global__ __launch_bounds__(256, NS > 8 ? 1 : NS == 2 ? 4 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
                                                     float* __restrict__ part_bc, float* __restrict__ part_a) {
     constexpr int NP = 4 * NS;
     constexpr int KH = NS > 4 ? 4 : 8;                      // steps whose states are held at a time
