@@ -1290,6 +1290,7 @@ def _ssm_args(u, dt, A, Bm, Cm, D, z, dt_bias, softplus, reset, lengths, y=None,
         raise ValueError("ssm_scan: unsupported sizes: u must be [T, B, D], Bm [T, B, N], N <= 64 (got %s, %s)" % (tuple(shape), tuple(bc)))
     T, B, Dc = shape
     N = bc[2]
+    bc = (T, B, N)                          # u's steps and rows, for Bm too
     dev, typ, f32 = _dev(u), u.dtype, torch.float32
     bf16, st, ld, lb, dn, d, n_ws = _typ(u), (B, Dc, N), (B * Dc, Dc), (B * N, N), (Dc, N), (Dc,), ws.numel()
     up, ut, ub = _rows3(u, shape, ld, typ, dev, "u")

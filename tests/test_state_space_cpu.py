@@ -164,3 +164,30 @@ def test_rows_of_outputs_may_not_overlap():
     with pytest.raises(ValueError, match="shares"):
         hip._apart((8, 8), ())
     hip._apart((8, 16, 0, 0), (0, 24))
+
+
+# ---- refusals past the device check: _dev is told that the CPU is the current GPU, and the arguments are only packed ----------
+def scan_args(T=50, B=4, D=8, N=4, backward=False, **kw):
+    z = lambda *s: torch.zeros(*s)                                          # noqa: E731
+    a = dict(u=z(T, B, D), dt=z(T, B, D), A=z(D, N), Bm=z(T, B, N), Cm=z(T, B, N), D=None, z=None, dt_bias=None, softplus=True, reset=None,
+             lengths=None, ws=z(64))
+    a.update(dict(y=z(T, B, D)) if not backward else
+             dict(ckpt=z((T + 7) // 8, B, D, N), dy=z(T, B, D), du=z(T, B, D), ddt=z(T, B, D), dA=z(D, N), dB=z(T, B, N), dC=z(T, B, N)))
+    a.update(kw)
+    return hip._ssm_args(**a)
+
+
+@pytest.mark.parametrize("backward", [False, True])
+def test_scan_coefficients_of_other_sizes_than_the_sequence_are_refused(monkeypatch, backward):
+    monkeypatch.setattr(hip, "_dev", lambda t: t.get_device())
+    scan_args(backward=backward)
+    grads = ("dB", "dC") if backward else ()
+    for shape in ((3, 1, 4), (50, 1, 4), (1, 4, 4), (49, 4, 4), (51, 4, 4), (50, 3, 4), (50, 5, 4), (4, 50, 4), (50, 4, 3)):
+        both = {k: torch.zeros(shape) for k in ("Bm", "Cm") + grads}
+        with pytest.raises(ValueError):                     # all of them alike: they agree with each other, not with u
+            scan_args(backward=backward, **both)
+        for k in both:
+            with pytest.raises(ValueError):
+                scan_args(backward=backward, **{k: both[k]})
+    batch_major = {k: torch.zeros(4, 50, 4).transpose(0, 1) for k in ("Bm", "Cm") + grads}
+    scan_args(backward=backward, **batch_major)             # a transpose of the right shape is fine
