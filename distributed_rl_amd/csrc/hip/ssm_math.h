@@ -13,9 +13,11 @@ __device__ __forceinline__ void st(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
 
 // exp(-|x|) by the hardware's 2^y: the part of x * log2(e) that its 24 bits lose comes back as a factor 1 + lost * ln 2
-// (without it the relative error grows with |x|: 4e-7 at 7, where a step size of 0.001 sits)
+// (without it the relative error grows with |x|: 4e-7 at 7, where a step size of 0.001 sits). From 128 on the result is 0; the
+// argument stops there (a NaN passes), as the product would leave the range with it and what it lost be no number: a step of
+// size -inf or of the type's lowest value holds the state.
 __device__ __forceinline__ float exp_neg_abs(float x) {
-    const float ax = -fabsf(x), hi = ax * LOG2E;
+    const float mx = -fabsf(x), ax = mx < -128.f ? -128.f : mx, hi = ax * LOG2E;
     const float lo = fmaf(ax, LOG2E, -hi) + ax * LOG2E_LO;
     const float p = __builtin_amdgcn_exp2f(hi);
     return fmaf(p, lo * LN2, p);

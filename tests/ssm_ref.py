@@ -154,3 +154,104 @@ def norm(v, eps=1e-5, mag=False):
         a, c = dn.mean(-1, keepdim=True), n * (dn * n).mean(-1, keepdim=True)
         out.update(dx=(dn + a + c if mag else dn - a - c) * rstd, dw=(dy * n).sum(0), db=dy.sum(0))
     return out
+
+
+def scan_bounds(v, softplus=True, cut=False):
+    """How far each output of the scan may be off before it is rounded to its type, counted along the recurrences, so that what
+    has decayed no longer counts: beside the magnitude M of a state or of its gradient runs its error E, and both fade by the
+    same decay. In half steps e = 2^-24: a step size is off by 14 + |pre| of itself (sum, exp, log1p), a decay by 4 (exp, its
+    product) and by its exponent times the 17 + |pre| of that (A log2(e), its product), a gate by 8 + 3 |z|, a product by 1 and a
+    sum of n terms by n + 6. ``cut``: the time may be cut into joined segments, whose summed step sizes take up to T / 4 + 3 more."""
+    e = 2.0 ** -24
+    T, B, Dc = v["u"].shape
+    A, N = v["A"], v["A"].shape[1]
+    zero = torch.zeros(Dc, dtype=torch.float64)
+    Dp, bias = (zero if v.get(k) is None else v[k] for k in ("D", "dt_bias"))
+    end = v["lengths"].clamp(0, T) if v.get("lengths") is not None else torch.full((B,), T)
+    live = torch.arange(T)[:, None] < end[None]
+    lv = lambda x: torch.where(live[..., None], x, 0.0)                       # noqa: E731
+    u, Bm, Cm, dtv = (lv(v[k]) for k in ("u", "Bm", "Cm", "dt"))
+    u, Bm, Cm = u.abs(), Bm.abs(), Cm.abs()
+    pre = dtv + bias
+    if softplus:
+        s, sg = pre.clamp(min=0) + torch.log1p(torch.exp(-pre.abs())), torch.sigmoid(pre)
+    else:
+        s, sg = pre, torch.ones_like(pre)
+    s, sg = lv(s), lv(sg)
+    ap = pre.abs().clamp(max=200.0)                           # beyond, a softplus is 0 or the sum itself
+    rs = (14 + ap) * e
+    x = s[..., None] * A
+    a = torch.exp(x)
+    ra = (4 + x.abs() * (17 + ap + (T / 4 + 3 if cut else 0))[..., None]) * e
+    s = s.abs()
+    keep = torch.ones(T, B) if v.get("reset") is None else (v["reset"] == 0).double()
+    if v.get("z") is not None:
+        z = lv(v["z"])
+        sz = torch.sigmoid(z)
+        gate, dgate = (z * sz).abs(), sz * (1 + z.abs() * (1 - sz))
+        rg = (8 + 3 * z.abs()) * e
+        e_dgate = (rg + 6 * e) * dgate + z.abs() * sz * sz * rg
+    else:
+        gate, dgate, rg, e_dgate = torch.ones_like(u), torch.zeros_like(u), torch.zeros_like(u), torch.zeros_like(u)
+    h = v["h0"].abs() if v.get("h0") is not None else torch.zeros(B, Dc, N, dtype=torch.float64)
+    eh = torch.zeros_like(h)
+    hs, ehs, olds, eolds, qs, eqs = [], [], [], [], [], []
+    for t in range(T):
+        ok, k = live[t][:, None, None], keep[t][:, None, None]
+        old, eold = h * k, eh * k
+        add = (s[t] * u[t])[..., None] * Bm[t][:, None]
+        new = a[t] * old + add
+        enew = a[t] * (eold + ra[t] * old) + (rs[t] + 3 * e)[..., None] * add + e * new
+        h, eh = torch.where(ok, new, h), torch.where(ok, enew, eh)
+        hs.append(h), ehs.append(eh)
+        olds.append(torch.where(ok, old, 0.0)), eolds.append(torch.where(ok, eold, 0.0))
+        q = (h * Cm[t][:, None]).sum(-1) + (Dp * u[t]).abs()
+        qs.append(q), eqs.append((eh * Cm[t][:, None]).sum(-1) + (N + 6) * e * q)
+    q, eq = torch.stack(qs), torch.stack(eqs)
+    out = {"y": lv(gate * eq + (rg + 3 * e) * gate * q), "hT": eh}
+    if v.get("dy") is None:
+        return {k: 1.01 * x for k, x in out.items()}          # products of two errors
+    dy = lv(v["dy"]).abs()
+    ds, rds = dy * gate, rg + 2 * e
+    G = v["dhT"].abs() if v.get("dhT") is not None else torch.zeros_like(h)
+    eG = torch.zeros_like(G)
+    r = {k: [None] * T for k in ("du", "ddt", "dB", "dC")}
+    dA, mA = torch.zeros_like(A), torch.zeros_like(A)
+    mdt = []
+    for t in range(T - 1, -1, -1):
+        ok, k = live[t][:, None, None], keep[t][:, None, None]
+        cds = ds[t][..., None] * Cm[t][:, None]
+        g = G + cds
+        eg = eG + rds[t][..., None] * cds + e * g
+        gB = (g * Bm[t][:, None]).sum(-1)
+        egB = (eg * Bm[t][:, None]).sum(-1) + (N + 6) * e * gB
+        r["du"][t] = (Dp * ds[t]).abs() * (rds[t] + 2 * e) + s[t] * (egB + (rs[t] + 3 * e) * gB)
+        w = g * a[t] * olds[t]
+        ew = a[t] * (eg * olds[t] + g * eolds[t] + (ra[t] + 2 * e) * g * olds[t])
+        wA = (w * A.abs()).sum(-1)
+        ewA = (ew * A.abs()).sum(-1) + (N + 6) * e * wA
+        m = wA + u[t] * gB
+        r["ddt"][t] = sg[t] * (ewA + u[t] * egB + (11 + ap[t]) * e * m)
+        mdt.append(sg[t] * m)
+        su = s[t] * u[t]
+        r["dB"][t] = (eg * su[..., None] + g * ((rs[t] + 2 * e) * su)[..., None] + (Dc + 8) * e * g * su[..., None]).sum(1)
+        r["dC"][t] = (ehs[t] * ds[t][..., None] + hs[t] * ((rds[t] + (Dc + 9) * e) * ds[t])[..., None]).sum(1)
+        dA = dA + (ew * s[t][..., None] + w * ((rs[t] + 2 * e) * s[t])[..., None]).sum(0)
+        mA = mA + (w * s[t][..., None]).sum(0)
+        G, eG = torch.where(ok, g * a[t] * k, G), torch.where(ok, a[t] * (eg + (ra[t] + e) * g) * k, eG)
+    out.update({k: torch.stack(x) for k, x in r.items()})
+    n = (T + B + 80) * e                                      # sums over the steps of a row, then over rows and segments
+    out.update(dz=dy * (eq * dgate + q * e_dgate + 3 * e * q * dgate), dA=dA + n * mA,
+               dD=((rds + 2 * e + n) * ds * u).sum((0, 1)), ddt_bias=out["ddt"].sum((0, 1)) + n * torch.stack(mdt).sum((0, 1)), dh0=eG)
+    return {k: 1.01 * x for k, x in out.items()}
+
+
+def within(got, ref, bound, name=""):
+    """|got - ref| <= bound + half a step of got's type."""
+    half = torch.finfo(got.dtype).eps / 2
+    got = got.detach().cpu().double()
+    assert got.shape == ref.shape, (name, got.shape, ref.shape)
+    tol = bound + half * (ref.abs() + bound) + 1e-37
+    bad = ~((got - ref).abs() <= tol)
+    assert not bad.any(), "%s: %d of %d outside, worst %.3g of its tolerance" % (
+        name, int(bad.sum()), bad.numel(), float(((got - ref).abs() / tol)[bad].max()))

@@ -385,6 +385,55 @@ def test_step_of_views():
     assert torch.equal(y[:, :D], y2) and torch.equal(h, h2) and bool((y[:, D:] == 7).all())
 
 
+# ---- steps that are held, states that diverged, factors of a segment that leave the range -------------------------------------
+def check_scan_tight(v, softplus=True, w=None):
+    """Against bounds that fade as the states do. ``w``: the values in 64 bits, where they are not all finite."""
+    got = run_scan(v, softplus)
+    w = clean(v) if w is None else w
+    ref, tol = ssm_ref.scan(w, softplus), ssm_ref.scan_bounds(w, softplus, cut=w["u"].shape[0] > 112)
+    for k in got:
+        ssm_ref.within(got[k], ref[k], tol[k], k)
+    return got
+
+
+LOWEST = [float("-inf"), torch.finfo(BF).min, -2.37e38, -129.0]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("low", LOWEST)
+@pytest.mark.parametrize("T,B,D,N", [(21, 4, 20, 16), (40, 2, 24, 40), (600, 2, 16, 8)])
+def test_scan_holds_its_state_over_steps_of_the_lowest_size(T, B, D, N, low, dtype):
+    v = scan_case(T, B, D, N, dtype, reset=0.02)
+    held = Gen(T).u(T, B) < 0.3
+    v["dt"][held] = low
+    w = clean(v)
+    w["dt"][held.cpu()] = low                                                       # clean() takes infinities out
+    got = check_scan_tight(v, w=w)
+    assert bool((got["ddt"][held] == 0).all())
+
+
+@pytest.mark.parametrize("T,B,D", [(40, 2, 24), (600, 2, 16)])
+def test_scan_takes_no_nan_for_a_held_step(T, B, D):
+    v = scan_case(T, B, D, 16, F32, reset=0, ragged=False)
+    v["dt"][T // 2, 0] = float("nan")
+    y = run_scan(v)["y"]
+    assert bool(y[T // 2:, 0].isnan().all()) and not bool(y[:T // 2].isnan().any()) and not bool(y[:, 1:].isnan().any())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("low", LOWEST + [torch.finfo(F32).min])
+@pytest.mark.parametrize("B,D,N", [(3, 17, 16), (4, 9, 5), (2, 70, 64)])
+def test_step_of_the_lowest_size_leaves_the_state(B, D, N, low, dtype):
+    v = scan_case(1, B, D, N, dtype, ragged=False, reset=0)
+    h, y = v["h0"].clone(), torch.empty(B, D, dtype=dtype, device=DEV)
+    dt = torch.full_like(v["dt"][0], low, dtype=F32).to(dtype)                      # (fp32's lowest value is -inf in bf16)
+    H.ssm_step(v["u"][0], dt, v["A"], v["Bm"][0], v["Cm"][0], h, y, D=v["D"], z=v["z"][0], dt_bias=v["dt_bias"])
+    assert torch.equal(h, v["h0"])
+    w = clean({k: x for k, x in v.items() if k not in ("dy", "dhT")})
+    w["dt"] = torch.full_like(w["dt"], low)
+    ssm_ref.within(y, ssm_ref.scan(w)["y"][0], ssm_ref.scan_bounds(w)["y"][0], "y")
+
+
 # ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
 def test_norm_past_32_bits():
     M, D = 150000, 16384                                    # 2.46e9 elements
