@@ -492,11 +492,16 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
 // KH steps of a chunk, s0 .. s0 + KH - 1, from the state before them: forward with the states and decays kept, then back.
 // mid() is called half way back, when half of those registers are free again: the next chunk's loads start there. emit(s, gB, wA)
 // gets the sums over the states for the lane's own step of each four that are done (s = their first).
+//
+// A reset chooses zeros for what passes it, the state forward and its gradient back: a factor of zero would make NaN of an
+// episode that diverged on the other side. By a select for each state, or from 17 states on by one branch a step (120 x 64 x
+// 1024 with resets, both passes, selects and branch: 4 states 81.0 and 84.1 us, 32 states 319 and 307, 64 states 772 and 759).
 template <int NS, int KH, bool RS, typename F, typename E>
 __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const float* bcb, float* red_w, unsigned rm, int s0, int g, int j,
                                           const float (&An)[NS], float (&hs)[KH + 1][NS], float (&G)[NS], float (&dAc)[NS],
                                           float (&y_w)[KC][16], F mid, E emit) {
     constexpr int NP = 4 * NS;
+    constexpr bool BRANCH = RS && NS > 4;
     // What a step reads from LDS. Forward a step ahead; back as it is needed: two steps ahead took registers that 32 states do
     // not have (120 x 64 x 1024 both passes 340 us, so 297) and gained nothing with fewer.
     struct In { float4 pw; float B[NS], C[NS]; };
@@ -520,7 +525,7 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const float e = __builtin_amdgcn_exp2f(x.pw.x * An[i]), in = x.pw.y * x.B[i], n = fmaf(e, hs[k][i], in);
-            a[k][i] = rs ? 0.f : e;
+            a[k][i] = e;
             hs[k + 1][i] = rs ? in : n;
             acc = fmaf(x.C[i], hs[k + 1][i], acc);
         }
@@ -542,17 +547,31 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
             const int c = (k + o) & 3;
             const float4 pw = xs[o].pw;
             pb[c] = 0.f; pa[c] = 0.f;
+            const bool rs = RS && (rm >> (s0 + k + o) & 1);
+            const auto back = [&](int i, float gh, bool cut) {  // through the decay, to the step before
+                const float q = gh * a[k + o][i], y = cut ? 0.f : q * hs[k + o][i];
+                G[i] = cut ? 0.f : q;
+                pa[c] = fmaf(y, An[i], pa[c]);
+                dAc[i] = fmaf(y, pw.x, dAc[i]);
+                pin(dAc[i]);
+            };
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const float gh = fmaf(pw.z, xs[o].C[i], G[i]);
                 vB[o][i] = gh * pw.y;
                 vC[o][i] = pw.z * hs[k + o + 1][i];
                 pb[c] = fmaf(gh, xs[o].B[i], pb[c]);
-                const float q = gh * a[k + o][i], y = q * hs[k + o][i];
-                G[i] = q;
-                pa[c] = fmaf(y, An[i], pa[c]);
-                dAc[i] = fmaf(y, pw.x, dAc[i]);
-                pin(dAc[i]);
+                if constexpr (BRANCH) G[i] = gh;
+                else back(i, gh, rs);
+            }
+            if constexpr (BRANCH) {
+                if (rs) {
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) G[i] = 0.f;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NS; ++i) back(i, G[i], false);
+                }
             }
             pin(pb[c]); pin(pa[c]);
         }

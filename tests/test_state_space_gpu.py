@@ -434,6 +434,27 @@ def test_step_of_the_lowest_size_leaves_the_state(B, D, N, low, dtype):
     ssm_ref.within(y, ssm_ref.scan(w)["y"][0], ssm_ref.scan_bounds(w)["y"][0], "y")
 
 
+@pytest.mark.parametrize("bad", [float("inf"), float("nan")])
+@pytest.mark.parametrize("N", [3, 8, 16, 24, 40, 64])
+@pytest.mark.parametrize("T,B,D,cuts,at", [(50, 2, 20, (3, 9, 16, 24, 37), 20), (50, 1, 20, (8, 13, 21), 15), (600, 1, 16, (24, 200, 383, 400), 250)])
+def test_scan_resets_shield_an_episode_from_one_that_diverged(T, B, D, cuts, at, N, bad):
+    """What diverges in the episode of step ``at``, its state or its gradient, leaves every other episode bit for bit alone."""
+    v = scan_case(T, B, D, N, F32, reset=0, ragged=False, shift=-4.0, scale=0.3)
+    v["reset"] = torch.zeros(T, B, dtype=torch.uint8, device=DEV)
+    v["reset"][list(cuts)] = 1
+    a, b = max(c for c in cuts if c <= at), min(c for c in cuts if c > at)
+    good = run_scan(v)
+    for k in ("u", "dy"):
+        w = dict(v)
+        w[k] = v[k].clone()
+        w[k][at] = bad
+        got = run_scan(w)
+        for n in ("y", "du", "ddt", "dz", "dB", "dC"):
+            assert torch.equal(got[n][:a], good[n][:a]), (k, n, "before")
+            assert torch.equal(got[n][b:], good[n][b:]), (k, n, "behind")
+        assert torch.equal(got["hT"], good["hT"]) and torch.equal(got["dh0"], good["dh0"]), k
+
+
 # ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
 def test_norm_past_32_bits():
     M, D = 150000, 16384                                    # 2.46e9 elements
