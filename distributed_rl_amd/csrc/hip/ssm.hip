@@ -353,12 +353,13 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
     const long long n = p.B * p.D * p.N, i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= n) return;
     const long long r = i / p.N;
-    const float A2 = p.A[r % p.D * p.N + i % p.N] * LOG2E;
+    // P as the square of R: it may leave the range where P h does not. R is finite: an empty state stays empty.
+    const float A2 = p.A[r % p.D * p.N + i % p.N] * (0.5f * LOG2E);
     const float* h0 = BWD ? p.dhT : p.h0;
     float h = h0 ? h0[i] : 0.f;
     constexpr int AHEAD = 16;                               // loads in flight: a carry is overwritten only after its batch is read
     for (int k0 = 0; k0 < S; k0 += AHEAD) {
-        float e[AHEAD], sum[AHEAD];
+        float e[AHEAD], sum[AHEAD], R[AHEAD];
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             const int s = BWD ? S - 1 - k0 - k : k0 + k;
@@ -367,10 +368,12 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
             sum[k] = in ? sums[s * p.B * p.D + r] : 0.f;
         }
 #pragma unroll
+        for (int k = 0; k < AHEAD; ++k) R[k] = fminf(__builtin_amdgcn_exp2f(sum[k] * A2), 3.402823466e38f);
+#pragma unroll
         for (int k = 0; k < AHEAD; ++k) {
             if (k0 + k >= S) break;
             carry[(BWD ? S - 1 - k0 - k : k0 + k) * n + i] = h;
-            h = sum[k] == __builtin_inff() ? e[k] : fmaf(__builtin_amdgcn_exp2f(sum[k] * A2), h, e[k]);
+            h = sum[k] == __builtin_inff() ? e[k] : fmaf(R[k], R[k] * h, e[k]);
         }
     }
 }

@@ -455,6 +455,28 @@ def test_scan_resets_shield_an_episode_from_one_that_diverged(T, B, D, cuts, at,
         assert torch.equal(got["hT"], good["hT"]) and torch.equal(got["dh0"], good["dh0"]), k
 
 
+@pytest.mark.parametrize("rate,h0", [(1.2, 1e-20), (-1.2, 1e25)])
+def test_scan_segment_factors_beyond_the_range(rate, h0):
+    """Segments of 600 steps whose exp(A sum of s) leaves the range of fp32, while the state that it stands for does not."""
+    v = scan_case(600, 1, 16, 16, F32, reset=0, ragged=False, opt=("h0", "dhT"))
+    v["A"].fill_(1.0)
+    v["dt"].zero_()
+    v["dt"][80:160] = rate                                  # exp(96) over one segment
+    v["u"][80:160] = 0
+    v["h0"], v["dhT"], v["dy"] = v["h0"] * h0, v["dhT"] * h0, v["dy"] * 1e-20
+    check_scan_tight(v, softplus=False)
+
+
+def test_scan_segment_factors_beyond_the_range_of_an_empty_state():
+    v = scan_case(600, 1, 16, 16, F32, reset=0, ragged=False, opt=False)
+    v["A"].fill_(1.0)
+    v["dt"].fill_(0.01)
+    v["dt"][80:320] = 1.2
+    v["u"][:320] = 0                                        # no state before step 320, and no gradient from there on
+    v["dy"][80:] = 0
+    check_scan_tight(v, softplus=False)
+
+
 # ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
 def test_norm_past_32_bits():
     M, D = 150000, 16384                                    # 2.46e9 elements
