@@ -267,7 +267,7 @@ __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float
     float A2[NS], h[NS];
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        A2[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
+        A2[i] = dv && g * NS + i < p.N ? rate(p.A[(long long)d * p.N + g * NS + i], LOG2E) : 0.f;
         h[i] = 0.f;
     }
     const float bias = dv && p.bias ? p.bias[d] : 0.f;
@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
     if (i >= n) return;
     const long long r = i / p.N;
     // P as the square of R: it may leave the range where P h does not. R is finite: an empty state stays empty.
-    const float A2 = p.A[r % p.D * p.N + i % p.N] * (0.5f * LOG2E);
+    const float A2 = rate(p.A[r % p.D * p.N + i % p.N], 0.5f * LOG2E);
     const float* h0 = BWD ? p.dhT : p.h0;
     float h = h0 ? h0[i] : 0.f;
     constexpr int AHEAD = 16;                               // loads in flight: a carry is overwritten only after its batch is read
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     const float* hp = carry ? carry + blockIdx.z * BDN : p.h0;
     get_states<NS>(hp + so, h, g * NS, p.N, dv && hp, vec4(hp, p.N));
 #pragma unroll
-    for (int i = 0; i < NS; ++i) A2[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] * LOG2E : 0.f;
+    for (int i = 0; i < NS; ++i) A2[i] = dv && g * NS + i < p.N ? rate(p.A[(long long)d * p.N + g * NS + i], LOG2E) : 0.f;
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
     const unsigned ou = R::offset(p.u_t, g, d), od = R::offset(p.dt_t, g, d), oz = R::offset(p.z_t, g, d), oy = R::offset(p.y_t, g, d);
     const bool has_z = p.z != nullptr, soft = p.softplus != 0, ck4 = vec4(p.ckpt, p.N);
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(256, NS > 8 ? 1 : NS == 2 ? 4 : 2) void k_ssm_bwd(S
     get_states<NS>(Gp + so, G, g * NS, p.N, dv && Gp, vec4(Gp, p.N));
 #pragma unroll
     for (int i = 0; i < NS; ++i) {
-        An[i] = dv && g * NS + i < p.N ? p.A[(long long)d * p.N + g * NS + i] : 0.f;
+        An[i] = dv && g * NS + i < p.N ? rate(p.A[(long long)d * p.N + g * NS + i], 1.f) : 0.f;
         dA[i] = 0.f;
     }
     const float Dd = dv && p.Dp ? p.Dp[d] : 0.f, bias = dv && p.bias ? p.bias[d] : 0.f;
@@ -871,9 +871,10 @@ __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
         const long long i = i0 + k * step;
         float s = dt[k], y = 0.f;
         if (p.softplus) s = softplus(s);
+        const float s2 = s * LOG2E;                         // (A log2(e) may leave the range, and a step of size 0 holds the state)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const float e = __builtin_amdgcn_exp2f(s * (A[k][v] * LOG2E));
+            const float e = __builtin_amdgcn_exp2f(s2 * A[k][v]);
             h[k][v] = fmaf(e, rs[k] ? 0.f : h[k][v], s * u[k] * Bv[k][v]);
             y = fmaf(Cv[k][v], h[k][v], y);
         }

@@ -30,6 +30,12 @@ __device__ __forceinline__ float softplus(float x, float* slope = nullptr) {
     if (slope) *slope = x >= 0.f ? r : e * r;
     return fmaxf(x, 0.f) + fmaf(e - (u - 1.0f), r, __builtin_amdgcn_logf(u) * LN2);
 }
+// A decay rate times c. It stops at the lowest finite value: a state of rate -inf (or whose product leaves the range) has no
+// memory, but a step of size 0 - past a row's end, or one that is held - leaves it alone. A NaN passes.
+__device__ __forceinline__ float rate(float a, float c) {
+    const float r = a * c, low = -3.402823466e38f;
+    return r < low ? low : r;
+}
 // for gates: exp's error of |x| half steps stands next to 1, or where the gate is nearly shut
 __device__ __forceinline__ float sigmoidf(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -LOG2E)); }
 

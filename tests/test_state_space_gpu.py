@@ -477,6 +477,37 @@ def test_scan_segment_factors_beyond_the_range_of_an_empty_state():
     check_scan_tight(v, softplus=False)
 
 
+@pytest.mark.parametrize("T,B,D,N", [(21, 4, 20, 16), (40, 3, 24, 5), (600, 4, 16, 8)])
+def test_scan_decay_rates_of_the_lowest_value(T, B, D, N):
+    """A = the lowest value of the type: a state without memory, but held where a row has ended and over steps of size zero."""
+    v = scan_case(T, B, D, N, F32, reset=0.02, shift=-1.0)
+    v["A"][:, ::2] = torch.finfo(F32).min
+    check_scan_tight(v)
+    # the gradient of a held step is the lowest value times a state; and -inf times a step of zero is no number
+    for low, size in ((torch.finfo(F32).min, float("-inf")), (float("-inf"), 0.0)):
+        v["A"][:, ::2], v["dt"][T // 3] = low, size
+        w = clean({k: x for k, x in v.items() if k != "dy"})
+        w["A"][:, ::2], w["dt"][T // 3] = torch.finfo(F32).min, size
+        got, ref, tol = run_scan(v), ssm_ref.scan(w), ssm_ref.scan_bounds(w, cut=T > 112)
+        for k in ("y", "hT"):
+            ssm_ref.within(got[k], ref[k], tol[k], k)
+
+
+@pytest.mark.parametrize("N", [16, 5])
+def test_step_with_decay_rates_of_the_lowest_value(N):
+    v = scan_case(1, 3, 20, N, F32, ragged=False, reset=0)
+    for low, size in ((torch.finfo(F32).min, -1.0), (torch.finfo(F32).min, float("-inf")), (float("-inf"), -1.0)):
+        v["A"][:, ::2] = low
+        dt = torch.full_like(v["dt"][0], size)
+        h, y = v["h0"].clone(), torch.empty_like(v["u"][0])
+        H.ssm_step(v["u"][0], dt, v["A"], v["Bm"][0], v["Cm"][0], h, y, D=v["D"], z=v["z"][0], dt_bias=v["dt_bias"])
+        w = clean({k: x for k, x in v.items() if k not in ("dy", "dhT")})
+        w["dt"], w["A"][:, ::2] = torch.full_like(w["dt"], size), torch.finfo(F32).min
+        ref, tol = ssm_ref.scan(w), ssm_ref.scan_bounds(w)
+        ssm_ref.within(y, ref["y"][0], tol["y"][0], "y")
+        ssm_ref.within(h, ref["hT"], tol["hT"], "h")
+
+
 # ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
 def test_norm_past_32_bits():
     M, D = 150000, 16384                                    # 2.46e9 elements
