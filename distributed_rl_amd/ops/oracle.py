@@ -228,7 +228,7 @@ def ssm_scan(u: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, Bm: torch.Tenso
         live = torch.ones(B, 1, dtype=torch.bool, device=u.device) if lengths is None else (t < lengths)[:, None]
         ut, st, Bt, Ct = (torch.where(live, v[t], 0.0) for v in (u, dt, Bm, Cm))
         st = st if dt_bias is None else st + dt_bias
-        st = F.softplus(st, threshold=1e9) if softplus else st
+        st = F.softplus(st, threshold=40.0) if softplus else st         # beyond, exp(-st) is less than half a step of fp64
         old = h if reset is None else torch.where((reset[t] != 0)[:, None, None], 0.0, h)
         h = torch.where(live[..., None], torch.exp(st[..., None] * A) * old + (st * ut)[..., None] * Bt[:, None], h)
         y = (h * Ct[:, None]).sum(-1)

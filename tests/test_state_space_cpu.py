@@ -56,6 +56,23 @@ def test_scan_in_pieces_is_the_whole_scan():
     torch.testing.assert_close(h, hT, rtol=1e-13, atol=1e-13)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_scan_oracle_over_the_whole_range_of_step_sizes(dtype):
+    low = torch.finfo(dtype).min
+    dt = torch.tensor([0.0, -1.0, 30.0, 45.0, 88.0, 100.0, 710.0, 800.0, 1e30, -800.0, low, float("-inf")], dtype=dtype).view(1, -1, 1)
+    n = dt.shape[1]
+    one = torch.ones(1, n, 1, dtype=dtype)
+    x = dt.clone().requires_grad_()
+    y, h = oracle.ssm_scan(one, x, -torch.ones(1, 1, dtype=dtype), one, one, h0=torch.full((n, 1, 1), 3.0, dtype=dtype))
+    s = torch.logaddexp(dt.double(), torch.zeros((), dtype=torch.float64))[0]
+    want = 3.0 * torch.exp(-s) + s
+    # exp, log1p, their sum, the decay (its exponent's error fades with it), two products and a sum: 8 steps; twice that for the slope
+    torch.testing.assert_close(y[0].double(), want, rtol=8 * torch.finfo(dtype).eps, atol=0)
+    assert torch.equal(h[-2:, 0, 0], torch.full((2,), 3.0, dtype=dtype))                    # steps that are held
+    y.sum().backward()
+    torch.testing.assert_close(x.grad[0].double(), (1 - 3.0 * torch.exp(-s)) * torch.sigmoid(dt[0].double()), rtol=16 * torch.finfo(dtype).eps, atol=0)
+
+
 def conv_inputs(T, B, D, W, seed=0):
     g = torch.Generator().manual_seed(seed)
     return dict(x=rnd(g, T, B, D), w=rnd(g, D, W), bias=rnd(g, D), state_in=rnd(g, B, W - 1, D), dy=rnd(g, T, B, D),
