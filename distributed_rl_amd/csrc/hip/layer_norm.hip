@@ -2,6 +2,7 @@
 //   y = (x - mean) rstd w + b;   dx = rstd (dn - mean(dn) - n mean(dn n)), n = (x - mean) rstd, dn = dy w
 //   dw = sum over rows of dy n,  db = sum over rows of dy
 // The variance is summed around the mean, not as E[x^2] - mean^2, which cancels for rows far from zero.
+#include "apart.h"
 #include "ssm_math.h"
 
 struct NormArgs {        // mirrored by ops/hip.py (_NORM): 64-bit words in this order
@@ -359,6 +360,8 @@ static void norm_dispatch(const NormArgs& p, bool bwd, float eps, hipStream_t s)
 DRL_API int drl_norm_fwd(const NormArgs* a, int bf16, float eps, hipStream_t s) {
     const NormArgs p = *a;
     if (!norm_ok(p.M, p.D)) return -1;
+    const long long e = bf16 ? 2 : 4, cols = p.D * 4, rows = p.M * 4;
+    if (!apart({{p.y, p.D * e, p.M, p.y_r * e}, {p.mean, rows}, {p.rstd, rows}}, {{p.x, p.D * e, p.M, p.x_r * e}, {p.w, cols}, {p.b, cols}})) return -3;
     if (bf16) norm_dispatch<bf16_t>(p, false, eps, s);
     else norm_dispatch<float>(p, false, eps, s);
     return (int)hipGetLastError();
@@ -369,6 +372,9 @@ DRL_API int drl_norm_bwd(const NormArgs* a, int bf16, hipStream_t s) {
     long long need;
     if (drl_norm_ws(p.M, p.D, &need)) return -1;
     if (p.ws_n < need) return -2;
+    const long long e = bf16 ? 2 : 4, cols = p.D * 4, rows = p.M * 4;
+    if (!apart({{p.dx, p.D * e, p.M, p.dx_r * e}, {p.dw, cols}, {p.db, cols}, {p.ws, need * 4}},
+               {{p.x, p.D * e, p.M, p.x_r * e}, {p.dy, p.D * e, p.M, p.dy_r * e}, {p.w, cols}, {p.mean, rows}, {p.rstd, rows}})) return -3;
     if (bf16) norm_dispatch<bf16_t>(p, true, 0.f, s);
     else norm_dispatch<float>(p, true, 0.f, s);
     k_norm_sum<<<(unsigned)((2 * p.D + 31) / 32), 1024, 0, s>>>(p.ws, norm_blocks(p.M, p.D, bf16 ? 8 : 4), (int)p.D, p.dw, p.db);

@@ -8,6 +8,7 @@
 // the last channel: the channels that it has twice come out alike. Runs of one row are walked side by side; each starts by
 // reading the W - 1 steps before it again. More channels a thread means fewer loads but also fewer waves on a SIMD: both
 // passes of 120 x 64 x 1024 bf16 29 us with 2, 30 with 1, 33 with 4; of 1021 x 9 x 771 fp32 46 with 4, 51 with 2, 54 with 1.
+#include "apart.h"
 #include "ssm_math.h"
 #include <type_traits>
 
@@ -435,9 +436,17 @@ static void launch_conv_step(const ConvArgs& p, dim3 grid, hipStream_t s) { k_co
 #define CONV_SEQ(T, V, W, BWD) cg.L >= 64 ? launch_conv<T, V, W, true>(p, cg, BWD, grid, s) : launch_conv<T, V, W, false>(p, cg, BWD, grid, s)
 #define CONV_ONE(T, V, W, _) launch_conv_step<T, V, W>(p, grid, s)
 
+// a [T, B, D] tensor (e bytes an element) and what else a call reads
+static View seq_view(const ConvArgs& p, const void* q, long long st, long long sb, long long e) { return {q, p.D * e, p.T, st * e, p.B, sb * e}; }
+static View state_view(const ConvArgs& p, const void* q, long long e) { return {q, p.B * (p.W - 1) * p.D * e}; }
+
 DRL_API int drl_short_conv_fwd(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(p.T, p.B, p.D, p.W)) return -1;
+    const long long e = bf16 ? 2 : 4;
+    if (!apart({seq_view(p, p.y, p.y_t, p.y_b, e), state_view(p, p.state_out, e)},
+               {seq_view(p, p.x, p.x_t, p.x_b, e), state_view(p, p.state_in, e), {p.w, p.D * p.W * 4}, {p.bias, p.D * 4}, {p.reset, p.T * p.B},
+                {p.lengths, p.B * 4}})) return -3;
     const ConvGrid cg = conv_grid(p.T, p.B, p.D, bf16, 0);
     const long long cv = conv_cols(p.D, conv_v(bf16)), per = 256 / cg.L;
     if ((cg.n_seg + per - 1) / per > 65535) return -1;
@@ -451,6 +460,10 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
     long long need;
     if (drl_short_conv_ws(p.T, p.B, p.D, p.W, &need)) return -1;
     if (p.ws_n < need) return -2;
+    const long long e = bf16 ? 2 : 4;
+    if (!apart({seq_view(p, p.dx, p.dx_t, p.dx_b, e), state_view(p, p.dstate_in, e), {p.dw, p.D * p.W * 4}, {p.db, p.D * 4}, {p.ws, need * 4}},
+               {seq_view(p, p.x, p.x_t, p.x_b, e), seq_view(p, p.dy, p.dy_t, p.dy_b, e), state_view(p, p.state_in, e), state_view(p, p.dstate_out, e),
+                {p.w, p.D * p.W * 4}, {p.bias, p.D * 4}, {p.reset, p.T * p.B}, {p.lengths, p.B * 4}})) return -3;
     const ConvGrid cg = conv_grid(p.T, p.B, p.D, bf16, (int)p.W - 1);
     const long long cv = conv_cols(p.D, conv_v(bf16)), n = (p.W + 1) * p.D;
     const dim3 grid((unsigned)((cv + cg.L - 1) / cg.L), (unsigned)cg.rows);
@@ -462,6 +475,9 @@ DRL_API int drl_short_conv_bwd(const ConvArgs* a, int bf16, hipStream_t s) {
 DRL_API int drl_short_conv_step(const ConvArgs* a, int bf16, hipStream_t s) {
     const ConvArgs p = *a;
     if (!conv_ok(1, 1, p.D, p.W) || p.B <= 0) return -1;
+    const long long e = bf16 ? 2 : 4;
+    if (!apart({{p.y, p.D * e, p.B, p.y_b * e}, state_view(p, p.state_out, e)},
+               {{p.x, p.D * e, p.B, p.x_b * e}, {p.w, p.D * p.W * 4}, {p.bias, p.D * 4}, {p.reset, p.B}})) return -3;
     const long long nb = (p.B * conv_cols(p.D, V_STEP) + 255) / 256;
     if (nb >= 1ll << 38) return -1;
     const long long x = nb < (1 << 23) ? nb : 1 << 23;

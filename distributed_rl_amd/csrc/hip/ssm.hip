@@ -11,6 +11,7 @@
 // Bound by vector issue: a state and step cost an exp (2.5 issue slots) and four more instructions forward, an exp and twelve
 // backward. Four lanes a channel keep 16 states at 4 registers a lane of each kind, and the sums over states at a row swap and
 // an add a step.
+#include "apart.h"
 #include "ssm_math.h"
 #include <type_traits>
 
@@ -978,11 +979,21 @@ static void launch_bwd(const SsmArgs& p, hipStream_t s) {
         default: NAME<T, 16>(p, s); break;    \
     }
 
+// [T, B, c] tensors of e bytes an element, and the fp32 ones
+static View seq_view(const SsmArgs& p, const void* q, long long st, long long sb, long long c, long long e) { return {q, c * e, p.T, st * e, p.B, sb * e}; }
+static View state_view(const SsmArgs& p, const void* q) { return {q, p.B * p.D * p.N * 4}; }
+static View ckpt_view(const SsmArgs& p) { return {p.ckpt, (p.T + SAVE - 1) / SAVE * p.B * p.D * p.N * 4}; }
+
 DRL_API int drl_ssm_fwd(const SsmArgs* a, int bf16, hipStream_t s) {
     SsmArgs p = *a;
     long long need;
     if (drl_ssm_ws(p.T, p.B, p.D, p.N, 0, &need) || !steps_ok(p)) return -1;
     if (p.ws_n < need) return -2;
+    const long long e = bf16 ? 2 : 4, cols = p.D * 4;
+    if (!apart({seq_view(p, p.y, p.y_t, p.y_b, p.D, e), state_view(p, p.hT), ckpt_view(p), {p.ws, need * 4}},
+               {seq_view(p, p.u, p.u_t, p.u_b, p.D, e), seq_view(p, p.dt, p.dt_t, p.dt_b, p.D, e), seq_view(p, p.z, p.z_t, p.z_b, p.D, e),
+                seq_view(p, p.Bm, p.B_t, p.B_b, p.N, e), seq_view(p, p.Cm, p.C_t, p.C_b, p.N, e), {p.A, cols * p.N}, {p.Dp, cols}, {p.bias, cols},
+                state_view(p, p.h0), {p.reset, p.T * p.B}, {p.lengths, p.B * 4}})) return -3;
     if (bf16) { SSM_NS(launch_fwd, bf16_t) } else { SSM_NS(launch_fwd, float) }
     return (int)hipGetLastError();
 }
@@ -992,6 +1003,13 @@ DRL_API int drl_ssm_bwd(const SsmArgs* a, int bf16, hipStream_t s) {
     long long need;
     if (drl_ssm_ws(p.T, p.B, p.D, p.N, 1, &need) || !p.ckpt || !steps_ok(p)) return -1;
     if (p.ws_n < need) return -2;
+    const long long e = bf16 ? 2 : 4, cols = p.D * 4;
+    if (!apart({seq_view(p, p.du, p.du_t, p.du_b, p.D, e), seq_view(p, p.ddt, p.ddt_t, p.ddt_b, p.D, e), seq_view(p, p.dz, p.dz_t, p.dz_b, p.D, e),
+                seq_view(p, p.dBm, p.dB_t, p.dB_b, p.N, e), seq_view(p, p.dCm, p.dC_t, p.dC_b, p.N, e), {p.dA, cols * p.N}, {p.dD, cols}, {p.dbias, cols},
+                state_view(p, p.dh0), {p.ws, need * 4}},
+               {seq_view(p, p.u, p.u_t, p.u_b, p.D, e), seq_view(p, p.dt, p.dt_t, p.dt_b, p.D, e), seq_view(p, p.z, p.z_t, p.z_b, p.D, e),
+                seq_view(p, p.Bm, p.B_t, p.B_b, p.N, e), seq_view(p, p.Cm, p.C_t, p.C_b, p.N, e), seq_view(p, p.dy, p.dy_t, p.dy_b, p.D, e),
+                {p.A, cols * p.N}, {p.Dp, cols}, {p.bias, cols}, state_view(p, p.dhT), ckpt_view(p), {p.reset, p.T * p.B}, {p.lengths, p.B * 4}})) return -3;
     if (bf16) { SSM_NS(launch_bwd, bf16_t) } else { SSM_NS(launch_bwd, float) }
     return (int)hipGetLastError();
 }
@@ -1025,6 +1043,10 @@ static void dispatch_step(const SsmArgs& p, hipStream_t s) {
 DRL_API int drl_ssm_step(const SsmArgs* a, int bf16, hipStream_t s) {
     const SsmArgs p = *a;
     if (p.B <= 0 || p.D <= 0 || p.D >= (1ll << 31) || p.N <= 0 || p.N > 64 || p.B * p.D >= (1ll << 33)) return -1;
+    const long long e = bf16 ? 2 : 4, cols = p.D * 4;
+    if (!apart({{p.y, p.D * e, p.B, p.y_b * e}, state_view(p, p.hT)},
+               {{p.u, p.D * e, p.B, p.u_b * e}, {p.dt, p.D * e, p.B, p.dt_b * e}, {p.z, p.D * e, p.B, p.z_b * e}, {p.Bm, p.N * e, p.B, p.B_b * e},
+                {p.Cm, p.N * e, p.B, p.C_b * e}, {p.A, cols * p.N}, {p.Dp, cols}, {p.bias, cols}, {p.reset, p.B}})) return -3;
     if (bf16) dispatch_step<bf16_t>(p, s);
     else dispatch_step<float>(p, s);
     return (int)hipGetLastError();

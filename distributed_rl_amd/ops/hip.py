@@ -1112,7 +1112,8 @@ def _rows3(t: Optional[torch.Tensor], shape: tuple, lead: tuple, dtype, dev: int
 
 
 def _apart(outs: tuple, ins: tuple) -> None:
-    """No output starts where an input or another output does (0: not given)."""
+    """No output starts where an input or another output does (0: not given). That none overlaps one from another start is
+    looked at by the library, which has the sizes and strides."""
     given = {*outs}
     given.discard(0)
     if len(given) != len(outs) - outs.count(0) or not given.isdisjoint(ins):
@@ -1136,9 +1137,11 @@ def _ws_numel(rc: int, n: ctypes.c_longlong, what: str, sizes) -> int:
     return n.value
 
 
-def _run(fn, rec: bytes, bf16: int, dev: int) -> None:
-    """Launch on the current stream of the tensors' device."""
-    rc = fn(rec, bf16, _raw_stream(dev))
+def _run(fn, rec: bytes, *args) -> None:
+    """Launch; the last of ``args`` is the GPU whose current stream it goes to."""
+    rc = fn(rec, *args[:-1], _raw_stream(args[-1]))
+    if rc == -3:
+        raise ValueError("an output shares its memory with an input or another output")
     if rc != 0:
         raise RuntimeError("%s failed with code %d%s" % (fn.__name__, rc, " (workspace too small)" if rc == -2 else ""))
 
@@ -1165,7 +1168,7 @@ def layer_norm_fwd(x, w, b, y, mean=None, rstd=None, eps: float = 1e-5) -> None:
     wp, bp = _vec(w, (D,), f32, dev, "w"), _opt(b, (D,), f32, dev, "b")
     mp, rp = _opt(mean, (M,), f32, dev, "mean"), _opt(rstd, (M,), f32, dev, "rstd")
     _apart((yp, mp, rp), (xp, wp, bp))
-    _ck(native.hip().drl_norm_fwd(_NORM_FWD.pack(xp, xs, wp, bp, yp, ys, mp, rp, M, D), bf16, eps, _raw_stream(dev)), "layer_norm_fwd")
+    _run(native.hip().drl_norm_fwd, _NORM_FWD.pack(xp, xs, wp, bp, yp, ys, mp, rp, M, D), bf16, eps, dev)
 
 
 def layer_norm_bwd(dy, x, w, mean, rstd, dx, dw, db, ws) -> None:

@@ -1,9 +1,15 @@
 """State-space operators on the CPU: the oracle against the formulas written out, its gradients against differences, cut
 sequences against whole ones, and what the entry points of the kernels refuse before anything is launched."""
+import os
+import random
+import shutil
+import subprocess
+
 import pytest
 import torch
 
 import ssm_ref
+from distributed_rl_amd import native
 from distributed_rl_amd.ops import hip, oracle
 
 
@@ -208,3 +214,91 @@ def test_scan_coefficients_of_other_sizes_than_the_sequence_are_refused(monkeypa
                 scan_args(backward=backward, **{k: both[k]})
     batch_major = {k: torch.zeros(4, 50, 4).transpose(0, 1) for k in ("Bm", "Cm") + grads}
     scan_args(backward=backward, **batch_major)             # a transpose of the right shape is fine
+
+
+# ---- outputs that overlap ------------------------------------------------------------------------------------------------------
+HARNESS = """
+#include <cstdio>
+#include "apart.h"
+int main() {
+    View v[2];
+    while (true) {
+        for (View& x : v)
+            if (std::scanf("%lld %lld %lld %lld %lld %lld", &x.at, &x.row, &x.n[0], &x.s[0], &x.n[1], &x.s[1]) != 6) return 0;
+        std::printf("%d\\n", share(v[0], v[1]));
+    }
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ not available")
+def test_views_share_memory_where_their_bytes_do(tmp_path):
+    src = tmp_path / "share.cpp"
+    src.write_text(HARNESS)
+    inc = os.path.join(os.path.dirname(hip.__file__), "..", "csrc", "hip")
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-I", inc, str(src), "-o", str(tmp_path / "share")], check=True)
+    r = random.Random(0)
+    views = [((0, 8, 5, 40, 3, 200), (8, 8, 5, 40, 3, 200)),                       # neighbours in the same rows
+             ((0, 8, 5, 40, 3, 200), (8, 33, 5, 40, 3, 200)),                      # ... one of them a byte too wide
+             ((0, 8, 3, 200, 5, 40), (8, 8, 5, 40, 3, 200)),                       # the axes the other way round
+             ((0, 4, 1000000, 0, 1, 0), (4, 4, 1000000, 0, 7, 4)),                 # one row read many times
+             ((0, 2, 70000, 32768, 60000, 64), (2, 2, 70000, 32768, 60000, 64)),   # past 32 bits
+             ((0, 2, 70000, 32768, 60000, 64), (2 + 69999 * 32768 + 59999 * 64, 2, 1, 0, 1, 0)),
+             ((0, 2, 70000, 32768, 60000, 64), (69999 * 32768 + 59999 * 64 + 1, 2, 1, 0, 1, 0)),
+             ((0, 0, 1, 0, 1, 0), (0, 8, 1, 0, 1, 0))]                             # no tensor
+    want = [False, True, False, False, False, False, True, False]
+    for _ in range(3000):
+        one = lambda: (r.randint(0, 60), r.choice([1, 2, 4, 8]), r.randint(1, 4), r.choice([0, 3, 8, 10, 16, 24, 40]), r.randint(1, 4),   # noqa: E731
+                       r.choice([0, 2, 8, 12, 16, 32, 72]))
+        a, b = one(), one()
+        byte = [{v[0] + i * v[3] + j * v[5] + k for i in range(v[2]) for j in range(v[4]) for k in range(v[1])} for v in (a, b)]
+        views.append((a, b))
+        want.append(bool(byte[0] & byte[1]))
+    text = "\n".join(" ".join(map(str, a + b)) for a, b in views)
+    got = subprocess.run([str(tmp_path / "share")], input=text, stdout=subprocess.PIPE, text=True, check=True, timeout=60).stdout.split()
+    assert [g == "1" for g in got] == want
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="tensors on the CPU are shown to the library as a GPU's: every call here is refused by it")
+def test_outputs_that_overlap_from_another_start_are_refused(monkeypatch):
+    if not native.hip_available():
+        pytest.skip("libdrl_hip.so is not built")
+    monkeypatch.setattr(hip, "_dev", lambda t: t.get_device())
+    monkeypatch.setattr(hip, "_raw_stream", lambda dev: 0)
+    z = lambda *s: torch.zeros(*s)                                          # noqa: E731
+    T, B, D, N, W = 10, 3, 8, 4, 4
+
+    def each(call, outs, ins, fixed):
+        names = outs + ins
+        for i, o in enumerate(outs):
+            for other in names[i + 1:]:
+                kw = dict(fixed)
+                small, large = sorted((o, other), key=lambda k: fixed[k].nbytes)
+                buf = torch.zeros(fixed[large].nbytes + 4, dtype=torch.uint8)
+                for k, at in ((large, 0), (small, 4)):
+                    kw[k] = buf[at:at + fixed[k].nbytes].view(fixed[k].dtype).view(fixed[k].shape)
+                with pytest.raises(ValueError, match="shares"):
+                    call(**kw)
+
+    each(hip.layer_norm_fwd, ["y", "mean", "rstd"], ["x", "w", "b"], dict(x=z(T, D), w=z(D), b=z(D), y=z(T, D), mean=z(T), rstd=z(T)))
+    each(hip.layer_norm_bwd, ["dx", "dw", "db", "ws"], ["dy", "x", "w", "mean", "rstd"],
+         dict(dy=z(T, D), x=z(T, D), w=z(D), mean=z(T), rstd=z(T), dx=z(T, D), dw=z(D), db=z(D), ws=hip.layer_norm_ws(T, D, "cpu")))
+    u8, i32 = dict(dtype=torch.uint8), dict(dtype=torch.int32)
+    conv = dict(x=z(T, B, D), w=z(D, W), bias=z(D), state_in=z(B, W - 1, D), reset=torch.zeros(T, B, **u8), lengths=torch.zeros(B, **i32))
+    each(hip.short_conv_fwd, ["y", "state_out"], list(conv), dict(conv, y=z(T, B, D), state_out=z(B, W - 1, D)))
+    each(hip.short_conv_bwd, ["dx", "dw", "db", "dstate_in", "ws"], list(conv) + ["dy", "dstate_out"],
+         dict(conv, dy=z(T, B, D), dstate_out=z(B, W - 1, D), dx=z(T, B, D), dw=z(D, W), db=z(D), dstate_in=z(B, W - 1, D),
+              ws=hip.short_conv_ws(T, B, D, W, "cpu")))
+    each(hip.short_conv_step, ["y", "state"], ["x", "w", "bias", "reset"],
+         dict(x=z(B, D), w=z(D, W), bias=z(D), state=z(B, W - 1, D), y=z(B, D), reset=torch.zeros(B, **u8)))
+    scan = dict(u=z(T, B, D), dt=z(T, B, D), A=z(D, N), Bm=z(T, B, N), Cm=z(T, B, N), D=z(D), z=z(T, B, D), dt_bias=z(D),
+                reset=torch.zeros(T, B, **u8), lengths=torch.zeros(B, **i32))
+    ckpt = hip.ssm_scan_ckpt(T, B, D, N, "cpu").zero_()
+    each(hip.ssm_scan_fwd, ["y", "hT", "ckpt"], list(scan) + ["h0"],
+         dict(scan, y=z(T, B, D), hT=z(B, D, N), h0=z(B, D, N), ckpt=ckpt, ws=hip.ssm_scan_ws(T, B, D, N, "cpu")))
+    grads = dict(du=z(T, B, D), ddt=z(T, B, D), dA=z(D, N), dB=z(T, B, N), dC=z(T, B, N), dD=z(D), dz=z(T, B, D), ddt_bias=z(D), dh0=z(B, D, N),
+                 ws=hip.ssm_scan_ws(T, B, D, N, "cpu"))
+    each(hip.ssm_scan_bwd, list(grads), list(scan) + ["dy", "ckpt", "dhT"], dict(scan, **grads, dy=z(T, B, D), ckpt=ckpt, dhT=z(B, D, N)))
+    each(hip.ssm_step, ["y", "h"], ["u", "dt", "A", "Bm", "Cm", "D", "z", "dt_bias", "reset"],
+         dict(u=z(B, D), dt=z(B, D), A=z(D, N), Bm=z(B, N), Cm=z(B, N), h=z(B, D, N), y=z(B, D), D=z(D), z=z(B, D), dt_bias=z(D),
+              reset=torch.zeros(B, **u8)))

@@ -807,3 +807,22 @@ def test_refusals():
         H.short_conv_ws(5, 2, 8, 5, DEV)
     with pytest.raises(ValueError):
         H.layer_norm_ws(5, 20000, DEV)
+
+
+def test_an_output_beside_an_input_of_the_same_rows_and_one_that_overlaps_it():
+    g = Gen(5)
+    T, B, D, W = 9, 3, 24, 4
+    w, buf = g.n(D, W), g.n(T, B, 2 * D)
+    x, ref = buf[..., :D].clone(), torch.empty(T, B, D, device=DEV)
+    H.short_conv_fwd(x, w, None, ref)
+    with pytest.raises(ValueError, match="shares"):
+        H.short_conv_fwd(buf[..., :D], w, None, buf[..., D - 1:2 * D - 1])
+    H.short_conv_fwd(buf[..., :D], w, None, buf[..., D:])
+    assert torch.equal(buf[..., D:], ref) and torch.equal(buf[..., :D], x)
+    rows = g.n(2 * T, D)
+    ref = torch.empty(T, D, device=DEV)
+    H.layer_norm_fwd(rows[::2], w[:, 0].contiguous(), None, ref)
+    with pytest.raises(ValueError, match="shares"):
+        H.layer_norm_fwd(rows[:T], w[:, 0].contiguous(), None, rows[T - 1:2 * T - 1])
+    H.layer_norm_fwd(rows[::2], w[:, 0].contiguous(), None, rows[1::2])
+    assert torch.equal(rows[1::2], ref)
