@@ -51,6 +51,30 @@ def test_scan_gradients_against_differences():
     assert torch.autograd.gradcheck(lambda *a: oracle.ssm_scan(**dict(zip(SCAN_KEYS, a)), reset=v["reset"], lengths=v["lengths"]), p)
 
 
+@pytest.mark.parametrize("T,shift", [(40, -2.0), (700, -4.0)])
+def test_scan_bounds_hold_for_fp32_and_not_for_a_state_of_fewer_bits(T, shift):
+    v = scan_inputs(T, 3, 17, 5, seed=1)
+    v["dt"] = v["dt"] * 0.6 + 2 + shift
+    v = {k: x.float().double() if x.dtype == torch.float64 else x for k, x in v.items()}
+    v.update(reset=(v["reset"] * (torch.arange(T) % 7 == 0)[:, None]).to(torch.uint8), lengths=torch.tensor([T, T - 9, 1], dtype=torch.int32))
+    ref, tol = ssm_ref.scan(v), ssm_ref.scan_bounds(v)
+    p = {k: v[k].float().requires_grad_() for k in SCAN_KEYS}
+    y, hT = oracle.ssm_scan(**p, reset=v["reset"], lengths=v["lengths"])
+    ((y * v["dy"].float()).sum() + (hT * v["dhT"].float()).sum()).backward()
+    got = dict(y=y, hT=hT, **{r: p[k].grad for k, r in dict(u="du", dt="ddt", A="dA", Bm="dB", Cm="dC", D="dD", z="dz", dt_bias="ddt_bias", h0="dh0").items()})
+    for k in got:
+        ssm_ref.within(got[k], ref[k], tol[k], k)
+    h, ys = v["h0"].float(), []
+    for t in range(T):                                      # the oracle with its state rounded to bf16 after every step
+        one = {k: v[k][t:t + 1].float() for k in ("u", "dt", "Bm", "Cm", "z")}
+        y, h = oracle.ssm_scan(**one, **{k: v[k].float() for k in ("A", "D", "dt_bias")}, h0=h, reset=v["reset"][t:t + 1], lengths=v["lengths"] - t)
+        h = h.bfloat16().float()
+        ys.append(y[0])
+    for k, x in (("y", torch.stack(ys)), ("hT", h)):
+        with pytest.raises(AssertionError, match="outside"):
+            ssm_ref.within(x, ref[k], tol[k], k)
+
+
 def test_scan_in_pieces_is_the_whole_scan():
     v = scan_inputs(17, 3, 4, 5, seed=2, grads=False)
     v["lengths"] = None
@@ -141,6 +165,26 @@ def test_sizes_are_refused(T, B, D, N):
         hip.short_conv_fwd(u, torch.empty(D, 5 if N else 1), None, u.clone())
     with pytest.raises(ValueError):
         hip.layer_norm_fwd(torch.empty(T * 0, 16385), torch.empty(16385), None, torch.empty(0, 16385))
+
+
+def test_each_size_of_the_convolution_and_the_norm_is_refused_for_itself():
+    for T, B, W in ((0, 3, 4), (3, 0, 4), (3, 2, 1), (3, 2, 5), (3, 2, 0)):
+        u = torch.empty(T, B, 8)
+        with pytest.raises(ValueError, match="short_conv: unsupported sizes"):
+            hip.short_conv_fwd(u, torch.empty(8, W), None, u.clone())
+    with pytest.raises(ValueError, match="short_conv: unsupported sizes"):
+        hip.short_conv_fwd(torch.empty(3, 2, 0), torch.empty(0, 4), None, torch.empty(3, 2, 0))
+    for W in (1, 5):
+        with pytest.raises(ValueError, match="short_conv_step"):
+            hip.short_conv_step(torch.empty(2, 8), torch.empty(8, W), None, torch.empty(2, 3, 8), torch.empty(2, 8))
+    for M, D in ((1, 16385), (0, 8), (1, 0)):
+        with pytest.raises(ValueError, match="layer_norm: x must be"):
+            hip.layer_norm_fwd(torch.empty(M, D), torch.empty(D), None, torch.empty(M, D))
+    with pytest.raises(TypeError, match="CUDA"):            # the largest sizes of each get as far as the device
+        hip.layer_norm_fwd(torch.empty(1, 16384), torch.empty(16384), None, torch.empty(1, 16384))
+    for W in (2, 4):
+        with pytest.raises(TypeError, match="CUDA"):
+            hip.short_conv_fwd(torch.empty(1, 1, 8), torch.empty(8, W), None, torch.empty(1, 1, 8))
 
 
 def test_sizes_past_the_limits_are_refused():

@@ -508,6 +508,30 @@ def test_step_with_decay_rates_of_the_lowest_value(N):
         ssm_ref.within(h, ref["hT"], tol["hT"], "h")
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("N,reset", [(16, 0), (5, 0.01), (40, 0.01)])
+def test_scan_rows_that_end_inside_a_cut_sequence(N, reset, dtype):
+    """600 steps of ten short rows are cut into segments of 80: rows that end in the middle of a chunk, around a segment's border,
+    with the first step, and never; what is behind is NaN."""
+    T, D = 600, 16
+    ends = torch.tensor([T, 245, 240, 239, 241, 1, 0, 480, 473, 81], dtype=torch.int32)
+    v = scan_case(T, len(ends), D, N, dtype, reset=reset, ragged=False, shift=-4.0, scale=0.3)
+    v["lengths"] = ends.to(DEV)
+    dead = torch.arange(T, device=DEV)[:, None] >= v["lengths"][None]
+    for k in ("u", "dt", "Bm", "Cm", "dy", "z"):
+        v[k][dead] = float("nan")
+    got = check_scan_tight(v)
+    assert torch.equal(got["hT"][6], v["h0"][6]) and torch.equal(got["dh0"][6], v["dhT"][6])
+    for k in ("y", "du", "ddt", "dz", "dB", "dC"):
+        assert bool((got[k][dead] == 0).all()), k
+
+
+@pytest.mark.parametrize("T,B,D,N,dtype", [(1100, 2, 17, 5, F32), (523, 1, 40, 8, BF), (260, 1, 64, 40, F32), (120, 3, 70, 16, F32), (90, 2, 33, 24, BF)])
+def test_scan_of_long_sequences_within_bounds_that_fade(T, B, D, N, dtype):
+    check_scan_tight(scan_case(T, B, D, N, dtype, reset=0.004, shift=-4.0, scale=0.3))
+    check_scan_tight(scan_case(T, B, D, N, dtype, reset=0, ragged=False, shift=-4.0, scale=0.3))
+
+
 # ---- offsets past 32 bits -----------------------------------------------------------------------------------------------
 def test_norm_past_32_bits():
     M, D = 150000, 16384                                    # 2.46e9 elements
