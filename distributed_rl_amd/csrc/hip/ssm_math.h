@@ -17,7 +17,7 @@ __device__ __forceinline__ void st(bf16_t* p, float v) { *p = f2bf(v); }
 // argument stops there (a NaN passes), as the product would leave the range with it and what it lost be no number: a step of
 // size -inf or of the type's lowest value holds the state.
 __device__ __forceinline__ float exp_neg_abs(float x) {
-    const float mx = -fabsf(x), ax = mx < -128.f ? -128.f : mx, hi = ax * LOG2E;
+    const float ax = __builtin_elementwise_maximum(-fabsf(x), -128.f), hi = ax * LOG2E;
     const float lo = fmaf(ax, LOG2E, -hi) + ax * LOG2E_LO;
     const float p = __builtin_amdgcn_exp2f(hi);
     return fmaf(p, lo * LN2, p);
@@ -33,8 +33,7 @@ __device__ __forceinline__ float softplus(float x, float* slope = nullptr) {
 // A decay rate times c. It stops at the lowest finite value: a state of rate -inf (or whose product leaves the range) has no
 // memory, but a step of size 0 - past a row's end, or one that is held - leaves it alone. A NaN passes.
 __device__ __forceinline__ float rate(float a, float c) {
-    const float r = a * c, low = -3.402823466e38f;
-    return r < low ? low : r;
+    return __builtin_elementwise_maximum(a * c, -3.402823466e38f);
 }
 // for gates: exp's error of |x| half steps stands next to 1, or where the gate is nearly shut
 __device__ __forceinline__ float sigmoidf(float x) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * -LOG2E)); }
