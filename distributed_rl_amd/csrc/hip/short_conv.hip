@@ -84,7 +84,6 @@ __device__ __forceinline__ void czero(float (&v)[V]) {
 __device__ __forceinline__ int row_end(const ConvArgs& p, int b) {
     return p.lengths ? max(0, min(p.lengths[b], (int)p.T)) : (int)p.T;
 }
-__device__ __forceinline__ bool resets(const ConvArgs& p, int b, int t) { return t >= 0 && p.reset && p.reset[(long long)t * p.B + b] != 0; }
 
 // WIDE: 64 or more threads across the channels, so a wave has one row and one run, whose steps and flags are scalars.
 template <bool WIDE>

@@ -253,7 +253,7 @@ __device__ __forceinline__ float sum_rows4(const float* be, const float* ce, con
 // h -> P h + e with P = exp(A sum of s) and e its end state from h = 0 (k_ssm_carry), the segments are joined in order
 // (k_ssm_join), and then every segment runs from its true state. The backward does the same against the time with
 // G -> P G + e. ``carry`` points at [S, B, D, N] carries (nullptr: one segment), [S, B, D] sums of s follow them. 4096 x 2 x 1024
-// fp32, 16 states: 37 us (40 backward) beside 52 (149) of the true pass and 6 (8) of the join.
+// fp32, 16 states: 36 us (38 backward) beside 51 (147) of the true pass and 6 (8) of the join.
 template <typename T, int NS, bool BWD>
 __global__ __launch_bounds__(256) void k_ssm_carry(SsmArgs p, int seg_len, float* __restrict__ carry, float* __restrict__ sums) {
     constexpr int NP = 4 * NS;
@@ -379,7 +379,7 @@ __global__ __launch_bounds__(256) void k_ssm_join(SsmArgs p, int S, float* __res
     }
 }
 
-// 120 x 64 x 1024 bf16, 16 states: 40 to 45 us, its vector units busy 88 % of the time, 1.6 TB/s; 32 states 68 us, 4
+// 120 x 64 x 1024 bf16, 16 states: 41 to 45 us, its vector units busy 89 % of the time, 1.6 TB/s; 32 states 68 us, 4
 // states 28 us.
 template <typename T, int NS>
 __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const float* __restrict__ carry) {
@@ -487,10 +487,10 @@ __global__ __launch_bounds__(256) void k_ssm_fwd(SsmArgs p, int seg_len, const f
     if (p.hT && dv && blockIdx.z == gridDim.z - 1) put_states<NS>(p.hT + so, h, g * NS, p.N, vec4(p.hT, p.N));
 }
 
-// Backward. g_t = C ds + a_{t+1} g_{t+1} runs against the time; the states it needs are recomputed chunk by chunk from the
-// saved ones and kept in registers (16 steps x NS, next to the decays). The sums over channels of dB and dC leave as partials
+// Backward. g_t = C ds + a_{t+1} g_{t+1} runs against the time; the states it needs are recomputed from the saved ones, KH = 8
+// steps at a time (4 from 17 states on), and kept in registers next to the decays. The sums over channels of dB and dC leave as partials
 // of 64 channels (a block), the sums over rows of dA, dD and the bias as partials of a row: a second launch adds them in a
-// fixed order. 120 x 64 x 1024 bf16, 16 states, resets and lengths of 30 .. 120: 99 to 105 us, vector units busy 74 % of the
+// fixed order. 120 x 64 x 1024 bf16, 16 states, resets and lengths of 30 .. 120: 102 to 107 us, vector units busy 74 % of the
 // time with two waves a SIMD. Three fit 168 registers only with spills or with LDS reads one step at a time: 3 to 8 % slower.
 //
 // KH steps of a chunk, s0 .. s0 + KH - 1, from the state before them: forward with the states and decays kept, then back.
@@ -594,7 +594,8 @@ __device__ __forceinline__ void bwd_piece(const float4 (&pw_w)[KC][16], const fl
     }
 }
 
-// Four waves a SIMD for up to 8 states: 120 x 64 x 1024 both passes 130 -> 117 us, though the form with resets spills 7 registers.
+// Four waves a SIMD for 5 to 8 states: 120 x 64 x 1024 both passes 130 -> 117 us, though up to 4 registers spill. Up to 4 states
+// they fit without being asked for.
 // HAS: the call has reset flags. (A branch on each chunk's flags instead holds the registers of both paths: spills.)
 template <typename T, int NS, bool HAS>
 __global__ __launch_bounds__(256, NS > 8 ? 1 : NS == 2 ? 4 : 2) void k_ssm_bwd(SsmArgs p, int seg_len, const float* __restrict__ carry,
@@ -834,10 +835,11 @@ __global__ __launch_bounds__(256) void k_ssm_finish(SsmArgs p, const float* __re
     else if (p.dbias) p.dbias[i - DN - p.D] = v;
 }
 
-// One step: h [B, D, N] is read and written once and is nearly all of the bytes. Consecutive lanes own consecutive V states
-// (16 bytes; one state where N or an address does not allow it), L = 2^k >= N / V lanes a channel, and add up the read-out
-// with cross-lane adds; what depends on the channel only is computed by each of its lanes. A thread takes R channels with
-// the loads of all of them under way. 4096 x 1024 bf16, 16 states: 119 us (4.8 TB/s), 64 x 1024 4.2 us.
+// One step: h [B, D, N] is read and written once and is nearly all of the bytes. Consecutive lanes own V consecutive states (four,
+// 16 bytes, where N is a power of two from 4 on and the addresses allow it, otherwise one), L = 2^k >= N / V lanes a channel,
+// and add up the read-out with cross-lane adds; what depends on the channel only is computed by each of its lanes. A thread
+// takes R channels with the loads of all of them under way. 4096 x 1024 bf16, 16 states: 119 us (4.8 TB/s), 64 x 1024 4.2 us.
+// One state a lane means a channel's step size in 32 or 64 lanes and idle ones: 24 states 566 us, 40 states 1 106 (1.2 TB/s).
 template <typename T, int V, int L, int R>
 __global__ __launch_bounds__(256) void k_ssm_step(SsmArgs p) {
     const int lane = threadIdx.x % L, n0 = lane * V, N = (int)p.N, D = (int)p.D;

@@ -1017,7 +1017,7 @@ def add2(a, b, out) -> None:
 # Sequences are time-major [T, B, channels]; a batch-major tensor is passed as its transpose(0, 1), the halves of a
 # projection as slices: any strides, as long as the channels are contiguous. Inputs, outputs and their gradients are all
 # fp32 or all bf16; parameters, their gradients, states of the scan and statistics are fp32. Outputs are written whole and
-# may not share memory with an input. Scratch (``*_ws``) belongs to the caller: calls that may run at the same time (two
+# may share no byte with an input or another output (refused; slices of one buffer that interleave do not). Scratch (``*_ws``) belongs to the caller: calls that may run at the same time (two
 # streams, two graphs) need one each.
 _NORM, _CONV, _SSM = (struct.Struct("<%dq" % n) for n in (18, 29, 56))
 _NORM_FWD, _CONV_FWD, _SSM_FWD = (struct.Struct("<%dq%dx" % (n, 8 * m)) for n, m in ((10, 8), (17, 12), (33, 23)))        # the rest zero
@@ -1344,7 +1344,8 @@ def ssm_scan_fwd(u, dt, A, Bm, Cm, y, ws, D=None, z=None, dt_bias=None, h0=None,
         y = (sum_n Cm h + D u) silu(z)             Cm [T, B, N]; D fp32 [D] and z [T, B, D] are optional
 
     ``h0`` / ``hT`` [B, D, N] fp32: state before the first and after the last step (None: zeros / not kept). ``reset`` uint8
-    [T, B]: a non-zero flag starts step t from h = 0. ``lengths`` int32 [B]: steps from lengths[b] on are padding: not read,
+    [T, B]: a non-zero flag starts step t from h = 0, whatever came before it, and lets no gradient back. A step of size -inf (or
+    the lowest value) before softplus has s = 0 and holds the state. ``lengths`` int32 [B]: steps from lengths[b] on are padding: not read,
     zero in y, and hT is the state after step lengths[b] - 1. ``ckpt`` (:func:`ssm_scan_ckpt`) keeps what
     :func:`ssm_scan_bwd` needs; ``ws`` from :func:`ssm_scan_ws`."""
     if u is None or dt is None or A is None or Bm is None or Cm is None or y is None or ws is None:
